@@ -764,7 +764,6 @@ conv3x3_c8w4_kernel(const Wino4Args a) {
         W4_STAMP(6);                                       // stores acknowledged
         if (tid == 0) a.dbg[(size_t)blockIdx.x * 128 + 7] = ((unsigned long long)__builtin_amdgcn_s_getreg(20 | (31 << 11)) << 32) |
                                                            (unsigned)__builtin_amdgcn_s_getreg(4 | (31 << 11));      // XCC_ID, HW_ID
-        asm volatile("s_dcache_wb" ::: "memory");
     }
 #endif
 }

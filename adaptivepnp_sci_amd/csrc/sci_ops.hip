@@ -669,9 +669,10 @@ __device__ __forceinline__ unsigned bit_select(unsigned mask, float a, unsigned 
     do {                                                                                                                \
         if (stamps) {                                                                                                   \
             unsigned long long t_;                                                                                      \
-            const unsigned long long* p_ = stamps + (slot);                                                             \
+            unsigned long long* p_ = const_cast<unsigned long long*>(stamps + (slot));                                        \
             __builtin_amdgcn_sched_barrier(0);                                                                          \
-            asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t_) : "s"(p_) : "memory"); \
+            asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(t_) : : "memory");                              \
+            if ((threadIdx.x & 63) == 0) *(volatile unsigned long long*)p_ = t_;                                        \
             __builtin_amdgcn_sched_barrier(0);                                                                          \
         }                                                                                                               \
     } while (0)
@@ -778,9 +779,6 @@ pm_dual_project_spec_kernel(const TvCandidates cd, double tv_weight, double tv_e
     DPS_STAMP(5);
     DPS_WAIT_VM();
     DPS_STAMP(6);                 // stores acknowledged
-#if defined(SCIPNP_TV_STAMPS) && defined(__HIP_DEVICE_COMPILE__)
-    if (stamps) asm volatile("s_dcache_wb" ::: "memory");
-#endif
 }
 
 // launch shape of pm_dual_project_kernel: pixels per thread, chunks per workgroup (more than one only where one workgroup per

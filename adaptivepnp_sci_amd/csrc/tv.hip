@@ -652,9 +652,10 @@ __device__ __forceinline__ void tv_band_run(const float* xc, const float* bc, fl
     do {                                                                                                                \
         if (stamps) {                                                                                                   \
             unsigned long long t_;                                                                                      \
-            const unsigned long long* p_ = stamps + (slot);                                                             \
+            unsigned long long* p_ = const_cast<unsigned long long*>(stamps + (slot));                                        \
             __builtin_amdgcn_sched_barrier(0);                                                                          \
-            asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t_) : "s"(p_) : "memory"); \
+            asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(t_) : : "memory");                              \
+            if ((threadIdx.x & 63) == 0) *(volatile unsigned long long*)p_ = t_;                                        \
             __builtin_amdgcn_sched_barrier(0);                                                                          \
         }                                                                                                               \
     } while (0)
@@ -662,8 +663,9 @@ __device__ __forceinline__ void tv_band_run(const float* xc, const float* bc, fl
     do {                                                                                                                \
         if (stamps) {                                                                                                   \
             unsigned long long t_;                                                                                      \
-            const unsigned long long* p_ = stamps + (slot);                                                             \
-            asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t_) : "s"(p_) : "memory"); \
+            unsigned long long* p_ = const_cast<unsigned long long*>(stamps + (slot));                                        \
+            asm volatile("s_memrealtime %0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(t_) : : "memory");                          \
+            if ((threadIdx.x & 63) == 0) *(volatile unsigned long long*)p_ = t_;                                        \
         }                                                                                                               \
     } while (0)
 #else
@@ -850,9 +852,6 @@ __device__ __forceinline__ void tv_band_run2(const float* xc, const float* bc, f
     }
     TVB_STAMP(53);
     TVB_REALTIME(61);
-#if defined(SCIPNP_TV_STAMPS) && defined(__HIP_DEVICE_COMPILE__)
-    if (stamps) asm volatile("s_dcache_wb" ::: "memory");      // (the scalar data cache is not written back at the end of a kernel)
-#endif
 }
 
 template <int COLS, int R, int STRIPS, int V2, typename... A>      // V2: 0 round-2 schedule, 1 round 5, 2 round 5 with N == COLS

@@ -112,16 +112,17 @@ __host__ __device__ __forceinline__ f32x2 splat<f32x2>(float v) { return f32x2{v
 template <>
 __host__ __device__ __forceinline__ f32x4 splat<f32x4>(float v) { return f32x4{v, v, v, v}; }
 
-// one clock stamp of wave 0, written with a SCALAR store (no vmcnt traffic: the K loop's waits count vector memory operations)
+// one clock stamp of wave 0, written by its first lane (the store counts in vmcnt: the K loop's counted waits only get stricter)
 #if defined(__HIP_DEVICE_COMPILE__)
 #define W4_STAMP(slot)                                                                                              \
     do {                                                                                                            \
         if constexpr ((DIAG & 64) != 0) {                                                                           \
             if (wvu == 0) {                                                                                         \
                 unsigned long long t_;                                                                              \
-                const unsigned long long* p_ = stamp_base + (slot);                                                 \
+                unsigned long long* p_ = const_cast<unsigned long long*>(stamp_base + (slot));                            \
                 __builtin_amdgcn_sched_barrier(0);                                                                  \
-                asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t_) : "s"(p_) : "memory"); \
+                asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(t_) : : "memory");                          \
+                if ((threadIdx.x & 63) == 0) *(volatile unsigned long long*)p_ = t_;                                    \
                 __builtin_amdgcn_sched_barrier(0);                                                                  \
             }                                                                                                       \
         }                                                                                                           \

@@ -59,9 +59,10 @@ conv3x3_c8wp_kernel(const Wino4Args a) {
         if constexpr ((DIAG & 64) != 0) {                                                                           \
             if (wvu == (wave)) {                                                                                    \
                 unsigned long long t_;                                                                              \
-                const unsigned long long* p_ = stamp_base + (slot);                                                 \
+                unsigned long long* p_ = const_cast<unsigned long long*>(stamp_base + (slot));                            \
                 __builtin_amdgcn_sched_barrier(0);                                                                  \
-                asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t_) : "s"(p_) : "memory"); \
+                asm volatile("s_memtime %0\n\ts_waitcnt lgkmcnt(0)" : "=&s"(t_) : : "memory");                          \
+                if ((threadIdx.x & 63) == 0) *(volatile unsigned long long*)p_ = t_;                                    \
                 __builtin_amdgcn_sched_barrier(0);                                                                  \
             }                                                                                                       \
         }                                                                                                           \
@@ -418,7 +419,6 @@ conv3x3_c8wp_kernel(const Wino4Args a) {
         WP_STAMP(0, 6);
         if (tid == 0) a.dbg[(size_t)blockIdx.x * 128 + 7] = ((unsigned long long)__builtin_amdgcn_s_getreg(20 | (31 << 11)) << 32) |
                                                            (unsigned)__builtin_amdgcn_s_getreg(4 | (31 << 11));
-        asm volatile("s_dcache_wb" ::: "memory");
     }
 #endif
 }

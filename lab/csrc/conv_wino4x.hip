@@ -475,7 +475,6 @@ conv3x3_c8w6_kernel(const Wino4Args a) {
         W4_STAMP(6);
         if (tid == 0) a.dbg[(size_t)blockIdx.x * 128 + 7] = ((unsigned long long)__builtin_amdgcn_s_getreg(20 | (31 << 11)) << 32) |
                                                            (unsigned)__builtin_amdgcn_s_getreg(4 | (31 << 11));
-        asm volatile("s_dcache_wb" ::: "memory");
     }
 #endif
 }
