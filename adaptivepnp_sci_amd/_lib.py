@@ -114,6 +114,14 @@ SIGNATURES = {
     'scipnp_ddnet_gather_bwd': (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int, C.POINTER(_int), _vp]),
     'scipnp_bilinear_up2_bwd_c8': (_int, [_vp, _vp, _int, _int, _int, _vp]),
     'scipnp_ffdnet_forward': (_int, [_vp, _vp, C.POINTER(_vp), _int, _int, _vp, _vp, _int, _int, _int, _vp]),
+    'scipnp_head_norm_rotate': (_int, [_vp, _vp]),
+    'scipnp_head_norm_rotate_backward_workspace_bytes': (_sz, [_vp]),
+    'scipnp_head_norm_rotate_backward': (_int, [_vp, _vp]),
+    'scipnp_block_summary': (_int, [_vp, _vp, _int, _vp, _vp] + [_int] * 6 + [_vp]),
+    'scipnp_select_blocks': (_int, [_vp, _vp]),
+    'scipnp_block_attn_workspace_bytes': (_sz, [_vp, _int]),
+    'scipnp_block_attn': (_int, [_vp, _vp]),
+    'scipnp_block_attn_backward': (_int, [_vp, _vp]),
     'scipnp_host_legacy_normal': (_int, [_vp, C.POINTER(_int), C.POINTER(_int), C.POINTER(C.c_double), C.c_double, C.c_double,
                                         _vp, _sz]),
     'scipnp_twostage_ffdnet_iterate': (_int, [_vp, C.POINTER(_int), _vp]),
@@ -173,6 +181,45 @@ class TwoStageFfdnetArgs(C.Structure):
                 ('overflow_word', C.c_void_p), ('side_stream', C.c_void_p),
                 ('side_fork_event', C.c_void_p), ('side_join_event', C.c_void_p), ('packed_wino4', C.c_void_p),
                 ('units', C.c_int), ('conv_form', C.c_int)]
+
+    def __init__(self, **kw):
+        super().__init__(C.sizeof(type(self)), **kw)
+
+
+_st3 = C.c_int64 * 3
+
+
+class HeadNormArgs(C.Structure):
+    """scipnp_head_norm_args of include/scipnp.h"""
+    _fields_ = ([('struct_size', C.c_size_t)] + [(n, C.c_int) for n in ('dtype', 'B', 'L', 'Hq', 'Hk', 'D', 'rot', 'first', 'Lout')]
+                + [('eps', C.c_float)] + [(n, C.c_void_p) for n in ('q', 'k', 'v', 'out_q', 'out_k', 'out_v', 'g_q', 'g_k', 'dwq', 'dwk')]
+                + [(n + '_stride', _st3) for n in ('q', 'k', 'v', 'out_q', 'out_k', 'out_v', 'g_q', 'g_k')]
+                + [(n, C.c_void_p) for n in ('wq', 'wk', 'turns', 'positions', 'slots', 'workspace')] + [('workspace_bytes', C.c_size_t)])
+
+    def __init__(self, **kw):
+        super().__init__(C.sizeof(type(self)), **kw)
+
+
+class SelectArgs(C.Structure):
+    """scipnp_select_args of include/scipnp.h"""
+    _fields_ = ([('struct_size', C.c_size_t)]
+                + [(n, C.c_int) for n in ('dtype', 'B', 'Lq', 'Lk', 'Hq', 'Hk', 'D', 'block', 'query_block', 'n_sel', 'sink', 'local', 'causal')]
+                + [('q', C.c_void_p), ('q_stride', _st3)] + [(n, C.c_void_p) for n in ('summary', 'qlen', 'klen', 'sel')])
+
+    def __init__(self, **kw):
+        super().__init__(C.sizeof(type(self)), **kw)
+
+
+class BlockAttnArgs(C.Structure):
+    """scipnp_block_attn_args of include/scipnp.h"""
+    _fields_ = ([('struct_size', C.c_size_t)]
+                + [(n, C.c_int) for n in ('dtype', 'B', 'Lq', 'Lk', 'Hq', 'Hk', 'D', 'block', 'query_block', 'n_sel', 'causal', 'num_buckets',
+                                          'max_distance')]
+                + [('scale', C.c_float)] + [(n, C.c_void_p) for n in ('q', 'k', 'v', 'out')]
+                + [(n + '_stride', _st3) for n in ('q', 'k', 'v', 'out')]
+                + [(n, C.c_void_p) for n in ('sel', 'qlen', 'klen', 'bucket_of', 'q_pos', 'k_pos', 'bias', 'lse', 'out32', 'dout')]
+                + [('dout_stride', _st3)] + [(n, C.c_void_p) for n in ('dq', 'dk', 'dv', 'dbias', 'workspace')]
+                + [('workspace_bytes', C.c_size_t)])
 
     def __init__(self, **kw):
         super().__init__(C.sizeof(type(self)), **kw)

@@ -20,7 +20,7 @@
  *           c8s    [n][C/8][2][h][w][8]  fp16: the same tensor as an error-compensated pair of planes, v = hi + lo'/2048
  *                  (hi = fp16(v), lo' = fp16((v - hi)*2048)), the operand format of the split-fp16 MFMA convolutions.
  *
- * Each entry cites the reference code it replaces (paths relative to the reference repository).
+ * Each entry that replaces reference code cites it (paths relative to the reference repository).
  */
 #ifndef SCIPNP_H
 #define SCIPNP_H
@@ -697,6 +697,89 @@ int scipnp_ddnet_gather_bwd(const float* d_tin_c8, const float* d_center, int Cd
                             const float* scale, float* d_src, double* part, int E, int Bn, int C, int h, int w, int* ncols,
                             scipnp_stream_t s);
 int scipnp_bilinear_up2_bwd_c8(const float* d_up_c8, float* d_in, int E, int h, int w, scipnp_stream_t s);
+
+/* -------------------------------------------------------------------------------------------------------------
+ * Non-local attention over selected blocks (adaptivepnp_sci_amd/attention.py).
+ *
+ * Tokens: q (B, Lq, Hq, D), k, v (B, Lk, Hk, D), Hq a multiple of Hk (G = Hq / Hk query heads read one key head), last dimension
+ * contiguous, element strides of batch, token and head free (multiples of 16 bytes; pointers 16-byte aligned).  dtype:
+ * SCIPNP_F32 (every product an exact fp32 product) or SCIPNP_BF16; sums, softmax statistics and states are fp32 or fp64.
+ * Sequence b has qlen[b] live queries and klen[b] live keys (NULL: all); query i stands at key position klen - qlen + i.
+ * Rows behind qlen are not written, keys behind klen are not read.  query_block neighbouring queries and the G heads of a key
+ * head choose key blocks together: sel int32 (B, Hk, ceil(Lq / query_block), n_sel), ascending, -1 behind the last; an entry
+ * that is outside the blocks or not greater than every entry before it is ignored.
+ * ------------------------------------------------------------------------------------------------------------- */
+#define SCIPNP_F32 0
+#define SCIPNP_BF16 1
+
+/* norm of every head with its learned weight, and the rotation by the token's position, one pass:
+ *   n = x / sqrt(mean(x^2) + eps) * w;  (n_i, n_{i+rot/2}) turned by positions * turns[i] (turns of the circle per position, fp64)
+ * computed in fp64 and rounded once.  k / v may be NULL; v rows are copied.  slots (B, L) int32: the row of out_k / out_v that
+ * token l goes to (a cache; NULL: row l); a slot outside [0, Lout) drops the row.  positions (B, L) int32, NULL: first + l.
+ * backward: dx of x (in `out_*`), dw fp32 from the gradients g_q / g_k of the rotated heads (v, slots not used). */
+typedef struct {
+    size_t struct_size;                 /* = sizeof(scipnp_head_norm_args) */
+    int dtype, B, L, Hq, Hk, D, rot, first, Lout;
+    float eps;
+    const void *q, *k, *v;
+    void *out_q, *out_k, *out_v;
+    const void *g_q, *g_k;              /* backward */
+    float *dwq, *dwk;                   /* backward */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_q_stride[3], out_k_stride[3], out_v_stride[3], g_q_stride[3], g_k_stride[3];
+    const float *wq, *wk;
+    const double* turns;                /* rot / 2 */
+    const int32_t *positions, *slots;
+    void* workspace;                    /* backward */
+    size_t workspace_bytes;
+} scipnp_head_norm_args;
+int scipnp_head_norm_rotate(const scipnp_head_norm_args* a, scipnp_stream_t s);
+size_t scipnp_head_norm_rotate_backward_workspace_bytes(const scipnp_head_norm_args* a);
+int scipnp_head_norm_rotate_backward(const scipnp_head_norm_args* a, scipnp_stream_t s);
+
+/* mean key of every block over its live keys, summed in fp64: summary fp32 (B, ceil(Lk / block), Hk, D) contiguous, zeros for a
+ * block behind klen.  newest > 0: only the blocks that the last `newest` live keys touch are written (a growing cache). */
+int scipnp_block_summary(const void* k, const int64_t* k_stride, int dtype, const int32_t* klen, float* summary, int B, int Lk, int Hk,
+                         int D, int block, int newest, scipnp_stream_t s);
+
+/* the n_sel blocks of every group of query_block queries with the largest (sum of the group's queries) . (mean key of the block),
+ * in fp64; ties to the lower block, a NaN below every number.  Always among them: the `sink` first blocks and the `local` blocks
+ * around the block of the group's last query (before every score).  causal: no block that starts behind the last query. */
+typedef struct {
+    size_t struct_size;                 /* = sizeof(scipnp_select_args) */
+    int dtype, B, Lq, Lk, Hq, Hk, D, block, query_block, n_sel, sink, local, causal;
+    const void* q;
+    int64_t q_stride[3];
+    const float* summary;               /* (B, ceil(Lk / block), Hk, D) */
+    const int32_t *qlen, *klen;
+    int32_t* sel;
+} scipnp_select_args;
+int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s);
+
+/* softmax(scale * q . k + bias[bucket_of[clamp(kpos - qpos, +-max_distance) + max_distance]][head]) v over the selected blocks.
+ * causal: keys behind the query's position are masked.  bias fp32 (num_buckets, Hq) (NULL: none), bucket_of int32
+ * (2 * max_distance + 1), q_pos (B, Lq) / k_pos (B, Lk) int32 (NULL: the key positions of query and key).  A row without a key:
+ * zeros, lse = -inf.  lse fp32 (B, Hq, Lq) and out32 fp32 (B, Lq, Hq, D) (the unrounded result) are written when given; the
+ * backward pass reads them.  backward: dq, dk, dv in dtype, dbias fp32; every row is written (zeros behind qlen / klen). */
+typedef struct {
+    size_t struct_size;                 /* = sizeof(scipnp_block_attn_args) */
+    int dtype, B, Lq, Lk, Hq, Hk, D, block, query_block, n_sel, causal, num_buckets, max_distance;
+    float scale;
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+    const int32_t *sel, *qlen, *klen, *bucket_of, *q_pos, *k_pos;
+    const float* bias;
+    float *lse, *out32;
+    const void* dout;                   /* backward: dout and the gradients; dq (B, Lq, Hq, D), dk / dv (B, Lk, Hk, D) contiguous */
+    int64_t dout_stride[3];
+    void *dq, *dk, *dv;
+    float* dbias;
+    void* workspace;
+    size_t workspace_bytes;
+} scipnp_block_attn_args;
+size_t scipnp_block_attn_workspace_bytes(const scipnp_block_attn_args* a, int backward);
+int scipnp_block_attn(const scipnp_block_attn_args* a, scipnp_stream_t s);
+int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t s);
 
 /* HOST function (no GPU involved): n deviates of NumPy's LEGACY normal stream -- np.random.normal(loc, scale, n) on the
  * global RandomState, bit for bit -- from / to a generator state in np.random.get_state() form (key[624], pos,
