@@ -75,9 +75,10 @@ struct Select {
     const int32_t *qlen, *klen;
     int32_t* sel;
     int B, Lq, Lk, Hq, Hk, D, block, qb, n, sink, local, causal, nb, ng;
+    int gpw, tiles, spare;                                // groups of a workgroup, workgroups of a (sequence, key head), LDS words behind the keys
 };
 
-constexpr int SEL_MAX_BLOCKS = 8192;
+constexpr int SEL_MAX_BLOCKS = 8192;                      // 64 KB of scores
 
 // A double as a whole number of the same order: NaN lowest (1), 0 is free for "not a candidate"
 __device__ __forceinline__ unsigned long long order_key(double v) {
@@ -86,143 +87,163 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-// the keys of 0 .. nb-1 are in LDS (0: no candidate): writes the n best of them, ascending; ties to the lower index.
-// Radix selection from the top byte: at most 8 counting passes, none once a byte's bucket is taken whole.
-__device__ void select_best(const unsigned long long* keys, int nb, int n, int32_t* out, int* hist /* 256 + 16 */) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int* const misc = hist + 256;
+// the keys of 0 .. nb-1 are in LDS (0: no candidate): one wave writes the n best of them, ascending; ties to the lower index.
+// Radix selection from the top byte over a histogram of its own: at most 8 counting passes, none once a byte's bucket is taken whole
+// (scores that differ in their first 20 bits need three).
+__device__ void select_best(const unsigned long long* keys, int nb, int n, int32_t* out, int* hist, int lane) {
     int cand = 0;
-    for (int j = tid; j < nb; j += 256) cand += keys[j] != 0;
-    if (tid == 0) misc[0] = 0;
-    __syncthreads();
-    if (cand) atomicAdd(&misc[0], cand);                   // (a count: the order of the additions does not matter)
-    __syncthreads();
-    const int total = misc[0];
+    for (int base = 0; base < nb; base += 64) cand += __popcll(__ballot(base + lane < nb && keys[base + lane] != 0));
     unsigned long long prefix = 0, mask = 0;               // the threshold's known upper bytes
-    int need = min(n, total);                              // still to take among the keys with that prefix
-    bool all = need == total;                              // take every key with the prefix (and every greater one)
+    int need = min(n, cand);                               // still to take among the keys with that prefix
+    bool all = need == cand;                               // take every key with the prefix (and every greater one)
     for (int shift = 56; shift >= 0 && !all; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < nb; j += 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hist[lane + 64 * i] = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int j = lane; j < nb; j += 64) {
             const unsigned long long k = keys[j];
-            if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+            if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);      // (counts: no order)
         }
-        __syncthreads();
-        // suffix sums over the 256 counts (from the greatest byte): one wave, four counts a lane
-        if (wave == 0) {
-            int c[4], s = 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // sums from the greatest byte down, four counts a lane
+        int c[4], s = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; s += c[i]; }
-            int incl = s;
-            for (int off = 1; off < 64; off <<= 1) {
-                const int o = __shfl_up(incl, off, 64);
-                if (lane >= off) incl += o;
-            }
-            int before = incl - s;
+        for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; s += c[i]; }
+        int incl = s;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (before < need && before + c[i] >= need) {          // exactly one lane and count
-                    misc[1] = 255 - (4 * lane + i);
-                    misc[2] = need - before;
-                    misc[3] = c[i];
-                }
-                before += c[i];
-            }
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(incl, off, 64);
+            if (lane >= off) incl += o;
         }
-        __syncthreads();
-        prefix |= (unsigned long long)misc[1] << shift;
+        int before = incl - s, byte = -1, rest = 0, have = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (before < need && before + c[i] >= need) { byte = 255 - (4 * lane + i); rest = need - before; have = c[i]; }
+            before += c[i];
+        }
+        const int src = __ffsll((unsigned long long)__ballot(byte >= 0)) - 1;                      // exactly one lane has it
+        prefix |= (unsigned long long)__shfl(byte, src, 64) << shift;
         mask |= 255ull << shift;
-        need = misc[2];
-        all = need == misc[3];
+        need = __shfl(rest, src, 64);
+        all = need == __shfl(have, src, 64);
     }
-    // greater than the prefix: in; equal: the first `need` of them; written in order of the index
-    if (tid == 0) { misc[4] = 0; misc[5] = 0; }
-    __syncthreads();
-    for (int base = 0; base < nb; base += 256) {
-        const int j = base + tid;
-        const unsigned long long k = j < nb ? keys[j] : 0;
+    // greater than the prefix: in; equal: the first `need` of them
+    int eqs = 0, at = 0;
+    for (int base = 0; base < nb; base += 64) {
+        const int j = base + lane;
+        const unsigned long long k = j < nb ? keys[j] : 0, below = (1ull << lane) - 1;
         const bool eq = k != 0 && (k & mask) == prefix, gt = k != 0 && (k & mask) > prefix;
         const unsigned long long be = __ballot(eq);
-        if (lane == 0) misc[8 + wave] = __popcll(be);
-        __syncthreads();
-        int eq_before = misc[4] + __popcll(be & ((1ull << lane) - 1));
-        for (int w = 0; w < wave; ++w) eq_before += misc[8 + w];
-        const bool in = gt || (eq && (all || eq_before < need));
+        const bool in = gt || (eq && (all || eqs + __popcll(be & below) < need));
         const unsigned long long bi = __ballot(in);
-        if (lane == 0) misc[12 + wave] = __popcll(bi);
-        __syncthreads();
-        int at = misc[5] + __popcll(bi & ((1ull << lane) - 1));
-        for (int w = 0; w < wave; ++w) at += misc[12 + w];
-        if (in && at < n) out[at] = j;
-        __syncthreads();
-        if (tid == 0)
-            for (int w = 0; w < 4; ++w) { misc[4] += misc[8 + w]; misc[5] += misc[12 + w]; }
-        __syncthreads();
+        if (in) out[at + __popcll(bi & below)] = j;
+        eqs += __popcll(be);
+        at += __popcll(bi);
     }
-    for (int i = misc[5] + tid; i < n; i += 256) out[i] = -1;
+    for (int i = at + lane; i < n; i += 64) out[i] = -1;
+}
+
+// One workgroup of eight waves: up to 16 query groups of one (sequence, key head) -- as many as have room for their scores in LDS.
+//   1. a wave sums the queries of one group (16 bytes a lane, the parts of its rows added in order);
+//   2. the scores of 16 blocks x 16 groups at a time on the fp64 matrix unit (v_mfma_f64_16x16x4_f64: lane -> row lane & 15,
+//      contraction lane >> 4; result register r: row 4 r + (lane >> 4), column lane & 15): a mean key is read once for all groups;
+//   3. a wave chooses the blocks of one group.
+typedef double f64x4a __attribute__((ext_vector_type(4)));
+constexpr int SEL_WAVES = 8;
+
+template <typename T, int ND>                              // ND * 16 >= D
+__global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int E = 16 / sizeof(T);
+    extern __shared__ __attribute__((aligned(16))) char smem_s[];
+    const int qst = a.D + 2;                               // (rows two banks apart)
+    double* const qs = (double*)smem_s;                    // [groups][qst]
+    unsigned long long* const keys = (unsigned long long*)(qs + a.gpw * qst);      // [groups][nb]; before that the parts of step 1
+    int* const hists = (int*)(keys + (size_t)a.gpw * a.nb + a.spare);
+    const long long total = (long long)a.B * a.Hk * a.tiles, item = xcd_item(blockIdx.x, total);
+    if (item < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g0 = (int)(item % a.tiles) * a.gpw, bh = (int)(item / a.tiles), hk = bh % a.Hk, b = bh / a.Hk;
+    const int ngr = min(a.gpw, a.ng - g0);
+    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Lq) : a.Lq, klen = a.klen ? min(max(a.klen[b], 0), a.Lk) : a.Lk;
+    const int G = a.Hq / a.Hk, nc = a.D / E, parts = 64 / nc;
+    for (int i = wave; i < a.gpw; i += SEL_WAVES) {
+        const int q0 = (g0 + i) * a.qb, rows = i < ngr ? min(a.qb, qlen - q0) * G : 0;
+        const int c = lane % nc, part = lane / nc;         // (D <= 256: at most 64 pieces of a row)
+        double s[E] = {};
+        if (part < parts) {
+            const T* base = (const T*)a.q + b * a.sq.b + c * E;
+#pragma unroll 4
+            for (int r = part; r < rows; r += parts) {
+                __attribute__((aligned(16))) T v[E];
+                *(f32x4a*)v = *(const f32x4a*)(base + (long long)(q0 + r / G) * a.sq.t + (hk * G + r % G) * a.sq.h);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[e] += (double)(float)v[e];
+            }
+        }
+        double* const mine = (double*)keys + (size_t)wave * 64 * E;        // (the keys come later)
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine[lane * E + e] = s[e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int d = lane; d < a.D; d += 64) {
+            double v = 0.0;
+            for (int p = 0; p < parts; ++p) v += mine[(p * nc + d / E) * E + d % E];
+            qs[i * qst + d] = v;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    // key position of the group's last query (this lane's column), and what the tile's last group may see
+    const int col = lane & 15, kq = lane >> 4, gc = g0 + col;
+    const bool group = col < ngr && gc * a.qb < qlen;
+    const int last = klen - qlen + min((gc + 1) * a.qb, qlen) - 1;
+    const int own = last >= 0 ? last / a.block : (last - a.block + 1) / a.block;
+    const int nt = (a.nb + 15) / 16;
+    const double* const qrow = qs + (col < a.gpw ? col : 0) * qst + 4 * kq;
+    for (int jt = wave; jt < nt; jt += SEL_WAVES) {
+        const int j = jt * 16 + col;                       // (A's row)
+        f32x4a m[ND];
+        const float* const row = a.summary + (((size_t)b * a.nb + (j < a.nb ? j : 0)) * a.Hk + hk) * a.D + 4 * kq;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) m[d] = j < a.nb && 16 * d + 4 * kq < a.D ? *(const f32x4a*)(row + 16 * d) : f32x4a{0.f, 0.f, 0.f, 0.f};
+        f64x4a s0 = {0.0, 0.0, 0.0, 0.0}, s1 = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            double q[4] = {0.0, 0.0, 0.0, 0.0};
+            if (16 * d + 4 * kq < a.D)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = qrow[16 * d + e];
+            s0 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][0], q[0], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][1], q[1], s1, 0, 0, 0);
+            s0 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][2], q[2], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][3], q[3], s1, 0, 0, 0);
+        }
+        if (col < a.gpw)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int jj = jt * 16 + 4 * r + kq;
+                if (jj >= a.nb) continue;
+                const bool may = group && (long long)jj * a.block < klen && (!a.causal || (long long)jj * a.block <= last);
+                const bool must = jj < a.sink || abs(jj - own) < a.local;
+                keys[(size_t)col * a.nb + jj] = !may ? 0 : must ? ~0ull : order_key(s0[r] + s1[r]);
+            }
+    }
+    __syncthreads();
+    for (int i = wave; i < ngr; i += SEL_WAVES)
+        select_best(keys + (size_t)i * a.nb, a.nb, a.n, a.sel + ((size_t)bh * a.ng + g0 + i) * a.n, hists + wave * 256, lane);
+#endif
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) select_blocks_kernel(Select a) {
-    extern __shared__ __attribute__((aligned(16))) char smem_s[];
-    double* const qs = (double*)smem_s;                                    // [D], then 256 more of scratch
-    double* const red = qs + a.D;
-    int* const hist = (int*)(red + 256);
-    unsigned long long* const keys = (unsigned long long*)(hist + 256 + 16);
-    const long long total = (long long)a.B * a.Hk * a.ng, item = xcd_item(blockIdx.x, total);
-    if (item < 0) return;
-    const int g = (int)(item % a.ng), bh = (int)(item / a.ng), hk = bh % a.Hk, b = bh / a.Hk;
-    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Lq) : a.Lq, klen = a.klen ? min(max(a.klen[b], 0), a.Lk) : a.Lk;
-    int32_t* const out = a.sel + (size_t)item * a.n;
-    const int q0 = g * a.qb, nq = min(a.qb, qlen - q0);
-    if (nq <= 0) {                                                         // (uniform: the whole workgroup leaves)
-        for (int i = threadIdx.x; i < a.n; i += 256) out[i] = -1;
-        return;
-    }
-    // the group's summed queries: thread = (dimension, part of the rows), the parts added in order
-    const int G = a.Hq / a.Hk, rows = nq * G, parts = max(1, 256 / a.D);
-    {
-        const int d = threadIdx.x % a.D, part = threadIdx.x / a.D;
-        double s = 0.0;
-        if (part < parts)
-            for (int r = part; r < rows; r += parts)
-                s += (double)(float)((const T*)a.q)[b * a.sq.b + (long long)(q0 + r / G) * a.sq.t + (hk * G + r % G) * a.sq.h + d];
-        red[threadIdx.x] = s;
-        __syncthreads();
-        if (threadIdx.x < a.D) {
-            for (int p = 1; p < parts; ++p) s += red[p * a.D + threadIdx.x];
-            qs[threadIdx.x] = s;
-        }
-        __syncthreads();
-    }
-    const int last = klen - qlen + q0 + nq - 1;                            // key position of the group's last query
-    const int own = last >= 0 ? last / a.block : (last - a.block + 1) / a.block;
-    // 16 lanes a block
-    const int l16 = threadIdx.x & 15;
-    for (int base = 0; base < a.nb; base += 16) {
-        const int j = base + (threadIdx.x >> 4);
-        const bool may = j < a.nb && (long long)j * a.block < klen && (!a.causal || (long long)j * a.block <= last);
-        double s = 0.0;
-        if (may) {
-            const float* m = a.summary + (((size_t)b * a.nb + j) * a.Hk + hk) * a.D;
-            for (int d = 4 * l16; d < a.D; d += 64) {
-                const f32x4a v = *(const f32x4a*)(m + d);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s += qs[d + e] * (double)v[e];
-            }
-        }
-        s += dpp_f64<0xB1>(s);
-        s += dpp_f64<0x4E>(s);
-        s += dpp_f64<0x141>(s);
-        s += dpp_f64<0x140>(s);
-        if (l16 == 0 && j < a.nb) {
-            const bool must = j < a.sink || abs(j - own) < a.local;
-            keys[j] = !may ? 0 : must ? ~0ull : order_key(s);
-        }
-    }
-    __syncthreads();
-    select_best(keys, a.nb, a.n, out, hist);
+static int select_launch(const Select& p, size_t lds, unsigned grid, hipStream_t st) {
+    static LdsAttrOnce once[3];
+    const int v = p.D <= 64 ? 0 : p.D <= 128 ? 1 : 2;
+    const void* fn = v == 0 ? (const void*)select_blocks_kernel<T, 4> : v == 1 ? (const void*)select_blocks_kernel<T, 8> : (const void*)select_blocks_kernel<T, 16>;
+    if (const int rc = once[v].ensure(fn, 163840, "select_blocks")) return rc;
+    if (v == 0) select_blocks_kernel<T, 4><<<grid, 64 * SEL_WAVES, lds, st>>>(p);
+    else if (v == 1) select_blocks_kernel<T, 8><<<grid, 64 * SEL_WAVES, lds, st>>>(p);
+    else select_blocks_kernel<T, 16><<<grid, 64 * SEL_WAVES, lds, st>>>(p);
+    return launch_status("scipnp_select_blocks");
 }
 
 }  // namespace scipnp
@@ -277,15 +298,17 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s) {
     p.B = a->B; p.Lq = a->Lq; p.Lk = a->Lk; p.Hq = a->Hq; p.Hk = a->Hk; p.D = a->D; p.block = a->block; p.qb = a->query_block;
     p.n = a->n_sel; p.sink = a->sink; p.local = a->local; p.causal = a->causal;
     p.ng = (a->Lq + a->query_block - 1) / a->query_block;
-    const long long items = (long long)a->B * a->Hk * p.ng;
-    SCIPNP_REQUIRE(items < (1ll << 30), "too many query groups");
-    const size_t lds = (size_t)(a->D + 256) * 8 + (256 + 16) * 4 + (size_t)p.nb * 8;
-    static LdsAttrOnce once[2];
-    const void* fn = a->dtype == SCIPNP_BF16 ? (const void*)select_blocks_kernel<__bf16> : (const void*)select_blocks_kernel<float>;
-    if (const int rc = once[a->dtype == SCIPNP_BF16].ensure(fn, (size_t)(256 + 256) * 8 + (256 + 16) * 4 + (size_t)SEL_MAX_BLOCKS * 8, "select_blocks")) return rc;
-    if (a->dtype == SCIPNP_BF16) select_blocks_kernel<__bf16><<<xcd_grid(items), 256, lds, (hipStream_t)s>>>(p);
-    else select_blocks_kernel<float><<<xcd_grid(items), 256, lds, (hipStream_t)s>>>(p);
-    return launch_status("scipnp_select_blocks");
+    // groups of a workgroup: up to 16 (the columns of a matrix instruction) with at most 64 KB of scores, two workgroups a CU
+    p.gpw = 65536 / (p.nb * 8);
+    p.gpw = p.gpw > 16 ? 16 : p.gpw < 1 ? 1 : p.gpw;
+    if (p.gpw > p.ng) p.gpw = p.ng;
+    p.tiles = (p.ng + p.gpw - 1) / p.gpw;
+    const int parts_words = SEL_WAVES * 64 * (16 / (int)attn_esize(a->dtype)), key_words = p.gpw * p.nb;
+    p.spare = parts_words > key_words ? parts_words - key_words : 0;
+    const long long items = (long long)a->B * a->Hk * p.tiles;
+    SCIPNP_REQUIRE(items < (1ll << 22) && (long long)p.ng * a->query_block < (1ll << 30), "too many query groups");
+    const size_t lds = (size_t)p.gpw * (a->D + 2) * 8 + (size_t)(key_words + p.spare) * 8 + SEL_WAVES * 256 * 4;
+    return a->dtype == SCIPNP_BF16 ? select_launch<__bf16>(p, lds, xcd_grid(items), (hipStream_t)s) : select_launch<float>(p, lds, xcd_grid(items), (hipStream_t)s);
 }
 
 }
