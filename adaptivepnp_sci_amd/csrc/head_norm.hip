@@ -62,24 +62,57 @@ __device__ __forceinline__ double row_sum(double v) {
     return v;
 }
 
-// cosines and sines of `nt` tokens from token t0 on: cs[tok][pair] = (cos, sin)
-__device__ __forceinline__ void fill_angles(const HeadNorm& a, double2* cs, long long t0, int nt) {
+// 1 / sqrt(x): the hardware's estimate and two Newton steps (its 2^-23 and more squares twice); 0 and infinity keep the estimate
+__device__ __forceinline__ double rsqrt64(double x) {
+    const double e = __builtin_amdgcn_rsq(x);
+    double y = e * fma(-0.5 * x * e, e, 1.5);
+    y = y * fma(-0.5 * x * y, y, 1.5);
+    return y == y ? y : e;
+}
+
+// What the rows of a token share, once per workgroup in LDS: where its heads begin, and the cosines and sines of its position
+struct Token { long long q, k, v, oq, ok, ov, gq, gk; int keep, pad[3]; };
+struct NormLds {
+    Token* tok;
+    double2* cs;                                           // [token][pair] = (cos, sin)
+};
+__device__ __forceinline__ NormLds norm_lds(const HeadNorm& a, char* lds) { return NormLds{(Token*)lds, (double2*)(lds + a.TT * sizeof(Token))}; }
+__device__ __forceinline__ void fill_tokens(const HeadNorm& a, const NormLds& s, long long t0, int nt) {
     const int half = a.rot >> 1;
-    for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
-        const int tok = i / half, pair = i - tok * half;
-        const long long t = t0 + tok;
-        const int b = (int)(t / a.L), l = (int)(t - (long long)b * a.L);
-        const double pos = a.positions ? (double)a.positions[t] : (double)(a.first + (long long)l);
+    const int b0 = (int)(t0 / a.L), l0 = (int)(t0 - (long long)b0 * a.L);   // (uniform)
+    for (int i = threadIdx.x; i < nt; i += 256) {
+        int b = b0, l = l0 + i;
+        while (l >= a.L) { l -= a.L; ++b; }
+        const int row = a.slots ? a.slots[t0 + i] : l;
+        Token k;
+        k.keep = row >= 0 && row < a.Lout;
+        const long long r = k.keep ? row : 0;
+        k.q = b * a.sq.b + l * a.sq.t;
+        k.k = b * a.sk.b + l * a.sk.t;
+        k.v = b * a.sv.b + l * a.sv.t;
+        k.oq = b * a.soq.b + l * a.soq.t;
+        k.ok = b * a.sok.b + r * a.sok.t;
+        k.ov = b * a.sov.b + r * a.sov.t;
+        k.gq = b * a.sgq.b + l * a.sgq.t;
+        k.gk = b * a.sgk.b + l * a.sgk.t;
+        s.tok[i] = k;
+    }
+    for (int i = threadIdx.x; i < nt * half; i += 256) {
+        const int tok = nt == 1 ? 0 : i / half, pair = i - tok * half;
+        int l = l0 + tok;
+        while (l >= a.L) l -= a.L;
+        const double pos = a.positions ? (double)a.positions[t0 + tok] : (double)(a.first + (long long)l);
         const double turn = pos * a.turns[pair];
-        double s, c;
-        sincospi(2.0 * (turn - floor(turn)), &s, &c);
-        cs[i] = make_double2(c, s);
+        double sn, c;
+        sincospi(2.0 * (turn - floor(turn)), &sn, &c);
+        s.cs[i] = make_double2(c, sn);
     }
 }
 
 template <typename T, int LPR>
 __global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm a) {
-    extern __shared__ __attribute__((aligned(16))) double2 cs[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const NormLds s = norm_lds(a, lds);
     const int l = threadIdx.x % LPR, slot0 = threadIdx.x / LPR;
     constexpr int RPI = 256 / LPR;                        // rows per pass of the workgroup
     const long long tokens = (long long)a.B * a.L, t0 = (long long)blockIdx.x * a.TT;
@@ -94,30 +127,24 @@ __global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm a) {
         load4(a.wq + o1, w1q);
         if (a.Hk) { load4(a.wk + o0, w0k); load4(a.wk + o1, w1k); }
     }
-    if (half) {
-        fill_angles(a, cs, t0, nt);
-        __syncthreads();
-    }
-    for (int r = slot0; r < nt * heads; r += RPI) {       // (a row's LPR lanes share r: the sums below stay inside them)
-        const int tok = r / heads, hd = r - tok * heads;
-        const long long t = t0 + tok;
-        const int b = (int)(t / a.L), li = (int)(t - (long long)b * a.L);
+    fill_tokens(a, s, t0, nt);
+    __syncthreads();
+    int tok = 0, hd = slot0;                              // row = (token, head); its LPR lanes share it, so the sums stay inside them
+    while (hd >= heads) { hd -= heads; ++tok; }
+    while (tok < nt) {
         const bool is_q = hd < a.Hq, is_v = hd >= a.Hq + a.Hk;
         const int h = is_q ? hd : is_v ? hd - a.Hq - a.Hk : hd - a.Hq;
-        const Strides si = is_q ? a.sq : is_v ? a.sv : a.sk, so = is_q ? a.soq : is_v ? a.sov : a.sok;
-        const T* in = (const T*)(is_q ? a.q : is_v ? a.v : a.k) + b * si.b + li * si.t + h * si.h;
-        int row = li;
-        if (!is_q && a.slots) row = a.slots[t];
-        const bool keep = on && (is_q || (row >= 0 && row < a.Lout));
-        T* out = (T*)(is_q ? a.oq : is_v ? a.ov : a.ok) + b * so.b + (long long)(keep ? row : 0) * so.t + h * so.h;
+        const Token& k = s.tok[tok];
+        const T* in = (const T*)(is_q ? a.q : is_v ? a.v : a.k) + (is_q ? k.q : is_v ? k.v : k.k) + h * (is_q ? a.sq.h : is_v ? a.sv.h : a.sk.h);
+        T* out = (T*)(is_q ? a.oq : is_v ? a.ov : a.ok) + (is_q ? k.oq : is_v ? k.ov : k.ok) + h * (is_q ? a.soq.h : is_v ? a.sov.h : a.sok.h);
         double x0[4] = {}, x1[4] = {};
         if (on) { load4(in + o0, x0); load4(in + o1, x1); }
         if (!is_v) {
             double ss = 0.0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+            for (int i = 0; i < 4; ++i) ss = fma(x1[i], x1[i], fma(x0[i], x0[i], ss));
             ss = row_sum<LPR>(ss);
-            const double rs = 1.0 / sqrt(ss * a.inv_d + a.eps);
+            const double rs = rsqrt64(fma(ss, a.inv_d, a.eps));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x0[i] *= rs * (is_q ? w0q[i] : w0k[i]);
@@ -126,20 +153,23 @@ __global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm a) {
             if (turned) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const double2 c = cs[tok * half + 4 * l + i];
+                    const double2 c = s.cs[tok * half + 4 * l + i];
                     const double u = x0[i], v = x1[i];
-                    x0[i] = u * c.x - v * c.y;
-                    x1[i] = v * c.x + u * c.y;
+                    x0[i] = fma(u, c.x, -(v * c.y));
+                    x1[i] = fma(v, c.x, u * c.y);
                 }
             }
         }
-        if (keep) { store4(out + o0, x0); store4(out + o1, x1); }
+        if (on && (is_q || k.keep)) { store4(out + o0, x0); store4(out + o1, x1); }
+        hd += RPI;
+        while (hd >= heads) { hd -= heads; ++tok; }
     }
 }
 
 template <typename T, int LPR>
 __global__ void __launch_bounds__(256) head_norm_bwd_kernel(HeadNorm a) {
-    extern __shared__ __attribute__((aligned(16))) double2 cs[];      // angles of a tile, then (reused) the workgroup's dw
+    extern __shared__ __attribute__((aligned(16))) char lds[];        // the tile's tokens, then (reused) the workgroup's dw
+    const NormLds s = norm_lds(a, lds);
     const int l = threadIdx.x % LPR, slot0 = threadIdx.x / LPR;
     constexpr int RPI = 256 / LPR;
     const long long tokens = (long long)a.B * a.L, tiles = (tokens + a.TT - 1) / a.TT;
@@ -157,54 +187,56 @@ __global__ void __launch_bounds__(256) head_norm_bwd_kernel(HeadNorm a) {
     for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const long long t0 = tile * a.TT;
         const int nt = (int)min((long long)a.TT, tokens - t0);
-        if (half) {
-            __syncthreads();
-            fill_angles(a, cs, t0, nt);
-            __syncthreads();
-        }
-        for (int r = slot0; r < nt * heads; r += RPI) {
-            const int tok = r / heads, hd = r - tok * heads;
-            const long long t = t0 + tok;
-            const int b = (int)(t / a.L), li = (int)(t - (long long)b * a.L);
+        __syncthreads();
+        fill_tokens(a, s, t0, nt);
+        __syncthreads();
+        int tok = 0, hd = slot0;
+        while (hd >= heads) { hd -= heads; ++tok; }
+        while (tok < nt) {
             const bool is_q = hd < a.Hq;
             const int h = is_q ? hd : hd - a.Hq;
-            const Strides si = is_q ? a.sq : a.sk, sg = is_q ? a.sgq : a.sgk, so = is_q ? a.soq : a.sok;
-            const T* in = (const T*)(is_q ? a.q : a.k) + b * si.b + li * si.t + h * si.h;
-            const T* gin = (const T*)(is_q ? a.gq : a.gk) + b * sg.b + li * sg.t + h * sg.h;
-            T* out = (T*)(is_q ? a.oq : a.ok) + b * so.b + li * so.t + h * so.h;
+            const Token& k = s.tok[tok];
+            const T* in = (const T*)(is_q ? a.q : a.k) + (is_q ? k.q : k.k) + h * (is_q ? a.sq.h : a.sk.h);
+            const T* gin = (const T*)(is_q ? a.gq : a.gk) + (is_q ? k.gq : k.gk) + h * (is_q ? a.sgq.h : a.sgk.h);
+            T* out = (T*)(is_q ? a.oq : a.ok) + (is_q ? k.oq : k.ok) + h * (is_q ? a.soq.h : a.sok.h);
             double x0[4] = {}, x1[4] = {}, g0[4] = {}, g1[4] = {};
             if (on) { load4(in + o0, x0); load4(in + o1, x1); load4(gin + o0, g0); load4(gin + o1, g1); }
             if (turned) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const double2 c = cs[tok * half + 4 * l + i];
+                    const double2 c = s.cs[tok * half + 4 * l + i];
                     const double u = g0[i], v = g1[i];
-                    g0[i] = u * c.x + v * c.y;
-                    g1[i] = v * c.x - u * c.y;
+                    g0[i] = fma(u, c.x, v * c.y);
+                    g1[i] = fma(v, c.x, -(u * c.y));
                 }
             }
             double ss = 0.0, gx = 0.0;                    // sum x^2, sum g w x
+            double wg0[4], wg1[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                ss += x0[i] * x0[i] + x1[i] * x1[i];
-                gx += g0[i] * (is_q ? w0q[i] : w0k[i]) * x0[i] + g1[i] * (is_q ? w1q[i] : w1k[i]) * x1[i];
+                wg0[i] = g0[i] * (is_q ? w0q[i] : w0k[i]);
+                wg1[i] = g1[i] * (is_q ? w1q[i] : w1k[i]);
+                ss = fma(x1[i], x1[i], fma(x0[i], x0[i], ss));
+                gx = fma(wg1[i], x1[i], fma(wg0[i], x0[i], gx));
             }
             ss = row_sum<LPR>(ss);
             gx = row_sum<LPR>(gx);
-            const double rs = 1.0 / sqrt(ss * a.inv_d + a.eps), back = gx * a.inv_d * rs * rs * rs;
+            const double rs = rsqrt64(fma(ss, a.inv_d, a.eps)), back = -gx * a.inv_d * rs * rs * rs;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const double u = g0[i] * x0[i] * rs, v = g1[i] * x1[i] * rs;
-                if (is_q) { dq0[i] += u; dq1[i] += v; }
-                else { dk0[i] += u; dk1[i] += v; }
-                x0[i] = rs * g0[i] * (is_q ? w0q[i] : w0k[i]) - back * x0[i];
-                x1[i] = rs * g1[i] * (is_q ? w1q[i] : w1k[i]) - back * x1[i];
+                const double u = x0[i] * rs, v = x1[i] * rs;
+                if (is_q) { dq0[i] = fma(g0[i], u, dq0[i]); dq1[i] = fma(g1[i], v, dq1[i]); }
+                else { dk0[i] = fma(g0[i], u, dk0[i]); dk1[i] = fma(g1[i], v, dk1[i]); }
+                x0[i] = fma(rs, wg0[i], back * x0[i]);
+                x1[i] = fma(rs, wg1[i], back * x1[i]);
             }
             if (on) { store4(out + o0, x0); store4(out + o1, x1); }
+            hd += RPI;
+            while (hd >= heads) { hd -= heads; ++tok; }
         }
     }
     // dw of the workgroup: the lanes that hold one column, in the order of their rows
-    double* red = (double*)cs;                            // [RPI][D]
+    double* red = (double*)lds;                           // [RPI][D]
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
         if (on) {
@@ -216,9 +248,9 @@ __global__ void __launch_bounds__(256) head_norm_bwd_kernel(HeadNorm a) {
         }
         __syncthreads();
         for (int d = threadIdx.x; d < a.D; d += 256) {
-            double s = 0.0;
-            for (int r = 0; r < RPI; ++r) s += red[r * a.D + d];
-            a.part[((size_t)blockIdx.x * 2 + which) * a.D + d] = s;
+            double v = 0.0;
+            for (int r = 0; r < RPI; ++r) v += red[r * a.D + d];
+            a.part[((size_t)blockIdx.x * 2 + which) * a.D + d] = v;
         }
     }
 }
@@ -292,7 +324,7 @@ static HeadNorm head_norm_params(const scipnp_head_norm_args* a) {
 
 template <int LPR>
 static void head_norm_launch(const HeadNorm& p, int dtype, bool backward, unsigned grid, hipStream_t st) {
-    size_t lds = (size_t)p.TT * (p.rot / 2) * sizeof(double2);
+    size_t lds = (size_t)p.TT * (sizeof(Token) + (p.rot / 2) * sizeof(double2));
     if (backward) {
         const size_t red = (size_t)(256 / LPR) * p.D * sizeof(double);
         lds = lds > red ? lds : red;
