@@ -10,7 +10,7 @@ typedef float f32x4a __attribute__((ext_vector_type(4)));
 typedef float f32x16a __attribute__((ext_vector_type(16)));
 typedef short s16x4a __attribute__((ext_vector_type(4)));
 
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.693147180559945309417f;
 
 // ---- host-side argument checks
 inline size_t attn_esize(int dtype) { return dtype == SCIPNP_BF16 ? 2 : 4; }
@@ -38,6 +38,16 @@ __device__ __forceinline__ long long xcd_item(unsigned x, long long total) {
     const long long per = (total + 7) >> 3;
     const long long i = (long long)(x & 7) * per + (x >> 3);
     return ((long long)(x >> 3) < per && i < total) ? i : -1;
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = min(v, __shfl_xor(v, off, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = max(v, __shfl_xor(v, off, 64));
+    return __builtin_amdgcn_readfirstlane(v);
 }
 inline unsigned xcd_grid(long long total) { return (unsigned)(((total + 7) >> 3) << 3); }
 

@@ -1,38 +1,36 @@
-// Attention over selected key blocks, forward.  One workgroup of four waves: up to 128 rows (queries x heads of a key head) of one query
-// group; RW waves hold 32 rows each, the 4 / RW others of a row set take every other key tile and are joined at the end (few rows:
-// a decoding step is 8 rows, four waves share its keys).  A pass over the selected tiles with running maximum and sum.
+// Attention over selected key blocks, forward.  One workgroup of RW waves holds up to 32 * RW rows (queries x heads of a key head) of
+// one query group, 32 a wave, and passes once over its part of the selected key tiles (32 keys of K and V, two buffers) with a running
+// maximum and sum; the parts of a group (few rows, many keys: a decoding step) are joined by a second launch.
+//
+// The scores are in units of ln 2: p = exp2(fma(s, scale log2 e, bias log2 e - m)), one fused multiply-add and one v_exp_f32 a score
+// where the tile has one bucket and no mask.  The maximum m is moved only when a tile exceeds it by 2^8: until then p <= 2^8, which
+// costs no accuracy in floating point, and the accumulators are not rescaled.
 #include "block_attn.hpp"
 
 namespace scipnp {
 
-template <typename T, int DP, int RW>
+template <typename T, int DP>
 struct FwdCfg {
-    static constexpr int KS = 4 / RW, NTH = 64 * RW;
-    static constexpr int KST = row_stride<T, DP>(), VST = col_stride<T, DP>();
-    static constexpr int TILE = KT * (KST + VST) * (int)sizeof(T);            // K and V of one tile
-    static constexpr int BUFS = KS == 4 ? 1 : 2;                              // four private tiles need no barrier and no second buffer
-    static constexpr int OST = DP + 4;
-    static constexpr int JOIN = KS > 1 ? RW * 32 * OST * 4 + KS * RW * 32 * 8 : 0;
-    static constexpr int TILES = KS * BUFS * TILE;
-    static constexpr int MAIN = TILES > JOIN ? TILES : JOIN;
-    static constexpr int KP = KS * BUFS * KT * 4;
+    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
+    static constexpr int MAIN = 2 * TILE;
+    static constexpr int KP = 2 * KT * 4;
 };
 
-template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
+template <typename T, int DP, int RW, bool SAVE>           // SAVE: out32 wanted (a training pass)
+__global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using C = FwdCfg<T, DP, RW>;
+    using C = FwdCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
+    constexpr int NB = (DP + 31) / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long total = (long long)a.B * a.Hk * a.ng * a.chunks * a.splits;
     const long long item = xcd_item(blockIdx.x, total);
     if (item < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hi = lane >> 5;
-    const int rw = wave % RW, ks = wave / RW, tsplit = rw * 64 + lane;
-    long long it0 = item;
-    const int part = (int)(it0 % a.splits); it0 /= a.splits;
-    const int chunk = (int)(it0 % a.chunks); it0 /= a.chunks;
-    const int g = (int)(it0 % a.ng), bh = (int)(it0 / a.ng), hk = bh % a.Hk, b = bh / a.Hk;
+    const int lane = threadIdx.x & 63, rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hi = lane >> 5;
+    unsigned it0 = (unsigned)item;
+    const int part = it0 % a.splits; it0 /= a.splits;
+    const int chunk = it0 % a.chunks; it0 /= a.chunks;
+    const int g = it0 % a.ng, bh = it0 / a.ng, hk = bh % a.Hk, b = bh / a.Hk;
     const Seq sq = seq_of(a, b);
     const int R = a.qb * a.G, r0 = chunk * 32 * RW;
     if (g * a.qb + r0 / a.G >= sq.qlen) return;           // (uniform) nothing live in this chunk
@@ -41,12 +39,11 @@ __global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
     const int qkey = sq.shift + tok;                      // key position of the row
     const int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;       // its last visible key
 
-    char* const main = smem;
     int* const kp_lds = (int*)(smem + C::MAIN);
     int* const list = (int*)(smem + C::MAIN + C::KP);
     int* const nlist = list + a.n;
     const Bias bias = load_bias(a, smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16, hk);
-    if (wave == 0) {
+    if (rw == 0) {
         const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
         const int far = a.causal ? min(sq.klen, sq.shift + g * a.qb + (rows_end - 1) / a.G + 1) : sq.klen;
         const int c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
@@ -55,157 +52,104 @@ __global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
     Frag qf[DP / Mat<T>::K];
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
-    RowRange range = {live ? qp : INT_MAX, live ? qp : INT_MIN};
-    int min_lim = live ? lim : INT_MAX, max_lim = lim;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        range.lo = min(range.lo, __shfl_xor(range.lo, off, 64));
-        range.hi = max(range.hi, __shfl_xor(range.hi, off, 64));
-        min_lim = min(min_lim, __shfl_xor(min_lim, off, 64));
-        max_lim = max(max_lim, __shfl_xor(max_lim, off, 64));
-    }
-    range.lo = __builtin_amdgcn_readfirstlane(range.lo);
-    range.hi = __builtin_amdgcn_readfirstlane(range.hi);
-    min_lim = __builtin_amdgcn_readfirstlane(min_lim);
-    max_lim = __builtin_amdgcn_readfirstlane(max_lim);
+    const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
+    const int min_lim = wave_min(live ? lim : INT_MAX), max_lim = wave_max(lim);
+    const unsigned ks = (unsigned)(a.sk.t * (long long)sizeof(T)), vs = (unsigned)(a.sv.t * (long long)sizeof(T));
+    DmaOffsets<T, DP, RW> ko, vo;
+    ko.init(rw, lane, ks, a.D);
+    vo.init(rw, lane, vs, a.D);
     __syncthreads();
 
-    const int tpb = a.block / KT, ntiles = *nlist * tpb;
+    const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist) * tpb;
     const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, t_end = min(ntiles, t_begin + per);
-    const int iters = t_end > t_begin ? (t_end - t_begin + C::KS - 1) / C::KS : 0;
-
     const T* const kb = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
     const T* const vb = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
-    TileRegs<T, DP, C::NTH> kr, vr;
     int kpr = 0;
-    auto key0_of = [&](int it) -> int {
-        const int t = t_begin + it * C::KS + ks;
-        if (t >= t_end) return -1;
+    auto key0_of = [&](int t) -> int {
         const int blk = t / tpb;
-        return list[blk] * a.block + (t - blk * tpb) * KT;
+        return __builtin_amdgcn_readfirstlane(list[blk]) * a.block + (t - blk * tpb) * KT;
     };
-    auto load = [&](int key0) {
-        if (key0 < 0) return;
-        kr.load(tsplit, a.D, [&](int r) { return key0 + r < sq.klen ? kb + (long long)(key0 + r) * a.sk.t : nullptr; });
-        vr.load(tsplit, a.D, [&](int r) { return key0 + r < sq.klen ? vb + (long long)(key0 + r) * a.sv.t : nullptr; });
-        if (a.k_pos && tsplit < KT) kpr = key0 + tsplit < sq.klen ? a.k_pos[(size_t)b * a.Lk + key0 + tsplit] : 0;
+    auto issue = [&](int key0, int buf) {
+        const int there = min(KT, sq.klen - key0);
+        if (there <= 0) return;                           // (the rest of a block behind the last key)
+        char* const tile = smem + buf * C::TILE;
+        ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
+        vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
+        if (a.k_pos && threadIdx.x < KT) kpr = (int)threadIdx.x < there ? a.k_pos[(size_t)b * a.Lk + key0 + threadIdx.x] : 0;
     };
-    f32x16a o[DP / 32];
+    f32x16a o[NB];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    int key0 = iters ? key0_of(0) : -1;
-    load(key0);
-    for (int it = 0; it < iters; ++it) {
-        const int buf = C::BUFS == 2 ? (it & 1) : 0;
-        T* const kt = (T*)(main + (ks * C::BUFS + buf) * C::TILE);
-        T* const vt = kt + KT * C::KST;
-        int* const kp = kp_lds + (ks * C::BUFS + buf) * KT;
-        if (key0 >= 0) {
-            kr.template store<C::KST>(tsplit, kt);
-            vr.template store<C::VST>(tsplit, vt);
-            if (a.k_pos && tsplit < KT) kp[tsplit] = kpr;
+    int key0 = t_begin < t_end ? key0_of(t_begin) : 0;
+    if (t_begin < t_end) issue(key0, 0);
+    for (int t = t_begin; t < t_end; ++t) {
+        const int buf = (t - t_begin) & 1, cur = key0;
+        int* const kp = kp_lds + buf * KT;
+        if (a.k_pos && threadIdx.x < KT) kp[threadIdx.x] = kpr;
+        dma_wait<RW>();                                   // this tile has landed, and everyone is done with the other buffer
+        if (t + 1 < t_end) {
+            key0 = key0_of(t + 1);
+            issue(key0, buf ^ 1);
         }
-        if constexpr (C::BUFS == 2) __syncthreads();
-        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int cur = key0;
-        key0 = it + 1 < iters ? key0_of(it + 1) : -1;
-        load(key0);
-        if (cur >= 0 && cur <= max_lim) {
-            f32x16a s;
+        if (cur > max_lim) continue;
+        const char* const kt = smem + buf * C::TILE;
+        f32x16a s;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.f;
-            s = mma_rows<T, DP>(kt + li * C::KST, qf, hi, s);
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        s = dma_rows<T, DP>(kt, qf, lane, s);
+        int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
+        const bool masked = cur + KT - 1 > min_lim;
+        float c = a.scale2, add = 0.f;
+        if (dist >= 0 && a.nbuckets) add = bias.tbl[bias.lut[dist] * a.G + gl];
+        if (dist < 0 || masked || c < 0.f) {              // the scores one by one
+            if (dist < 0) {
+                float x[16];
+                tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= a.scale;
-            if (a.nbuckets) {
-                const int dist = tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane);
-                if (dist >= 0) {
-                    const float bv = bias.tbl[bias.lut[dist] * a.G + gl];
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, x[r]);
+            } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] += bv;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int k = a.k_pos ? kp[tile_key(r, hi)] : cur + tile_key(r, hi);
-                        s[r] += bias.tbl[bias.lut[clamp_dist(k - qp, a.maxd)] * a.G + gl];
-                    }
-                }
+                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, add);
             }
-            if (cur + KT - 1 > min_lim) {
+            if (masked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : -INFINITY;
             }
-            float mt = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float mn = fmaxf(m, mt), ms = mn == -INFINITY ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f((m - ms) * LOG2E);
-            m = mn;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f((s[r] - ms) * LOG2E);
-                sum += s[r];
-            }
-            l = fmaf(l, alpha, sum);
-            if (__ballot(alpha != 1.f)) {
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-            }
-            // P rounded to bf16 is off by 2^-8 of each probability, of the order of the output's own rounding; with out32 wanted it is
-            // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
-            mma_cols<T, DP, C::VST>(vt, s, lane, o, a.out32 != nullptr);
+            c = 1.f;
+            add = 0.f;
         }
-        if constexpr (C::BUFS == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float mt = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+        mt = fmaf(mt, c, add);
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if (__ballot(mt > m + 8.f)) {
+            const float mn = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+        }
+        const float shift = add - (m == -INFINITY ? 0.f : m);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, shift));
+            sum[r & 3] += s[r];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // P rounded to bf16 is off by 2^-8 of each probability, of the order of the output's own rounding; with out32 wanted it is
+        // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
+        dma_cols<T, DP, SAVE>(kt + DmaTile<T, DP>::BYTES, s, lane, o);
     }
     l += __shfl_xor(l, 32, 64);
 
-    if constexpr (C::KS > 1) {                            // the row set's other waves: maxima and sums first, then the sums of O in order
-        float* const obuf = (float*)main + rw * 32 * C::OST;
-        float2* const ml = (float2*)(main + RW * 32 * C::OST * 4) + rw * 32;
-        __syncthreads();
-        if (hi == 0) ml[ks * RW * 32 + li] = make_float2(m, l);
-        __syncthreads();
-        float M = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < C::KS; ++k) M = fmaxf(M, ml[k * RW * 32 + li].x);
-        const float Ms = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-#pragma unroll
-        for (int k = 0; k < C::KS; ++k) L = fmaf(ml[k * RW * 32 + li].y, __builtin_amdgcn_exp2f((ml[k * RW * 32 + li].x - Ms) * LOG2E), L);
-        const float f = __builtin_amdgcn_exp2f((m - Ms) * LOG2E);
-        m = M;
-        l = L;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[db][r] *= f;
-        for (int k = C::KS - 1; k >= 0; --k) {
-            if (ks == k) {
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        f32x4a* const p = (f32x4a*)(obuf + li * C::OST + 32 * db + 8 * q + 4 * hi);
-                        f32x4a v = f32x4a{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-                        if (k < C::KS - 1) v += *p;
-                        if (k > 0) *p = v;
-                        else
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[db][4 * q + e] = v[e];
-                    }
-            }
-            if (k > 0) __syncthreads();
-        }
-        if (ks > 0) return;
-    }
     if (!live) return;
     const size_t id = ((size_t)b * a.Lq + tok) * a.Hq + head;
     if (a.splits > 1) {
@@ -213,7 +157,7 @@ __global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
         if (hi == 0) *(float2*)(a.pml + 2 * (part * rows + id)) = make_float2(m, l);
         float* const po = a.po + (part * rows + id) * a.D;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
+        for (int db = 0; db < NB; ++db)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int d = 32 * db + 8 * q + 4 * hi;
@@ -224,7 +168,7 @@ __global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);             // (a NaN sum stays one)
     T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int d = 32 * db + 8 * q + 4 * hi;
@@ -240,9 +184,9 @@ __global__ void __launch_bounds__(256) block_attn_kernel(Attn a) {
             } else {
                 *(f32x4a*)(out + d) = v;
             }
-            if (a.out32) *(f32x4a*)(a.out32 + id * a.D + d) = v;
+            if constexpr (SAVE) *(f32x4a*)(a.out32 + id * a.D + d) = v;
         }
-    if (a.lse && hi == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = l == 0.f ? -INFINITY : m + __logf(l);
+    if (a.lse && hi == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 #endif
 }
 
@@ -259,7 +203,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(Attn a) {
     float L = 0.f, s[2] = {0.f, 0.f};
     for (int p = 0; p < a.splits; ++p) {
         const float2 ml = *(const float2*)(a.pml + 2 * (p * rows + id));
-        const float f = __builtin_amdgcn_exp2f((ml.x - Ms) * LOG2E);
+        const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
         L = fmaf(ml.y, f, L);
         const float* po = a.po + (p * rows + id) * a.D;
 #pragma unroll
@@ -275,7 +219,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(Attn a) {
         ((T*)a.out)[b * a.so.b + (long long)tok * a.so.t + head * a.so.h + d] = (T)v;
         if (a.out32) a.out32[id * a.D + d] = v;
     }
-    if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = L == 0.f ? -INFINITY : M + __logf(L);
+    if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
 }
 
 static int row_waves(const scipnp_block_attn_args* a) {
@@ -283,13 +227,13 @@ static int row_waves(const scipnp_block_attn_args* a) {
     return R <= 32 ? 1 : R <= 64 ? 2 : 4;
 }
 
-// parts of a group's keys: enough workgroups for two on every CU, none with fewer than four tiles a wave
+// parts of a group's keys: enough waves for four on every CU, none with fewer than four tiles
 static int attn_splits(const scipnp_block_attn_args* a) {
     const int rw = row_waves(a), R = a->query_block * (a->Hq / a->Hk);
     const long long groups = (long long)a->B * a->Hk * ((a->Lq + a->query_block - 1) / a->query_block) * ((R + 32 * rw - 1) / (32 * rw));
     const int nb = (a->Lk + a->block - 1) / a->block;
     const long long tiles = (long long)(a->n_sel < nb ? a->n_sel : nb) * (a->block / KT);
-    long long want = 512 / (groups > 0 ? groups : 1), most = tiles / (4 * (4 / rw));
+    long long want = 1024 / (groups * rw), most = tiles / 4;
     if (want > most) want = most;
     if (want > 64) want = 64;
     return want < 1 ? 1 : (int)want;
@@ -314,6 +258,7 @@ int attn_check(const scipnp_block_attn_args* a) {
     }
     SCIPNP_ALIGNED(a->q); SCIPNP_ALIGNED(a->k); SCIPNP_ALIGNED(a->v);
     SCIPNP_STRIDES(a->q_stride, a->dtype); SCIPNP_STRIDES(a->k_stride, a->dtype); SCIPNP_STRIDES(a->v_stride, a->dtype);
+    SCIPNP_REQUIRE(a->k_stride[1] < (1 << 24) && a->v_stride[1] < (1 << 24), "token strides of k and v: below 2^24 elements");
     const long long rows = (long long)a->query_block * (a->Hq / a->Hk);
     SCIPNP_REQUIRE((long long)a->B * a->Hk * ((a->Lq + a->query_block - 1) / a->query_block) * ((rows + 31) / 32) < (1ll << 23), "too many query groups");
     return SCIPNP_OK;
@@ -326,6 +271,7 @@ Attn attn_params(const scipnp_block_attn_args* a) {
     p.nb = (a->Lk + a->block - 1) / a->block; p.ng = (a->Lq + a->query_block - 1) / a->query_block;
     p.chunks = p.splits = 1;
     p.scale = a->scale;
+    p.scale2 = a->scale * LOG2E;
     p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.dout = a->dout;
     p.sq = strides_of(a->q_stride); p.sk = strides_of(a->k_stride); p.sv = strides_of(a->v_stride); p.so = strides_of(a->out_stride);
     p.sdo = strides_of(a->dout_stride);
@@ -336,23 +282,24 @@ Attn attn_params(const scipnp_block_attn_args* a) {
     return p;
 }
 
-template <typename T, int DP, int RW>
+template <typename T, int DP, int RW, bool SAVE>
 static int fwd_launch(const Attn& p, unsigned grid, hipStream_t st) {
-    using C = FwdCfg<T, DP, RW>;
-    const size_t fixed = (size_t)C::MAIN + C::KP, lds = fixed + (size_t)(p.n + 4) / 4 * 16 + bias_lds(p.nbuckets, p.maxd, p.G);
+    using C = FwdCfg<T, DP>;
+    const size_t lds = (size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + bias_lds(p.nbuckets, p.maxd, p.G);
     static LdsAttrOnce once;
-    const size_t most = fixed + 1028 * 4 + bias_lds(1, 4096, 1) + 2048 * 4;
-    if (const int rc = once.ensure((const void*)block_attn_kernel<T, DP, RW>, most < 163840 ? most : 163840, "block_attn")) return rc;
-    if (lds > 163840) return fail(SCIPNP_EINVAL, "block_attn: %zu bytes of LDS needed", lds);
-    block_attn_kernel<T, DP, RW><<<grid, 256, lds, st>>>(p);
+    if (const int rc = once.ensure((const void*)block_attn_kernel<T, DP, RW, SAVE>, 163840, "block_attn")) return rc;
+    block_attn_kernel<T, DP, RW, SAVE><<<grid, 64 * RW, lds, st>>>(p);
     return SCIPNP_OK;
 }
 template <typename T, int DP>
 static int fwd_rows(const Attn& p, int rw, unsigned grid, hipStream_t st) {
-    return rw == 1 ? fwd_launch<T, DP, 1>(p, grid, st) : rw == 2 ? fwd_launch<T, DP, 2>(p, grid, st) : fwd_launch<T, DP, 4>(p, grid, st);
+    if (p.out32) return rw == 1 ? fwd_launch<T, DP, 1, true>(p, grid, st) : rw == 2 ? fwd_launch<T, DP, 2, true>(p, grid, st) : fwd_launch<T, DP, 4, true>(p, grid, st);
+    return rw == 1 ? fwd_launch<T, DP, 1, false>(p, grid, st) : rw == 2 ? fwd_launch<T, DP, 2, false>(p, grid, st) : fwd_launch<T, DP, 4, false>(p, grid, st);
 }
 template <typename T>
 static int fwd_dim(const Attn& p, int rw, unsigned grid, hipStream_t st) {
+    if constexpr (sizeof(T) == 4)                          // fp32 products are the cost: 33 to 48 columns as 48 in the score product
+        if (p.D > 32 && p.D <= 48) return fwd_rows<T, 48>(p, rw, grid, st);
     return p.D <= 32 ? fwd_rows<T, 32>(p, rw, grid, st) : p.D <= 64 ? fwd_rows<T, 64>(p, rw, grid, st)
          : p.D <= 96 ? fwd_rows<T, 96>(p, rw, grid, st) : fwd_rows<T, 128>(p, rw, grid, st);
 }

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     load_frags<T, DP>(live ? (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + head * a.sdo.h : nullptr, a.D, hi, gf);
     const size_t stat = ((size_t)b * a.Hq + head) * a.Lq + tok;
-    const float lse = live ? a.lse[stat] : 0.f, delta = live ? a.delta[stat] : 0.f;
+    const float lse = live ? a.lse[stat] * LOG2E : 0.f, delta = live ? a.delta[stat] : 0.f;
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
     RowRange range = {live ? qp : INT_MAX, live ? qp : INT_MIN};
     int min_lim = live ? lim : INT_MAX, max_lim = lim;
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
             s = mma_rows<T, DP>(kt + li * C::ST, qf, hi, s);
             dp = mma_rows<T, DP>(vt + li * C::ST, gf, hi, dp);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= a.scale;
+            for (int r = 0; r < 16; ++r) s[r] *= a.scale2;
             int dist = -1;
             if (a.nbuckets) {
                 dist = tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane);
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f((s[r] - lse) * LOG2E);
+                const float p = __builtin_amdgcn_exp2f(s[r] - lse);
                 s[r] = cur + tile_key(r, hi) <= lim ? p * (dp[r] - delta) : 0.f;
             }
             if (a.dbias) {
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
             ilim = -1; ilse = idelta = 0.f; iqp = 0; ig = gl;
             if (tok >= 0) {
                 const size_t stat = ((size_t)b * a.Hq + hk * a.G + gl) * a.Lq + tok;
-                ilse = a.lse[stat];
+                ilse = a.lse[stat] * LOG2E;
                 idelta = a.delta[stat];
                 ilim = a.causal ? min(sq.shift + tok, sq.klen - 1) : sq.klen - 1;
                 iqp = a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : sq.shift + tok;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * q + e;
                 const bool see = key <= lims[e];
-                const float p = see ? __builtin_amdgcn_exp2f((s[r] * a.scale + add[e] - lse[e]) * LOG2E) : 0.f;
+                const float p = see ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, add[e] - lse[e])) : 0.f;
                 s[r] = p;
                 dp[r] = see ? p * (dp[r] - delta[e]) : 0.f;
             }
