@@ -39,6 +39,9 @@ __device__ __forceinline__ long long xcd_item(unsigned x, long long total) {
     const long long i = (long long)(x & 7) * per + (x >> 3);
     return ((long long)(x >> 3) < per && i < total) ? i : -1;
 }
+// four neighbouring results, rounded to T
+__device__ __forceinline__ void store_four(float* p, f32x4a v) { *(f32x4a*)p = v; }
+__device__ __forceinline__ void store_four(__bf16* p, f32x4a v) { *(bf16x4*)p = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; }
 __device__ __forceinline__ int wave_min(int v) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) v = min(v, __shfl_xor(v, off, 64));

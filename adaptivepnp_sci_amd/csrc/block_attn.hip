@@ -16,37 +16,48 @@ struct FwdCfg {
     static constexpr int KP = 2 * KT * 4;
 };
 
+// A workgroup holds `sets` sets of RW waves, each with work of its own: four waves a workgroup land one on each SIMD of a CU, where
+// workgroups of one or two leave some SIMDs with three waves and some with one.
 template <typename T, int DP, int RW, bool SAVE>           // SAVE: out32 wanted (a training pass)
-__global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
+__global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = FwdCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
     const long long total = (long long)a.B * a.Hk * a.ng * a.chunks * a.splits;
-    const long long item = xcd_item(blockIdx.x, total);
-    if (item < 0) return;
-    const int lane = threadIdx.x & 63, rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, hi = lane >> 5;
-    unsigned it0 = (unsigned)item;
+    const long long first = xcd_item(blockIdx.x, (total + sets - 1) / sets);
+    if (first < 0) return;
+    const int lane = threadIdx.x & 63, li = lane & 31, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int set = wave / RW, rw = wave % RW, tset = rw * 64 + lane;
+    const bool there_is = first * sets + set < total;
+    unsigned it0 = there_is ? (unsigned)(first * sets + set) : 0;
     const int part = it0 % a.splits; it0 /= a.splits;
     const int chunk = it0 % a.chunks; it0 /= a.chunks;
     const int g = it0 % a.ng, bh = it0 / a.ng, hk = bh % a.Hk, b = bh / a.Hk;
     const Seq sq = seq_of(a, b);
     const int R = a.qb * a.G, r0 = chunk * 32 * RW;
-    if (g * a.qb + r0 / a.G >= sq.qlen) return;           // (uniform) nothing live in this chunk
+    const bool any = there_is && g * a.qb + r0 / a.G < sq.qlen;             // a live row in this chunk
     const int row = r0 + rw * 32 + li, tok = g * a.qb + row / a.G, gl = row % a.G, head = hk * a.G + gl;
-    const bool live = row < R && tok < sq.qlen;
+    const bool live = there_is && row < R && tok < sq.qlen;
     const int qkey = sq.shift + tok;                      // key position of the row
     const int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;       // its last visible key
 
+    unsigned char* const lut = (unsigned char*)smem_all;  // shared by the sets; then each set's own
+    char* const smem = smem_all + bias_lut_bytes(a.nbuckets, a.maxd) + 16 + set * set_bytes;
+    int* const longest = (int*)(smem_all + bias_lut_bytes(a.nbuckets, a.maxd));
     int* const kp_lds = (int*)(smem + C::MAIN);
     int* const list = (int*)(smem + C::MAIN + C::KP);
     int* const nlist = list + a.n;
-    const Bias bias = load_bias(a, smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16, hk);
+    const Bias bias = load_bias(a, lut, (float*)(smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16), hk, tset, 64 * RW);
+    if (threadIdx.x == 0) *longest = 0;
     if (rw == 0) {
-        const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
-        const int far = a.causal ? min(sq.klen, sq.shift + g * a.qb + (rows_end - 1) / a.G + 1) : sq.klen;
-        const int c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
+        int c = 0;
+        if (any) {
+            const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
+            const int far = a.causal ? min(sq.klen, sq.shift + g * a.qb + (rows_end - 1) / a.G + 1) : sq.klen;
+            c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
+        }
         if (lane == 0) *nlist = c;
     }
     Frag qf[DP / Mat<T>::K];
@@ -61,13 +72,24 @@ __global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
     __syncthreads();
 
     const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist) * tpb;
-    const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, t_end = min(ntiles, t_begin + per);
+    const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, count = max(0, min(ntiles, t_begin + per) - t_begin);
+    int trips = count;                                    // sets that share a barrier take the same number of trips
+    if constexpr (RW > 1) {
+        if (sets > 1) {
+            if (tset == 0) atomicMax(longest, count);
+            __syncthreads();
+            trips = __builtin_amdgcn_readfirstlane(*longest);
+        }
+    }
     const T* const kb = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
     const T* const vb = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
     int kpr = 0;
-    auto key0_of = [&](int t) -> int {
-        const int blk = t / tpb;
-        return __builtin_amdgcn_readfirstlane(list[blk]) * a.block + (t - blk * tpb) * KT;
+    int blk = t_begin / tpb, off = (t_begin - blk * tpb) * KT;              // the next tile to ask for
+    auto next_key = [&]() -> int {
+        const int key = __builtin_amdgcn_readfirstlane(list[blk]) * a.block + off;
+        off += KT;
+        if (off == a.block) { off = 0; ++blk; }
+        return key;
     };
     auto issue = [&](int key0, int buf) {
         const int there = min(KT, sq.klen - key0);
@@ -75,8 +97,10 @@ __global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
         char* const tile = smem + buf * C::TILE;
         ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
         vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
-        if (a.k_pos && threadIdx.x < KT) kpr = (int)threadIdx.x < there ? a.k_pos[(size_t)b * a.Lk + key0 + threadIdx.x] : 0;
+        if (a.k_pos && tset < KT) kpr = tset < there ? a.k_pos[(size_t)b * a.Lk + key0 + tset] : 0;
     };
+    const int far = 2 * a.maxd;                           // the two ends, where most tiles lie: their bias in registers
+    const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
     f32x16a o[NB];
 #pragma unroll
     for (int db = 0; db < NB; ++db)
@@ -84,27 +108,29 @@ __global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
         for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    int key0 = t_begin < t_end ? key0_of(t_begin) : 0;
-    if (t_begin < t_end) issue(key0, 0);
-    for (int t = t_begin; t < t_end; ++t) {
-        const int buf = (t - t_begin) & 1, cur = key0;
+    int key0 = 0;
+    if (count > 0) {
+        key0 = next_key();
+        issue(key0, 0);
+    }
+    for (int t = 0; t < trips; ++t) {
+        const int buf = t & 1, cur = key0;
         int* const kp = kp_lds + buf * KT;
-        if (a.k_pos && threadIdx.x < KT) kp[threadIdx.x] = kpr;
+        if (a.k_pos && tset < KT) kp[tset] = kpr;
         dma_wait<RW>();                                   // this tile has landed, and everyone is done with the other buffer
-        if (t + 1 < t_end) {
-            key0 = key0_of(t + 1);
+        if (t + 1 < count) {
+            key0 = next_key();
             issue(key0, buf ^ 1);
         }
-        if (cur > max_lim) continue;
+        if (t >= count || cur > max_lim) continue;
         const char* const kt = smem + buf * C::TILE;
-        f32x16a s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        s = dma_rows<T, DP>(kt, qf, lane, s);
-        int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
+        f32x16a s = dma_rows<T, DP>(kt, qf, lane);
+        ColTile<T, DP> vt;
+        vt.read(kt + DmaTile<T, DP>::BYTES, lane);
+        const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
         const bool masked = cur + KT - 1 > min_lim;
         float c = a.scale2, add = 0.f;
-        if (dist >= 0 && a.nbuckets) add = bias.tbl[bias.lut[dist] * a.G + gl];
+        if (dist >= 0 && a.nbuckets) add = dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
         if (dist < 0 || masked || c < 0.f) {              // the scores one by one
             if (dist < 0) {
                 float x[16];
@@ -146,7 +172,7 @@ __global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // P rounded to bf16 is off by 2^-8 of each probability, of the order of the output's own rounding; with out32 wanted it is
         // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
-        dma_cols<T, DP, SAVE>(kt + DmaTile<T, DP>::BYTES, s, lane, o);
+        vt.template mma<SAVE>(s, o);
     }
     l += __shfl_xor(l, 32, 64);
 
@@ -156,36 +182,21 @@ __global__ void __launch_bounds__(64 * RW, 2) block_attn_kernel(Attn a) {
         const size_t rows = (size_t)a.B * a.Lq * a.Hq;
         if (hi == 0) *(float2*)(a.pml + 2 * (part * rows + id)) = make_float2(m, l);
         float* const po = a.po + (part * rows + id) * a.D;
-#pragma unroll
-        for (int db = 0; db < NB; ++db)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int d = 32 * db + 8 * q + 4 * hi;
-                if (d < a.D) *(f32x4a*)(po + d) = f32x4a{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-            }
+        each_four<T, NB>(hi, [&](int d, auto at) {
+            if (d < a.D) *(f32x4a*)(po + d) = f32x4a{o[at(0) >> 4][at(0) & 15], o[at(1) >> 4][at(1) & 15], o[at(2) >> 4][at(2) & 15], o[at(3) >> 4][at(3) & 15]};
+        });
         return;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);             // (a NaN sum stays one)
     T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
+    each_four<T, NB>(hi, [&](int d, auto at) {
+        if (d >= a.D) return;
+        f32x4a v;
 #pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = 32 * db + 8 * q + 4 * hi;
-            if (d >= a.D) continue;
-            f32x4a v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = o[db][4 * q + e] * inv;
-            if constexpr (sizeof(T) == 2) {
-                bf16x4 w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (__bf16)v[e];
-                *(bf16x4*)(out + d) = w;
-            } else {
-                *(f32x4a*)(out + d) = v;
-            }
-            if constexpr (SAVE) *(f32x4a*)(a.out32 + id * a.D + d) = v;
-        }
+        for (int e = 0; e < 4; ++e) v[e] = o[at(e) >> 4][at(e) & 15] * inv;
+        store_four(out + d, v);
+        if constexpr (SAVE) *(f32x4a*)(a.out32 + id * a.D + d) = v;
+    });
     if (a.lse && hi == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 #endif
 }
@@ -283,25 +294,29 @@ Attn attn_params(const scipnp_block_attn_args* a) {
 }
 
 template <typename T, int DP, int RW, bool SAVE>
-static int fwd_launch(const Attn& p, unsigned grid, hipStream_t st) {
+static int fwd_launch(const Attn& p, hipStream_t st) {
     using C = FwdCfg<T, DP>;
-    const size_t lds = (size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + bias_lds(p.nbuckets, p.maxd, p.G);
+    const size_t set = ((size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + (size_t)p.nbuckets * p.G * 4 + 15) / 16 * 16;
+    const size_t shared = bias_lut_bytes(p.nbuckets, p.maxd) + 16;
+    int sets = 4 / RW;
+    while (sets > 1 && shared + sets * set > 163840) sets >>= 1;
     static LdsAttrOnce once;
     if (const int rc = once.ensure((const void*)block_attn_kernel<T, DP, RW, SAVE>, 163840, "block_attn")) return rc;
-    block_attn_kernel<T, DP, RW, SAVE><<<grid, 64 * RW, lds, st>>>(p);
+    const long long items = (long long)p.B * p.Hk * p.ng * p.chunks * p.splits;
+    block_attn_kernel<T, DP, RW, SAVE><<<xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set);
     return SCIPNP_OK;
 }
 template <typename T, int DP>
-static int fwd_rows(const Attn& p, int rw, unsigned grid, hipStream_t st) {
-    if (p.out32) return rw == 1 ? fwd_launch<T, DP, 1, true>(p, grid, st) : rw == 2 ? fwd_launch<T, DP, 2, true>(p, grid, st) : fwd_launch<T, DP, 4, true>(p, grid, st);
-    return rw == 1 ? fwd_launch<T, DP, 1, false>(p, grid, st) : rw == 2 ? fwd_launch<T, DP, 2, false>(p, grid, st) : fwd_launch<T, DP, 4, false>(p, grid, st);
+static int fwd_rows(const Attn& p, int rw, hipStream_t st) {
+    if (p.out32) return rw == 1 ? fwd_launch<T, DP, 1, true>(p, st) : rw == 2 ? fwd_launch<T, DP, 2, true>(p, st) : fwd_launch<T, DP, 4, true>(p, st);
+    return rw == 1 ? fwd_launch<T, DP, 1, false>(p, st) : rw == 2 ? fwd_launch<T, DP, 2, false>(p, st) : fwd_launch<T, DP, 4, false>(p, st);
 }
 template <typename T>
-static int fwd_dim(const Attn& p, int rw, unsigned grid, hipStream_t st) {
+static int fwd_dim(const Attn& p, int rw, hipStream_t st) {
     if constexpr (sizeof(T) == 4)                          // fp32 products are the cost: 33 to 48 columns as 48 in the score product
-        if (p.D > 32 && p.D <= 48) return fwd_rows<T, 48>(p, rw, grid, st);
-    return p.D <= 32 ? fwd_rows<T, 32>(p, rw, grid, st) : p.D <= 64 ? fwd_rows<T, 64>(p, rw, grid, st)
-         : p.D <= 96 ? fwd_rows<T, 96>(p, rw, grid, st) : fwd_rows<T, 128>(p, rw, grid, st);
+        if (p.D > 32 && p.D <= 48) return fwd_rows<T, 48>(p, rw, st);
+    return p.D <= 32 ? fwd_rows<T, 32>(p, rw, st) : p.D <= 64 ? fwd_rows<T, 64>(p, rw, st)
+         : p.D <= 96 ? fwd_rows<T, 96>(p, rw, st) : fwd_rows<T, 128>(p, rw, st);
 }
 
 size_t attn_backward_workspace(const scipnp_block_attn_args* a);
@@ -336,8 +351,7 @@ int scipnp_block_attn(const scipnp_block_attn_args* a, scipnp_stream_t s) {
         p.po = (float*)a->workspace;
         p.pml = p.po + (size_t)p.splits * a->B * a->Lq * a->Hq * a->D;
     }
-    const unsigned grid = xcd_grid((long long)p.B * p.Hk * p.ng * p.chunks * p.splits);
-    if (const int rc = a->dtype == SCIPNP_BF16 ? fwd_dim<__bf16>(p, rw, grid, st) : fwd_dim<float>(p, rw, grid, st)) return rc;
+    if (const int rc = a->dtype == SCIPNP_BF16 ? fwd_dim<__bf16>(p, rw, st) : fwd_dim<float>(p, rw, st)) return rc;
     if (p.splits > 1) {
         const unsigned jg = (unsigned)(((size_t)p.B * p.Lq * p.Hq + 3) / 4);
         if (a->dtype == SCIPNP_BF16) block_attn_join_kernel<__bf16><<<jg, 256, 0, st>>>(p);

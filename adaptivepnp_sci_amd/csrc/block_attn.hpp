@@ -180,114 +180,200 @@ struct DmaOffsets {
     }
 };
 
-// score products: acc += A B^T, A = row li of the tile
+// score products: A B^T, A = row li of the tile.  All of a half's reads are under way before its first product
 template <typename T, int DP>
-__device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int lane, f32x16a acc) {
-    constexpr int LC = DmaTile<T, DP>::LC;
+__device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int lane) {
+    constexpr int LC = DmaTile<T, DP>::LC, N = DP / Mat<T>::K, H = N <= 8 ? N : N / 2;
     const int li = lane & 31, x = (lane >> 5) ^ swz<T, LC>(li);
     const char* row = tile + li * LC * 16;
+    f32x16a acc;
 #pragma unroll
-    for (int s = 0; s < DP / Mat<T>::K; ++s) {
-        const typename Mat<T>::Frag a = *(const typename Mat<T>::Frag*)(row + ((x ^ (2 * s)) << 4));
-        if constexpr (sizeof(T) == 2) {
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[s], acc, 0, 0, 0);
-        } else {
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[s][j], acc, 0, 0, 0);
+    for (int h = 0; h < N; h += H) {
+        typename Mat<T>::Frag a[H];
+#pragma unroll
+        for (int s = 0; s < H; ++s) a[s] = *(const typename Mat<T>::Frag*)(row + ((x ^ (2 * (h + s))) << 4));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < H; ++s) {
+            if constexpr (sizeof(T) == 2) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s], b[h + s], acc, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], b[h + s][j], acc, 0, 0, 0);
+            }
         }
     }
     return acc;
 }
 
-// transposing reads of one or two column blocks (4 rows and the 4 rows 8 below): the 16 lanes of a group supply 4 rows x 16 columns (8
-// bytes each) and receive a column's 4 rows.  Written as assembly because the compiler takes the builtin for a reader of every request
-// in flight and waits for the NEXT tile in front of it; each block waits for its own reads.
+// second products: acc += X^T P over the tile's 32 rows (P in an accumulator's registers, rounded to T), NB column blocks of 32.
+// bf16: read() brings the transposed tile into registers, early, so that the reads overlap the score products and the softmax;
+//   the 16 lanes of a group supply 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows.  Assembly because the compiler
+//   takes the builtin for a reader of every request in flight and waits for the NEXT tile in front of it; the block waits for its reads.
+//   Column 32 db + m is row m of block db.  EXACT: P as three bf16 numbers that add up to its 24 bits, three products.
+// fp32: with 2 or 4 blocks a lane reads 2 or 4 neighbouring columns at once: column NB m + db is row m of block db.
 typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
-template <int OFF, int DOWN>
-__device__ __forceinline__ void tr_read(unsigned a0, unsigned a1, bf16x8& x) {
+template <typename T, int DP>
+struct ColTile {
+    static constexpr int LC = DmaTile<T, DP>::LC, NB = (DP + 31) / 32;
+    union Pair { u32x2a s[2]; bf16x8 v; };
+    Pair u[sizeof(T) == 2 ? NB : 1][2];
+    const char* tile;
+    int lane;
+    __device__ __forceinline__ void read(const char* tile_, int lane_) {
+        tile = tile_;
+        lane = lane_;
 #if defined(__HIP_DEVICE_COMPILE__)
-    union { u32x2a s[2]; bf16x8 v; } u;
-    asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%4\n\tds_read_b64_tr_b16 %1, %3 offset:%5\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(u.s[0]), "=&v"(u.s[1]) : "v"(a0), "v"(a1), "n"(OFF), "n"(OFF + DOWN));
-    x = u.v;
-#endif
-}
-template <int OFF, int DOWN>
-__device__ __forceinline__ void tr_read2(unsigned a0, unsigned a1, unsigned b0, unsigned b1, bf16x8& x, bf16x8& y) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    union { u32x2a s[2]; bf16x8 v; } u, w;
-    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%9\n\t"
-                 "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%9\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(u.s[0]), "=&v"(u.s[1]), "=&v"(w.s[0]), "=&v"(w.s[1])
-                 : "v"(a0), "v"(a1), "v"(b0), "v"(b1), "n"(OFF), "n"(OFF + DOWN));
-    x = u.v;
-    y = w.v;
-#endif
-}
-
-// second products: acc[db] += X^T P over the tile's 32 rows, P in an accumulator's registers, rounded to T.  EXACT (bf16): P as three
-// bf16 numbers that add up to its 24 bits, three products
-template <typename T, int DP, bool EXACT = false>
-__device__ __forceinline__ void dma_cols(const char* tile, const f32x16a& p, int lane, f32x16a (&acc)[(DP + 31) / 32]) {
-    constexpr int LC = DmaTile<T, DP>::LC, NB = (DP + 31) / 32;
-    const int li = lane & 31, hi = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-        const int q = (lane >> 2) & 3, c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), r0 = 4 * hi + q;
-        const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) const char*)tile + r0 * LC * 16 + 8 * (lane & 1);
-        const int f0 = c0 ^ swz<T, LC>(r0), f1 = c0 ^ swz<T, LC>(r0 + 8);
-        bf16x8 pb[2], p1[2], p2[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = p[8 * k + i];
-                pb[k][i] = (__bf16)x;
-                if constexpr (EXACT) {
-                    const float r1 = x - (float)pb[k][i];
-                    p1[k][i] = (__bf16)r1;
-                    p2[k][i] = (__bf16)(r1 - (float)p1[k][i]);
-                }
-            }
-        auto product = [&](int db, int k, const bf16x8& x) {
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pb[k], acc[db], 0, 0, 0);
-            if constexpr (EXACT) {
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, p1[k], acc[db], 0, 0, 0);
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, p2[k], acc[db], 0, 0, 0);
-            }
-        };
-        constexpr int STEP = 16 * LC * 16, DOWN = 8 * LC * 16;             // 16 rows, 8 rows
-#pragma unroll
-        for (int db = 0; db + 1 < NB; db += 2) {
-            const unsigned a0 = base + ((f0 ^ (4 * db)) << 4), a1 = base + ((f1 ^ (4 * db)) << 4);
-            const unsigned b0 = base + ((f0 ^ (4 * db + 4)) << 4), b1 = base + ((f1 ^ (4 * db + 4)) << 4);
-            bf16x8 x, y;
-            tr_read2<0, DOWN>(a0, a1, b0, b1, x, y);
-            product(db, 0, x);
-            product(db + 1, 0, y);
-            tr_read2<STEP, DOWN>(a0, a1, b0, b1, x, y);
-            product(db, 1, x);
-            product(db + 1, 1, y);
-        }
-        if constexpr (NB & 1) {
-            const unsigned a0 = base + ((f0 ^ (4 * (NB - 1))) << 4), a1 = base + ((f1 ^ (4 * (NB - 1))) << 4);
-            bf16x8 x;
-            tr_read<0, DOWN>(a0, a1, x);
-            product(NB - 1, 0, x);
-            tr_read<STEP, DOWN>(a0, a1, x);
-            product(NB - 1, 1, x);
-        }
-    } else {
-        const char* base = tile + 4 * hi * LC * 16 + 4 * (li & 3);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = 8 * (r >> 2) + (r & 3);        // + 4 hi
-            const int f = (li >> 2) ^ swz<T, LC>(row + 4 * hi);
+        if constexpr (sizeof(T) == 2) {
+            const int q = (lane >> 2) & 3, c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), r0 = 4 * (lane >> 5) + q;
+            const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) const char*)tile + r0 * LC * 16 + 8 * (lane & 1);
+            const int f0 = c0 ^ swz<T, LC>(r0), f1 = c0 ^ swz<T, LC>(r0 + 8);
+            constexpr int STEP = 16 * LC * 16, DOWN = 8 * LC * 16;         // 16 rows, 8 rows
+            unsigned at[2 * NB];
 #pragma unroll
             for (int db = 0; db < NB; ++db) {
-                const float x = *(const float*)(base + row * LC * 16 + ((f ^ (8 * db)) << 4));
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[r], acc[db], 0, 0, 0);
+                at[2 * db] = base + ((f0 ^ (4 * db)) << 4);
+                at[2 * db + 1] = base + ((f1 ^ (4 * db)) << 4);
+            }
+            read_blocks<STEP, DOWN>(at);
+        }
+#endif
+    }
+#if defined(__HIP_DEVICE_COMPILE__)
+    template <int STEP, int DOWN>
+    __device__ __forceinline__ void read_blocks(const unsigned (&at)[2 * NB]) {
+        if constexpr (NB == 1)
+            asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+                     "ds_read_b64_tr_b16 %1, %5 offset:%7\n\t"
+                     "ds_read_b64_tr_b16 %2, %4 offset:%8\n\t"
+                     "ds_read_b64_tr_b16 %3, %5 offset:%9\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(u[0][0].s[0]), "=&v"(u[0][0].s[1]), "=&v"(u[0][1].s[0]), "=&v"(u[0][1].s[1])
+                         : "v"(at[0]), "v"(at[1]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
+        if constexpr (NB == 2)
+            asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %1, %9 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %5, %11 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %2, %8 offset:%14\n\t"
+                     "ds_read_b64_tr_b16 %3, %9 offset:%15\n\t"
+                     "ds_read_b64_tr_b16 %6, %10 offset:%14\n\t"
+                     "ds_read_b64_tr_b16 %7, %11 offset:%15\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(u[0][0].s[0]), "=&v"(u[0][0].s[1]), "=&v"(u[0][1].s[0]), "=&v"(u[0][1].s[1]), "=&v"(u[1][0].s[0]), "=&v"(u[1][0].s[1]), "=&v"(u[1][1].s[0]), "=&v"(u[1][1].s[1])
+                         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
+        if constexpr (NB == 3)
+            asm volatile("ds_read_b64_tr_b16 %0, %12 offset:%18\n\t"
+                     "ds_read_b64_tr_b16 %1, %13 offset:%19\n\t"
+                     "ds_read_b64_tr_b16 %4, %14 offset:%18\n\t"
+                     "ds_read_b64_tr_b16 %5, %15 offset:%19\n\t"
+                     "ds_read_b64_tr_b16 %8, %16 offset:%18\n\t"
+                     "ds_read_b64_tr_b16 %9, %17 offset:%19\n\t"
+                     "ds_read_b64_tr_b16 %2, %12 offset:%20\n\t"
+                     "ds_read_b64_tr_b16 %3, %13 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %6, %14 offset:%20\n\t"
+                     "ds_read_b64_tr_b16 %7, %15 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %10, %16 offset:%20\n\t"
+                     "ds_read_b64_tr_b16 %11, %17 offset:%21\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(u[0][0].s[0]), "=&v"(u[0][0].s[1]), "=&v"(u[0][1].s[0]), "=&v"(u[0][1].s[1]), "=&v"(u[1][0].s[0]), "=&v"(u[1][0].s[1]), "=&v"(u[1][1].s[0]), "=&v"(u[1][1].s[1]), "=&v"(u[2][0].s[0]), "=&v"(u[2][0].s[1]), "=&v"(u[2][1].s[0]), "=&v"(u[2][1].s[1])
+                         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
+        if constexpr (NB == 4)
+            asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%24\n\t"
+                     "ds_read_b64_tr_b16 %1, %17 offset:%25\n\t"
+                     "ds_read_b64_tr_b16 %4, %18 offset:%24\n\t"
+                     "ds_read_b64_tr_b16 %5, %19 offset:%25\n\t"
+                     "ds_read_b64_tr_b16 %8, %20 offset:%24\n\t"
+                     "ds_read_b64_tr_b16 %9, %21 offset:%25\n\t"
+                     "ds_read_b64_tr_b16 %12, %22 offset:%24\n\t"
+                     "ds_read_b64_tr_b16 %13, %23 offset:%25\n\t"
+                     "ds_read_b64_tr_b16 %2, %16 offset:%26\n\t"
+                     "ds_read_b64_tr_b16 %3, %17 offset:%27\n\t"
+                     "ds_read_b64_tr_b16 %6, %18 offset:%26\n\t"
+                     "ds_read_b64_tr_b16 %7, %19 offset:%27\n\t"
+                     "ds_read_b64_tr_b16 %10, %20 offset:%26\n\t"
+                     "ds_read_b64_tr_b16 %11, %21 offset:%27\n\t"
+                     "ds_read_b64_tr_b16 %14, %22 offset:%26\n\t"
+                     "ds_read_b64_tr_b16 %15, %23 offset:%27\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(u[0][0].s[0]), "=&v"(u[0][0].s[1]), "=&v"(u[0][1].s[0]), "=&v"(u[0][1].s[1]), "=&v"(u[1][0].s[0]), "=&v"(u[1][0].s[1]), "=&v"(u[1][1].s[0]), "=&v"(u[1][1].s[1]), "=&v"(u[2][0].s[0]), "=&v"(u[2][0].s[1]), "=&v"(u[2][1].s[0]), "=&v"(u[2][1].s[1]), "=&v"(u[3][0].s[0]), "=&v"(u[3][0].s[1]), "=&v"(u[3][1].s[0]), "=&v"(u[3][1].s[1])
+                         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
+    }
+#endif
+    template <bool EXACT = false>
+    __device__ __forceinline__ void mma(const f32x16a& p, f32x16a (&acc)[NB]) const {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                bf16x8 pb, p1, p2;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = p[8 * k + i];
+                    pb[i] = (__bf16)x;
+                    if constexpr (EXACT) {
+                        const float r1 = x - (float)pb[i];
+                        p1[i] = (__bf16)r1;
+                        p2[i] = (__bf16)(r1 - (float)p1[i]);
+                    }
+                }
+#pragma unroll
+                for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, pb, acc[db], 0, 0, 0);
+                if constexpr (EXACT) {
+#pragma unroll
+                    for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p1, acc[db], 0, 0, 0);
+#pragma unroll
+                    for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[db], 0, 0, 0);
+                }
+            }
+        } else {
+            constexpr int W = NB == 3 ? 1 : NB;            // floats of a read
+            typedef float vec __attribute__((ext_vector_type(W == 1 ? 1 : W)));
+            const int li = lane & 31, hi = lane >> 5;
+            const char* base = tile + 4 * hi * LC * 16 + (W * 4 * li & 15);
+            float x[2][4][NB];
+            auto fetch = [&](int a, float (&y)[4][NB]) {   // rows 8 a + 4 hi + 0..3
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 8 * a + e, f = swz<T, LC>(row + 4 * hi);
+                    if constexpr (W == 1) {
+#pragma unroll
+                        for (int db = 0; db < NB; ++db) y[e][db] = *(const float*)(base + row * LC * 16 + ((((li >> 2) + 8 * db) ^ f) << 4));
+                    } else {
+                        const vec v = *(const vec*)(base + row * LC * 16 + (((W * li >> 2) ^ f) << 4));
+#pragma unroll
+                        for (int db = 0; db < NB; ++db) y[e][db] = v[db];
+                    }
+                }
+            };
+            fetch(0, x[0]);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                if (a < 3) fetch(a + 1, x[(a + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[a & 1][e][db], p[4 * a + e], acc[db], 0, 0, 0);
             }
         }
+    }
+};
+// the accumulators of a lane's row, four neighbouring columns at a time: f(column, values, block and register of each)
+template <typename T, int NB, typename F>
+__device__ __forceinline__ void each_four(int hi, F f) {
+    if constexpr (sizeof(T) == 4 && NB == 4) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) f(4 * (8 * (r >> 2) + 4 * hi + (r & 3)), [=](int e) { return e * 16 + r; });
+    } else if constexpr (sizeof(T) == 4 && NB == 2) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) f(2 * (8 * (r >> 2) + 4 * hi + (r & 3)), [=](int e) { return (e & 1) * 16 + r + (e >> 1); });
+    } else {
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f(32 * db + 8 * q + 4 * hi, [=](int e) { return db * 16 + 4 * q + e; });
     }
 }
 // all of this wave's requests have landed; every wave's, with more than one
@@ -365,17 +451,14 @@ __device__ __forceinline__ float bias_log2(float b) {
     const float x = b * LOG2E;
     return __builtin_isinf(x) && !__builtin_isinf(b) ? copysignf(3.402823466e38f, b) : x;
 }
-__device__ __forceinline__ Bias load_bias(const Attn& a, char* lds, int hk) {
-    Bias s;
-    unsigned char* lut = (unsigned char*)lds;
-    float* tbl = (float*)(lds + (2 * a.maxd + 1 + 3) / 4 * 4);
-    s.lut = lut;
-    s.tbl = tbl;
+__host__ __device__ inline int bias_lut_bytes(int nbuckets, int maxd) { return nbuckets ? (2 * maxd + 1 + 15) / 16 * 16 : 0; }
+// the table of buckets by the whole workgroup, a key head's biases by `n` threads
+__device__ __forceinline__ Bias load_bias(const Attn& a, unsigned char* lut, float* tbl, int hk, int t, int n) {
     if (a.nbuckets) {
         for (int i = threadIdx.x; i < 2 * a.maxd + 1; i += blockDim.x) lut[i] = (unsigned char)min(max(a.bucket_of[i], 0), a.nbuckets - 1);
-        for (int i = threadIdx.x; i < a.nbuckets * a.G; i += blockDim.x) tbl[i] = bias_log2(a.bias[(size_t)(i / a.G) * a.Hq + hk * a.G + i % a.G]);
+        for (int i = t; i < a.nbuckets * a.G; i += n) tbl[i] = bias_log2(a.bias[(size_t)(i / a.G) * a.Hq + hk * a.G + i % a.G]);
     }
-    return s;
+    return Bias{lut, tbl};
 }
 __device__ __forceinline__ int clamp_dist(int d, int maxd) { return min(max(d, -maxd), maxd) + maxd; }
 __device__ __forceinline__ int tile_key(int r, int hi) { return 8 * (r >> 2) + 4 * hi + (r & 3); }
@@ -401,6 +484,6 @@ __device__ __forceinline__ void tile_bias(const Attn& a, const Bias& s, int key0
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = s.tbl[d[r] * a.G + gl];
 }
-inline size_t bias_lds(int nbuckets, int maxd, int G) { return nbuckets ? ((size_t)(2 * maxd + 1 + 3) / 4 * 4 + (size_t)nbuckets * G * 4 + 15) / 16 * 16 : 0; }
+inline size_t bias_lds(int nbuckets, int maxd, int G) { return (size_t)bias_lut_bytes(nbuckets, maxd) + ((size_t)nbuckets * G * 4 + 15) / 16 * 16; }
 
 }  // namespace scipnp

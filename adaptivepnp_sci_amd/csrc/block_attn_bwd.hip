@@ -133,8 +133,9 @@ __global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
     int* const list = (int*)(smem + C::MAIN + C::KP);
     int* const nlist = list + a.n;
     char* const bias_at = smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16;
-    const Bias bias = load_bias(a, bias_at, hk);
-    float* const hist = (float*)(bias_at + (a.nbuckets ? ((2 * a.maxd + 1 + 3) / 4 * 4 + a.nbuckets * a.G * 4 + 15) / 16 * 16 : 0));
+    const int lut_bytes = bias_lut_bytes(a.nbuckets, a.maxd);
+    const Bias bias = load_bias(a, (unsigned char*)bias_at, (float*)(bias_at + lut_bytes), hk, threadIdx.x, 256);
+    float* const hist = (float*)(bias_at + lut_bytes + (a.nbuckets * a.G * 4 + 15) / 16 * 16);
     float* const mine = hist + wave * a.nbuckets * HROW + lane;
     for (int i = 0; i < a.nbuckets; ++i) mine[i * HROW] = 0.f;
     if (wave == 0) {
@@ -354,7 +355,8 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
     char* const main = smem;
     int* const list = (int*)(smem + C::MAIN);
     int* const misc = list + C::LIST;                     // block, scan
-    const Bias bias = load_bias(a, smem + C::MAIN + (C::LIST + 8) * 4, hk);
+    char* const bias_at = smem + C::MAIN + (C::LIST + 8) * 4;
+    const Bias bias = load_bias(a, (unsigned char*)bias_at, (float*)(bias_at + bias_lut_bytes(a.nbuckets, a.maxd)), hk, tid, 256);
     for (int j = tid; j < a.nb; j += 256)
         if (cs[j] <= c && c < cs[j + 1]) misc[0] = j;
     __syncthreads();
