@@ -24,72 +24,6 @@ template <> struct Mat<float> {
     static constexpr int K = 8;                           // four v_mfma_f32_32x32x2_f32 a fragment
 };
 
-// element stride of an LDS tile that is read row-wise (16 bytes of 32 rows): 4 banks further each row
-template <typename T, int DP> constexpr int row_stride() { return DP + Mat<T>::E; }
-// ... of one that is only read transposed: bf16 4 rows x 32 columns cover the 64 banks once; fp32 rows 4 apart are 32 banks apart
-template <typename T, int DP> constexpr int col_stride() { return sizeof(T) == 2 ? (DP == 128 ? 160 : DP == 64 ? 96 : DP) : DP + 8; }
-
-// acc += A B^T over DP: A = the tile's row li (LDS), B = fragments in registers
-template <typename T, int DP>
-__device__ __forceinline__ f32x16a mma_rows(const T* row, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int hi, f32x16a acc) {
-#pragma unroll
-    for (int s = 0; s < DP / Mat<T>::K; ++s) {
-        if constexpr (sizeof(T) == 2) {
-            const bf16x8 a = *(const bf16x8*)(row + 16 * s + 8 * hi);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[s], acc, 0, 0, 0);
-        } else {
-            const f32x4a a = *(const f32x4a*)(row + 8 * s + 4 * hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[s][j], acc, 0, 0, 0);
-        }
-    }
-    return acc;
-}
-
-// acc[db] += X^T P over the tile's 32 rows: X the tile (element stride ST), P in an accumulator's registers, rounded to T.
-// exact (bf16): P as three bf16 numbers that add up to its 24 bits, three products
-template <typename T, int DP, int ST>
-__device__ __forceinline__ void mma_cols(const T* tile, const f32x16a& p, int lane, f32x16a (&acc)[DP / 32], bool exact = false) {
-    const int li = lane & 31, hi = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-        // transposing read: the 16 lanes of a group supply 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows
-        const int q = (lane >> 2) & 3, c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            bf16x8 b, b1, b2;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = (__bf16)p[8 * k + i];
-            if (exact) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float r1 = p[8 * k + i] - (float)b[i];
-                    b1[i] = (__bf16)r1;
-                    b2[i] = (__bf16)(r1 - (float)b1[i]);
-                }
-            }
-            const T* base = tile + (16 * k + 4 * hi + q) * ST + c;
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db) {
-                union { s16x4a s[2]; bf16x8 v; } u;
-                u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4a*)(base + 32 * db));
-                u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4a*)(base + 8 * ST + 32 * db));
-                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, b, acc[db], 0, 0, 0);
-                if (exact) {
-                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, b1, acc[db], 0, 0, 0);
-                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, b2, acc[db], 0, 0, 0);
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const T* x = tile + (8 * (r >> 2) + 4 * hi + (r & 3)) * ST + li;
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[32 * db], p[r], acc[db], 0, 0, 0);
-        }
-    }
-}
-
 // fragments of one row in global memory (nullptr: zeros); columns past D are zero
 template <typename T, int DP>
 __device__ __forceinline__ void load_frags(const T* row, int D, int hi, typename Mat<T>::Frag (&f)[DP / Mat<T>::K]) {
@@ -102,33 +36,6 @@ __device__ __forceinline__ void load_frags(const T* row, int D, int hi, typename
             for (int i = 0; i < Mat<T>::E; ++i) f[s][i] = (T)0.f;
     }
 }
-
-// ---- a tile on its way from global memory to LDS: 32 rows of DP elements, NTH threads, 16 bytes each
-template <typename T, int DP, int NTH>
-struct TileRegs {
-    static constexpr int C = DP / Mat<T>::E;              // 16-byte chunks of a row
-    static constexpr int N = (KT * C + NTH - 1) / NTH;
-    static constexpr bool EVEN = KT * C % NTH == 0;
-    f32x4a v[N];
-    // row_of(i): address of row i's first element, nullptr for a row that is zeros
-    template <typename F>
-    __device__ __forceinline__ void load(int t, int D, F row_of) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int x = t + i * NTH, r = x / C, c = (x - r * C) * Mat<T>::E;
-            const T* p = EVEN || r < KT ? row_of(r) : nullptr;
-            v[i] = (p && c < D) ? *(const f32x4a*)(p + c) : f32x4a{0.f, 0.f, 0.f, 0.f};
-        }
-    }
-    template <int ST>
-    __device__ __forceinline__ void store(int t, T* tile) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int x = t + i * NTH, r = x / C, c = (x - r * C) * Mat<T>::E;
-            if (EVEN || r < KT) *(f32x4a*)(tile + r * ST + c) = v[i];
-        }
-    }
-};
 
 // ---- a tile that the memory system writes into LDS itself (buffer_load ... lds: no registers, no address arithmetic per tile)
 //
@@ -401,7 +308,8 @@ struct Attn {
     float *po, *pml;                                      // forward, splits > 1: partial results, their maxima and sums
     // backward
     const float* delta;
-    unsigned* member;                                     // [b, hk][key block][ng bits]
+    float* zeros;                                         // 256 bytes
+    unsigned* member;                                     // [b, hk][key block][ng bits], then [b, hk][key block] counts
     int words;
     const int* chunk_start;                               // [b, hk][key block + 1]
     int max_chunks;

@@ -21,11 +21,12 @@ __device__ __forceinline__ unsigned fast_div(unsigned x, unsigned d, unsigned m,
 }
 static inline unsigned div_magic(int d) { return d <= 1 ? 0xFFFFFFFFu : (unsigned)((1ull << 32) / (unsigned)d); }
 
-// ---- delta of every live row (16 lanes a row), and the membership bits cleared for the launch behind it
+// ---- delta of every live row (16 lanes a row), and the membership bits (and counts) cleared for the launch behind it
 template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(Attn a, float* delta, size_t member_words) {
     const size_t rows = (size_t)a.B * a.Lq * a.Hq;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < member_words; i += (size_t)gridDim.x * 256) a.member[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 64) a.zeros[threadIdx.x] = 0;      // what the rows that do not exist are read from
     for (size_t id = (size_t)blockIdx.x * 16 + (threadIdx.x >> 4); id < rows; id += (size_t)gridDim.x * 16) {
         const int head = (int)(id % a.Hq), tok = (int)(id / a.Hq % a.Lq), b = (int)(id / a.Hq / a.Lq), l16 = threadIdx.x & 15;
         float s = 0.f;
@@ -45,7 +46,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(Attn a, float* delta, s
     }
 }
 
-// ---- the selection the other way round: one wave a query group sets its bit in each of its blocks (an OR: no order)
+// ---- the selection the other way round: one wave a query group sets its bit in each of its blocks and counts itself (whole numbers: no order)
 __global__ void __launch_bounds__(256) attn_mark_kernel(Attn a) {
     extern __shared__ int lists[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -59,7 +60,11 @@ __global__ void __launch_bounds__(256) attn_mark_kernel(Attn a) {
     const int far = a.causal ? min(s.klen, s.shift + q0 + nq) : s.klen;
     const int c = live_blocks(a, a.sel + (size_t)item * a.n, far, list, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int i = lane; i < c; i += 64) atomicOr(&a.member[((size_t)bh * a.nb + list[i]) * a.words + (g >> 5)], 1u << (g & 31));
+    unsigned* const counts = a.member + (size_t)a.B * a.Hk * a.nb * a.words;
+    for (int i = lane; i < c; i += 64) {
+        atomicOr(&a.member[((size_t)bh * a.nb + list[i]) * a.words + (g >> 5)], 1u << (g & 31));
+        atomicAdd(&counts[(size_t)bh * a.nb + list[i]], 1u);
+    }
 }
 
 // ---- chunks of every key block of one (sequence, key head): chunk_start[j] = chunks of the blocks before j
@@ -73,9 +78,8 @@ __global__ void __launch_bounds__(256) attn_plan_kernel(Attn a, int* chunk_start
         const int j = base + tid;
         int c = 0;
         if (j < a.nb) {
-            const unsigned* w = a.member + ((size_t)bh * a.nb + j) * a.words;
-            for (int i = 0; i < a.words; ++i) c += __popc(w[i]);
-            c = (int)(((long long)c * R + CH - 1) / CH);
+            const unsigned* counts = a.member + (size_t)a.B * a.Hk * a.nb * a.words;
+            c = (int)(((long long)counts[(size_t)bh * a.nb + j] * R + CH - 1) / CH);
         }
         int incl = c;
         for (int off = 1; off < 64; off <<= 1) {
@@ -94,51 +98,51 @@ __global__ void __launch_bounds__(256) attn_plan_kernel(Attn a, int* chunk_start
     if (tid == 0) cs[a.nb] = carry;
 }
 
-// ---- dQ, dbias: the forward's workgroup and tiles
-template <typename T, int DP, int RW>
+// ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums of a lane's row: one LDS word a bucket and lane, the two ends
+// (where most tiles lie) in registers
+template <typename T, int DP>
 struct DqCfg {
-    static constexpr int KS = 4 / RW, NTH = 64 * RW, ST = row_stride<T, DP>();
-    static constexpr int TILE = 2 * KT * ST * (int)sizeof(T);
-    // private tiles need one buffer; the widest fp32 tiles leave room for one beside the bias sums (then a second barrier)
-    static constexpr int BUFS = KS == 4 || (KS == 2 && sizeof(T) == 4 && DP >= 96) ? 1 : 2;
-    static constexpr int OST = DP + 4;
-    static constexpr int JOIN = KS > 1 ? RW * 32 * OST * 4 : 0;
-    static constexpr int TILES = KS * BUFS * TILE;
-    static constexpr int MAIN = TILES > JOIN ? TILES : JOIN;
-    static constexpr int KP = KS * BUFS * KT * 4;
+    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
+    static constexpr int MAIN = 2 * TILE;
+    static constexpr int KP = 2 * KT * 4;
 };
 constexpr int HROW = 65;                                  // a bucket's 64 lane sums, rows shifted by a bank
 
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
+__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using C = DqCfg<T, DP, RW>;
+    using C = DqCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    const long long total = (long long)a.B * a.Hk * a.ng * a.chunks, item = xcd_item(blockIdx.x, total);
-    if (item < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hi = lane >> 5;
-    const int rw = wave % RW, ks = wave / RW, tsplit = rw * 64 + lane;
-    const int chunk = (int)(item % a.chunks), g = (int)(item / a.chunks % a.ng), bh = (int)(item / a.chunks / a.ng), hk = bh % a.Hk, b = bh / a.Hk;
+    constexpr int NB = (DP + 31) / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
+    const long long total = (long long)a.B * a.Hk * a.ng * a.chunks, first = xcd_item(blockIdx.x, (total + sets - 1) / sets);
+    if (first < 0) return;
+    const int lane = threadIdx.x & 63, li = lane & 31, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int set = wave / RW, rw = wave % RW, tset = rw * 64 + lane;
+    const bool there_is = first * sets + set < total;
+    const unsigned item = there_is ? (unsigned)(first * sets + set) : 0;
+    const int chunk = item % a.chunks, g = item / a.chunks % a.ng, bh = item / a.chunks / a.ng, hk = bh % a.Hk, b = bh / a.Hk;
     const Seq sq = seq_of(a, b);
     const int R = a.qb * a.G, r0 = chunk * 32 * RW;
     const int row = r0 + rw * 32 + li, tok = g * a.qb + row / a.G, gl = row % a.G, head = hk * a.G + gl;
-    const bool live = row < R && tok < sq.qlen;
+    const bool live = there_is && row < R && tok < sq.qlen;
     const int qkey = sq.shift + tok;
     const int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;
-    const bool any = g * a.qb + r0 / a.G < sq.qlen;       // (uniform) a live row in this chunk
+    const bool any = there_is && g * a.qb + r0 / a.G < sq.qlen;             // a live row in this chunk
 
-    char* const main = smem;
+    unsigned char* const lut = (unsigned char*)smem_all;
+    int* const longest = (int*)(smem_all + bias_lut_bytes(a.nbuckets, a.maxd));
+    char* const smem = smem_all + bias_lut_bytes(a.nbuckets, a.maxd) + 16 + set * set_bytes;
     int* const kp_lds = (int*)(smem + C::MAIN);
     int* const list = (int*)(smem + C::MAIN + C::KP);
     int* const nlist = list + a.n;
-    char* const bias_at = smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16;
-    const int lut_bytes = bias_lut_bytes(a.nbuckets, a.maxd);
-    const Bias bias = load_bias(a, (unsigned char*)bias_at, (float*)(bias_at + lut_bytes), hk, threadIdx.x, 256);
-    float* const hist = (float*)(bias_at + lut_bytes + (a.nbuckets * a.G * 4 + 15) / 16 * 16);
-    float* const mine = hist + wave * a.nbuckets * HROW + lane;
+    float* const tbl = (float*)(smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16);
+    const Bias bias = load_bias(a, lut, tbl, hk, tset, 64 * RW);
+    float* const hist = tbl + (a.nbuckets * a.G + 3) / 4 * 4;
+    float* const mine = hist + rw * a.nbuckets * HROW + lane;
     for (int i = 0; i < a.nbuckets; ++i) mine[i * HROW] = 0.f;
-    if (wave == 0) {
+    if (threadIdx.x == 0) *longest = 0;
+    if (rw == 0) {
         int c = 0;
         if (any) {
             const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
@@ -153,161 +157,129 @@ __global__ void __launch_bounds__(256) block_attn_dq_kernel(Attn a) {
     const size_t stat = ((size_t)b * a.Hq + head) * a.Lq + tok;
     const float lse = live ? a.lse[stat] * LOG2E : 0.f, delta = live ? a.delta[stat] : 0.f;
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
-    RowRange range = {live ? qp : INT_MAX, live ? qp : INT_MIN};
-    int min_lim = live ? lim : INT_MAX, max_lim = lim;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        range.lo = min(range.lo, __shfl_xor(range.lo, off, 64));
-        range.hi = max(range.hi, __shfl_xor(range.hi, off, 64));
-        min_lim = min(min_lim, __shfl_xor(min_lim, off, 64));
-        max_lim = max(max_lim, __shfl_xor(max_lim, off, 64));
-    }
-    range.lo = __builtin_amdgcn_readfirstlane(range.lo);
-    range.hi = __builtin_amdgcn_readfirstlane(range.hi);
-    min_lim = __builtin_amdgcn_readfirstlane(min_lim);
-    max_lim = __builtin_amdgcn_readfirstlane(max_lim);
+    const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
+    const int min_lim = wave_min(live ? lim : INT_MAX), max_lim = wave_max(lim);
+    const unsigned ks = (unsigned)(a.sk.t * (long long)sizeof(T)), vs = (unsigned)(a.sv.t * (long long)sizeof(T));
+    DmaOffsets<T, DP, RW> ko, vo;
+    ko.init(rw, lane, ks, a.D);
+    vo.init(rw, lane, vs, a.D);
     __syncthreads();
 
-    const int tpb = a.block / KT, ntiles = *nlist * tpb, iters = (ntiles + C::KS - 1) / C::KS;
+    const int tpb = a.block / KT, count = __builtin_amdgcn_readfirstlane(*nlist) * tpb;
+    int trips = count;                                    // sets that share a barrier take the same number of trips
+    if constexpr (RW > 1) {
+        if (sets > 1) {
+            if (tset == 0) atomicMax(longest, count);
+            __syncthreads();
+            trips = __builtin_amdgcn_readfirstlane(*longest);
+        }
+    }
     const T* const kb = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
     const T* const vb = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
-    TileRegs<T, DP, C::NTH> kr, vr;
-    int kpr = 0;
-    auto key0_of = [&](int it) -> int {
-        const int t = it * C::KS + ks;
-        if (t >= ntiles) return -1;
-        const int blk = t / tpb;
-        return list[blk] * a.block + (t - blk * tpb) * KT;
+    int kpr = 0, blk = 0, off = 0;                        // the next tile to ask for
+    auto next_key = [&]() -> int {
+        const int key = __builtin_amdgcn_readfirstlane(list[blk]) * a.block + off;
+        off += KT;
+        if (off == a.block) { off = 0; ++blk; }
+        return key;
     };
-    auto load = [&](int key0) {
-        if (key0 < 0) return;
-        kr.load(tsplit, a.D, [&](int r) { return key0 + r < sq.klen ? kb + (long long)(key0 + r) * a.sk.t : nullptr; });
-        vr.load(tsplit, a.D, [&](int r) { return key0 + r < sq.klen ? vb + (long long)(key0 + r) * a.sv.t : nullptr; });
-        if (a.k_pos && tsplit < KT) kpr = key0 + tsplit < sq.klen ? a.k_pos[(size_t)b * a.Lk + key0 + tsplit] : 0;
+    auto issue = [&](int key0, int buf) {
+        const int there = min(KT, sq.klen - key0);
+        if (there <= 0) return;
+        char* const tile = smem + buf * C::TILE;
+        ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
+        vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
+        if (a.k_pos && tset < KT) kpr = tset < there ? a.k_pos[(size_t)b * a.Lk + key0 + tset] : 0;
     };
-    f32x16a o[DP / 32];
+    const int far = 2 * a.maxd;
+    const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
+    float sum_lo = 0.f, sum_hi = 0.f;
+    f32x16a o[NB];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
 
-    int key0 = iters ? key0_of(0) : -1;
-    load(key0);
-    for (int it = 0; it < iters; ++it) {
-        const int buf = C::BUFS == 2 ? (it & 1) : 0;
-        T* const kt = (T*)(main + (ks * C::BUFS + buf) * C::TILE);
-        T* const vt = kt + KT * C::ST;
-        int* const kp = kp_lds + (ks * C::BUFS + buf) * KT;
-        if (key0 >= 0) {
-            kr.template store<C::ST>(tsplit, kt);
-            vr.template store<C::ST>(tsplit, vt);
-            if (a.k_pos && tsplit < KT) kp[tsplit] = kpr;
-        }
-        if constexpr (C::KS < 4) __syncthreads();
-        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const int cur = key0;
-        key0 = it + 1 < iters ? key0_of(it + 1) : -1;
-        load(key0);
-        if (cur >= 0 && cur <= max_lim) {
-            f32x16a s, dp;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-            s = mma_rows<T, DP>(kt + li * C::ST, qf, hi, s);
-            dp = mma_rows<T, DP>(vt + li * C::ST, gf, hi, dp);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] *= a.scale2;
-            int dist = -1;
-            if (a.nbuckets) {
-                dist = tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane);
-                if (dist >= 0) {
-                    const float bv = bias.tbl[bias.lut[dist] * a.G + gl];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] += bv;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int k = a.k_pos ? kp[tile_key(r, hi)] : cur + tile_key(r, hi);
-                        s[r] += bias.tbl[bias.lut[clamp_dist(k - qp, a.maxd)] * a.G + gl];
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(s[r] - lse);
-                s[r] = cur + tile_key(r, hi) <= lim ? p * (dp[r] - delta) : 0.f;
-            }
-            if (a.dbias) {
-                if (dist >= 0) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += s[r];
-                    mine[bias.lut[dist] * HROW] += sum;
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int k = a.k_pos ? kp[tile_key(r, hi)] : cur + tile_key(r, hi);
-                        mine[bias.lut[clamp_dist(k - qp, a.maxd)] * HROW] += s[r];
-                    }
-                }
-            }
-            mma_cols<T, DP, C::ST>(kt, s, lane, o);
-        }
-        if constexpr (C::KS == 4) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        else if constexpr (C::BUFS == 1) __syncthreads();
+    int key0 = 0;
+    if (count > 0) {
+        key0 = next_key();
+        issue(key0, 0);
     }
-    if (a.dbias) {                                        // the workgroup's sums: a (bucket, head) adds its lanes in order, in fp64
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.nbuckets * a.G; i += 256) {
-            const int n = i / a.G, h = i - n * a.G;
-            double sum = 0.0;
-            for (int w = 0; w < 4; ++w)
-                for (int x = 0; x < 64; ++x)
-                    if ((r0 + (w % RW) * 32 + (x & 31)) % a.G == h) sum += (double)hist[(w * a.nbuckets + n) * HROW + x];
-            a.pbias[(size_t)item * a.nbuckets * a.G + i] = sum;
+    for (int t = 0; t < trips; ++t) {
+        const int buf = t & 1, cur = key0;
+        int* const kp = kp_lds + buf * KT;
+        if (a.k_pos && tset < KT) kp[tset] = kpr;
+        dma_wait<RW>();
+        if (t + 1 < count) {
+            key0 = next_key();
+            issue(key0, buf ^ 1);
         }
-    }
-    if constexpr (C::KS > 1) {
-        float* const obuf = (float*)main + rw * 32 * C::OST;
-        __syncthreads();
-        for (int k = C::KS - 1; k >= 0; --k) {
-            if (ks == k) {
+        if (t >= count || cur > max_lim) continue;
+        const char* const kt = smem + buf * C::TILE;
+        f32x16a s = dma_rows<T, DP>(kt, qf, lane);
+        const f32x16a dp = dma_rows<T, DP>(kt + DmaTile<T, DP>::BYTES, gf, lane);
+        ColTile<T, DP> kc;
+        kc.read(kt, lane);
+        const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
+        float x[16];
+        if (dist >= 0) {
+            float add = 0.f;
+            if (a.nbuckets) add = dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
+            for (int r = 0; r < 16; ++r) x[r] = add - lse;
+        } else {
+            tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        f32x4a* const p = (f32x4a*)(obuf + li * C::OST + 32 * db + 8 * q + 4 * hi);
-                        f32x4a v = f32x4a{o[db][4 * q], o[db][4 * q + 1], o[db][4 * q + 2], o[db][4 * q + 3]};
-                        if (k < C::KS - 1) v += *p;
-                        if (k > 0) *p = v;
-                        else
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[db][4 * q + e] = v[e];
-                    }
-            }
-            if (k > 0) __syncthreads();
+            for (int r = 0; r < 16; ++r) x[r] -= lse;
         }
-        if (ks > 0) return;
-    }
-    if (row >= R || tok >= a.Lq) return;
-    T* const dst = (T*)a.dq + (((size_t)b * a.Lq + tok) * a.Hq + head) * a.D;
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, x[r])) * (dp[r] - delta);
+        if (cur + KT - 1 > min_lim) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = 32 * db + 8 * q + 4 * hi;
-            if (d >= a.D) continue;
-            f32x4a v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = live ? o[db][4 * q + e] * a.scale : 0.f;
-            if constexpr (sizeof(T) == 2) {
-                bf16x4 w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (__bf16)v[e];
-                *(bf16x4*)(dst + d) = w;
+            for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : 0.f;
+        }
+        if (a.dbias) {
+            if (dist >= 0) {
+                const float sum = (((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]))) +
+                                  (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
+                if (dist == 0) sum_lo += sum;
+                else if (dist == far) sum_hi += sum;
+                else mine[bias.lut[dist] * HROW] += sum;
             } else {
-                *(f32x4a*)(dst + d) = v;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int k = a.k_pos ? kp[tile_key(r, hi)] : cur + tile_key(r, hi);
+                    mine[bias.lut[clamp_dist(k - qp, a.maxd)] * HROW] += s[r];
+                }
             }
         }
+        kc.mma(s, o);
+    }
+    if (a.dbias) {                                        // the set's sums: a (bucket, head) adds its lanes in order, in fp64
+        mine[bias.lut[0] * HROW] += sum_lo;
+        mine[bias.lut[far] * HROW] += sum_hi;
+        __syncthreads();
+        if (there_is)
+            for (int i = tset; i < a.nbuckets * a.G; i += 64 * RW) {
+                const int n = i / a.G, h = i - n * a.G;
+                double sum = 0.0;
+                for (int w = 0; w < RW; ++w) {
+                    const int at = (r0 + w * 32) % a.G;
+                    for (int y = (h - at + a.G) % a.G; y < 32; y += a.G)
+                        sum += (double)hist[(w * a.nbuckets + n) * HROW + y] + (double)hist[(w * a.nbuckets + n) * HROW + y + 32];
+                }
+                a.pbias[(size_t)item * a.nbuckets * a.G + i] = sum;
+            }
+    }
+    if (!there_is || row >= R || tok >= a.Lq) return;
+    T* const dst = (T*)a.dq + (((size_t)b * a.Lq + tok) * a.Hq + head) * a.D;
+    each_four<T, NB>(hi, [&](int d, auto at) {
+        if (d >= a.D) return;
+        f32x4a v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live ? o[at(e) >> 4][at(e) & 15] * a.scale : 0.f;
+        store_four(dst + d, v);
+    });
 #endif
 }
 
@@ -325,33 +297,36 @@ __global__ void __launch_bounds__(64) attn_dbias_kernel(Attn a) {
 }
 
 // ---- dK, dV of 64 keys over one chunk of the query rows that chose their block.  Waves: two halves of the keys x two of the row tiles;
-// a wave keeps its 32 keys and values in registers (the B operands) and streams rows: S, dP with the rows as A, then dV += dO^T P and
+// a wave keeps its 32 keys and values in registers (the B operands) and streams rows, which the memory system writes to LDS
+// (global_load ... lds: the rows of a tile may belong to several query groups): S, dP with the rows as A, then dV += dO^T P and
 // dK += Q^T dS with the transposed rows as A and the score registers as B.
+// What a row brings besides: its last visible key, delta, and bias - lse where all 64 keys share its bucket.
 template <typename T, int DP>
 struct DkvCfg {
-    static constexpr int ST = row_stride<T, DP>();
-    static constexpr int INFO = KT * 20;                  // lse, delta, last key, position, head of each row
-    static constexpr int TILE = 2 * KT * ST * (int)sizeof(T) + INFO;
+    static constexpr int INFO = KT * 20 + 16;             // bias - lse (or - lse), delta, last key, position, head of each row; flags
+    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES + INFO;
     static constexpr int MAIN = 4 * TILE;                 // two row tiles, two buffers
     static constexpr int OST = DP + 4;
-    static constexpr int JOIN = 2 * 32 * OST * 4;
+    static constexpr int JOIN = 2 * 32 * ((DP + 31) / 32 * 32 + 4) * 4;
     static_assert(JOIN <= MAIN, "the join reuses the tiles");
     static constexpr int LIST = 1032;                     // query groups of a chunk
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int subs, unsigned magic_r, unsigned magic_g) {
+__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(Attn a, int CH, int subs, unsigned magic_r, unsigned magic_g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DkvCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
+    constexpr int NB = (DP + 31) / 32, LC = DmaTile<T, DP>::LC, PIECES = DmaTile<T, DP>::PIECES, MINE = (PIECES + 1) / 2, BYTES = DmaTile<T, DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long total = (long long)a.B * a.Hk * a.max_chunks * subs, item = xcd_item(blockIdx.x, total);
     if (item < 0) return;
-    const int sub = (int)(item % subs), c = (int)(item / subs % a.max_chunks), bh = (int)(item / subs / a.max_chunks), hk = bh % a.Hk, b = bh / a.Hk;
+    const unsigned it0 = (unsigned)item;
+    const int sub = it0 % subs, c = it0 / subs % a.max_chunks, bh = it0 / subs / a.max_chunks, hk = bh % a.Hk, b = bh / a.Hk;
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     if (c >= cs[a.nb]) return;                            // (uniform)
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hi = lane >> 5, kw = wave & 1, rs = wave >> 1;
-    const int tsplit = kw * 64 + lane;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave & 1, rs = wave >> 1, tsplit = kw * 64 + lane;
     char* const main = smem;
     int* const list = (int*)(smem + C::MAIN);
     int* const misc = list + C::LIST;                     // block, scan
@@ -360,7 +335,7 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
     for (int j = tid; j < a.nb; j += 256)
         if (cs[j] <= c && c < cs[j + 1]) misc[0] = j;
     __syncthreads();
-    const int j = misc[0], nchunks = cs[j + 1] - cs[j];
+    const int j = __builtin_amdgcn_readfirstlane(misc[0]), nchunks = cs[j + 1] - cs[j];
     const int R = a.qb * a.G;
     const Seq sq = seq_of(a, b);
     // the chunk's rows are x0 .. x1 of the block's groups laid end to end; their groups into the list
@@ -391,16 +366,22 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
     const unsigned x1 = (unsigned)min((long long)x0 + CH, (long long)count * R);
     const int e0 = (int)(x0 / R);
 
-    const int kbase = j * a.block + sub * KB + kw * 32, key = kbase + li;
+    const int k64 = j * a.block + sub * KB, kbase = k64 + kw * 32, key = kbase + li;
     const bool klive = key < sq.klen;
     Frag kf[DP / Mat<T>::K], vf[DP / Mat<T>::K];
     load_frags<T, DP>(klive ? (const T*)a.k + b * a.sk.b + (long long)key * a.sk.t + hk * a.sk.h : nullptr, a.D, hi, kf);
     load_frags<T, DP>(klive ? (const T*)a.v + b * a.sv.b + (long long)key * a.sv.t + hk * a.sv.h : nullptr, a.D, hi, vf);
     const int kpos = a.k_pos ? (klive ? a.k_pos[(size_t)b * a.Lk + key] : 0) : key;
+    int klo = k64, khi = k64 + KB - 1;                    // positions of the 64 keys
+    if (a.k_pos) {
+        const int mine = k64 + lane < sq.klen ? a.k_pos[(size_t)b * a.Lk + k64 + lane] : INT_MAX;
+        klo = wave_min(mine);
+        khi = wave_max(k64 + lane < sq.klen ? mine : INT_MIN);
+    }
 
-    f32x16a dk[DP / 32], dv[DP / 32];
+    f32x16a dk[NB], dv[NB];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) { dk[db][r] = 0.f; dv[db][r] = 0.f; }
 
@@ -414,27 +395,33 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
         const int t = list[(int)e - e0] * a.qb + (int)q;
         if (t < sq.qlen) { tok = t; gl = (int)h; }
     };
-    TileRegs<T, DP, 128> qr, gr;
-    float ilse = 0.f, idelta = 0.f;
+    const T* const qb0 = (const T*)a.q + b * a.sq.b + hk * a.G * a.sq.h;
+    const T* const gb0 = (const T*)a.dout + b * a.sdo.b + hk * a.G * a.sdo.h;
+    float iadd = 0.f, idelta = 0.f;
     int ilim = -1, iqp = 0, ig = 0;
-    auto load = [&](unsigned x) {                         // rows x .. x + 31
-        qr.load(tsplit, a.D, [&](int r) -> const T* {
-            int tok, gl;
-            row_of(x + r, tok, gl);
-            return tok < 0 ? nullptr : (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + (hk * a.G + gl) * a.sq.h;
-        });
-        gr.load(tsplit, a.D, [&](int r) -> const T* {
-            int tok, gl;
-            row_of(x + r, tok, gl);
-            return tok < 0 ? nullptr : (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + (hk * a.G + gl) * a.sdo.h;
-        });
+    auto load = [&](unsigned x, int buf) {                // rows x .. x + 31
+        char* const tile = main + (rs * 2 + buf) * C::TILE;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int piece = kw + 2 * i;
+            if (PIECES % 2 == 0 || piece < PIECES) {
+                const int y = piece * 64 + lane, r = y / LC, ch = (y % LC) ^ swz<T, LC>(r);
+                int tok, gl;
+                row_of(x + r, tok, gl);
+                const bool ok = tok >= 0 && ch * Mat<T>::E < a.D;
+                const T* const qa = ok ? qb0 + tok * a.sq.t + gl * a.sq.h + ch * Mat<T>::E : (const T*)a.zeros;
+                const T* const ga = ok ? gb0 + tok * a.sdo.t + gl * a.sdo.h + ch * Mat<T>::E : (const T*)a.zeros;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)qa, (__attribute__((address_space(3))) void*)(tile + 1024 * piece), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ga, (__attribute__((address_space(3))) void*)(tile + BYTES + 1024 * piece), 16, 0, 0);
+            }
+        }
         if (tsplit < KT) {
             int tok, gl;
             row_of(x + tsplit, tok, gl);
-            ilim = -1; ilse = idelta = 0.f; iqp = 0; ig = gl;
+            ilim = -1; iadd = idelta = 0.f; iqp = 0; ig = gl;
             if (tok >= 0) {
                 const size_t stat = ((size_t)b * a.Hq + hk * a.G + gl) * a.Lq + tok;
-                ilse = a.lse[stat] * LOG2E;
+                iadd = a.lse[stat];
                 idelta = a.delta[stat];
                 ilim = a.causal ? min(sq.shift + tok, sq.klen - 1) : sq.klen - 1;
                 iqp = a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : sq.shift + tok;
@@ -442,71 +429,84 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
         }
     };
     const int iters = (int)((x1 - x0 + 2 * KT - 1) / (2 * KT));
-    load(x0 + rs * KT);
+    load(x0 + rs * KT, 0);
     for (int it = 0; it < iters; ++it) {
         char* const at = main + (rs * 2 + (it & 1)) * C::TILE;
-        T* const qt = (T*)at;
-        T* const gt = qt + KT * C::ST;
-        float* const info = (float*)(at + 2 * KT * C::ST * (int)sizeof(T));
-        qr.template store<C::ST>(tsplit, qt);
-        gr.template store<C::ST>(tsplit, gt);
+        float* const info = (float*)(at + 2 * BYTES);
         if (tsplit < KT) {
-            info[tsplit] = ilse;
+            float add = -iadd * LOG2E;
+            bool one = true;                              // every key has the same bucket for this row
+            if (a.nbuckets && ilim >= 0) {
+                const int lo = clamp_dist(klo - iqp, a.maxd);
+                one = lo == clamp_dist(khi - iqp, a.maxd);
+                if (one) add += bias.tbl[bias.lut[lo] * a.G + ig];
+            }
+            const bool all_one = __ballot(!one) == 0, open = __ballot(ilim < k64 + KB - 1) == 0;
+            if (!all_one) add = -iadd * LOG2E;
+            info[tsplit] = add;
             info[KT + tsplit] = idelta;
             ((int*)info)[2 * KT + tsplit] = ilim;
             ((int*)info)[3 * KT + tsplit] = iqp;
             ((int*)info)[4 * KT + tsplit] = ig;
+            if (tsplit == 0) ((int*)info)[5 * KT] = (all_one ? 1 : 0) | (open ? 2 : 0);
         }
-        __syncthreads();
-        if (it + 1 < iters) load(x0 + (it + 1) * 2 * KT + rs * KT);
-        f32x16a s, dp;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
-        s = mma_rows<T, DP>(qt + li * C::ST, kf, hi, s);
-        dp = mma_rows<T, DP>(gt + li * C::ST, vf, hi, dp);
+        dma_wait<4>();
+        if (it + 1 < iters) load(x0 + (it + 1) * 2 * KT + rs * KT, (it + 1) & 1);
+        const int flags = __builtin_amdgcn_readfirstlane(((int*)info)[5 * KT]);
+        f32x16a s = dma_rows<T, DP>(at, kf, lane);
+        f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
+        ColTile<T, DP> gc, qc;
+        gc.read(at + BYTES, lane);
+        qc.read(at, lane);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int r4 = 8 * q + 4 * hi;
-            const f32x4a lse = *(const f32x4a*)(info + r4), delta = *(const f32x4a*)(info + KT + r4);
-            const int4 lim = *(const int4*)((int*)info + 2 * KT + r4);
-            const int lims[4] = {lim.x, lim.y, lim.z, lim.w};
-            float add[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.nbuckets) {
+            f32x4a add = *(const f32x4a*)(info + r4);
+            const f32x4a delta = *(const f32x4a*)(info + KT + r4);
+            if (!(flags & 1)) {
                 const int4 qp = *(const int4*)((int*)info + 3 * KT + r4), gh = *(const int4*)((int*)info + 4 * KT + r4);
                 const int qps[4] = {qp.x, qp.y, qp.z, qp.w}, ghs[4] = {gh.x, gh.y, gh.z, gh.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) add[e] = bias.tbl[bias.lut[clamp_dist(kpos - qps[e], a.maxd)] * a.G + ghs[e]];
+                for (int e = 0; e < 4; ++e) add[e] += bias.tbl[bias.lut[clamp_dist(kpos - qps[e], a.maxd)] * a.G + ghs[e]];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * q + e;
-                const bool see = key <= lims[e];
-                const float p = see ? __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, add[e] - lse[e])) : 0.f;
-                s[r] = p;
-                dp[r] = see ? p * (dp[r] - delta[e]) : 0.f;
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, add[e]));
+                dp[r] = s[r] * (dp[r] - delta[e]);
+            }
+            if (!(flags & 2)) {
+                const int4 lim = *(const int4*)((int*)info + 2 * KT + r4);
+                const int lims[4] = {lim.x, lim.y, lim.z, lim.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool see = key <= lims[e];
+                    s[4 * q + e] = see ? s[4 * q + e] : 0.f;
+                    dp[4 * q + e] = see ? dp[4 * q + e] : 0.f;
+                }
             }
         }
-        mma_cols<T, DP, C::ST>(gt, s, lane, dv);
-        mma_cols<T, DP, C::ST>(qt, dp, lane, dk);
+        gc.mma(s, dv);
+        qc.mma(dp, dk);
     }
     // the two row halves: 1 into LDS, 0 adds
-    float* const obuf = (float*)main + kw * 32 * C::OST;
-    auto join = [&](f32x16a (&x)[DP / 32]) {
+    float* const obuf = (float*)main + kw * 32 * (NB * 32 + 4);
+    auto join = [&](f32x16a (&x)[NB]) {
         __syncthreads();
+        float* const p = obuf + li * (NB * 32 + 4) + 4 * hi;
         if (rs == 1) {
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+            for (int db = 0; db < NB; ++db)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *(f32x4a*)(obuf + li * C::OST + 32 * db + 8 * q + 4 * hi) = f32x4a{x[db][4 * q], x[db][4 * q + 1], x[db][4 * q + 2], x[db][4 * q + 3]};
+                for (int q = 0; q < 4; ++q) *(f32x4a*)(p + 32 * db + 8 * q) = f32x4a{x[db][4 * q], x[db][4 * q + 1], x[db][4 * q + 2], x[db][4 * q + 3]};
         }
         __syncthreads();
         if (rs == 0) {
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+            for (int db = 0; db < NB; ++db)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const f32x4a v = *(const f32x4a*)(obuf + li * C::OST + 32 * db + 8 * q + 4 * hi);
+                    const f32x4a v = *(const f32x4a*)(p + 32 * db + 8 * q);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[db][4 * q + e] += v[e];
                 }
@@ -516,31 +516,18 @@ __global__ void __launch_bounds__(256) block_attn_dkv_kernel(Attn a, int CH, int
     join(dk);
     if (rs == 1) return;
     const size_t slot = ((size_t)bh * a.max_chunks + c) * subs + sub;
+    auto put = [&](const f32x16a (&x)[NB], int which, T* dst, float scale) {
+        each_four<T, NB>(hi, [&](int d, auto at) {
+            if (d >= a.D) return;
+            f32x4a v;
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int d = 32 * db + 8 * q + 4 * hi;
-                if (d >= a.D) continue;
-                f32x4a v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = which ? dv[db][4 * q + e] : dk[db][4 * q + e] * a.scale;
-                if (nchunks > 1) {
-                    *(f32x4a*)(a.pkv + ((slot * 2 + which) * KB + kw * 32 + li) * a.D + d) = v;
-                } else if (key < a.Lk) {
-                    T* const dst = (T*)(which ? a.dv : a.dk) + (((size_t)b * a.Lk + key) * a.Hk + hk) * a.D + d;
-                    if constexpr (sizeof(T) == 2) {
-                        bf16x4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = (__bf16)v[e];
-                        *(bf16x4*)dst = w;
-                    } else {
-                        *(f32x4a*)dst = v;
-                    }
-                }
-            }
+            for (int e = 0; e < 4; ++e) v[e] = x[at(e) >> 4][at(e) & 15] * scale;
+            if (nchunks > 1) *(f32x4a*)(a.pkv + ((slot * 2 + which) * KB + kw * 32 + li) * a.D + d) = v;
+            else if (key < a.Lk) store_four(dst + (((size_t)b * a.Lk + key) * a.Hk + hk) * a.D + d, v);
+        });
+    };
+    put(dk, 0, (T*)a.dk, a.scale);
+    put(dv, 1, (T*)a.dv, 1.f);
 #endif
 }
 
@@ -551,28 +538,22 @@ __global__ void __launch_bounds__(256) attn_dkv_join_kernel(Attn a, int subs) {
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     const int c0 = cs[j], n = cs[j + 1] - c0;
     if (n == 1) return;
-    const int per = a.D / 4;
-    for (int i = threadIdx.x; i < KB * per; i += 256) {
-        const int k = i / per, d = 4 * (i - k * per), key = j * a.block + sub * KB + k;
-        if (key >= a.Lk) continue;
+    const int per = a.D / 4, i = blockIdx.z * 256 + threadIdx.x, which = i / (KB * per), k = i / per % KB, d = 4 * (i % per);
+    const int key = j * a.block + sub * KB + k;
+    if (which > 1 || key >= a.Lk) return;
+    f32x4a s = {0.f, 0.f, 0.f, 0.f};
+    const float* p = a.pkv + ((((size_t)bh * a.max_chunks + c0) * subs + sub) * 2 + which) * KB * a.D + (size_t)k * a.D + d;
+    const size_t step = (size_t)subs * 2 * KB * a.D;
+    int c = 0;
+    for (; c + 8 <= n; c += 8) {
+        f32x4a v[8];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            f32x4a s = {0.f, 0.f, 0.f, 0.f};
-            for (int c = 0; c < n; ++c) {
-                const size_t slot = ((size_t)bh * a.max_chunks + c0 + c) * subs + sub;
-                s += *(const f32x4a*)(a.pkv + ((slot * 2 + which) * KB + k) * a.D + d);
-            }
-            T* const dst = (T*)(which ? a.dv : a.dk) + (((size_t)b * a.Lk + key) * a.Hk + hk) * a.D + d;
-            if constexpr (sizeof(T) == 2) {
-                bf16x4 w;
+        for (int u = 0; u < 8; ++u) v[u] = *(const f32x4a*)(p + (c + u) * step);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = (__bf16)s[e];
-                *(bf16x4*)dst = w;
-            } else {
-                *(f32x4a*)dst = s;
-            }
-        }
+        for (int u = 0; u < 8; ++u) s += v[u];
     }
+    for (; c < n; ++c) s += *(const f32x4a*)(p + c * step);
+    store_four((T*)(which ? a.dv : a.dk) + (((size_t)b * a.Lk + key) * a.Hk + hk) * a.D + d, s);
 }
 
 struct BwdPlan {
@@ -583,7 +564,6 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
     BwdPlan p = {};
     p.R = a->query_block * (a->Hq / a->Hk);
     p.rw = p.R <= 32 ? 1 : p.R <= 64 ? 2 : 4;
-    if (p.rw == 1 && a->dtype == SCIPNP_F32 && a->D > 64) p.rw = 2;       // four private fp32 tiles of 128 would not fit beside the bias sums
     p.chunks = (p.R + 32 * p.rw - 1) / (32 * p.rw);
     p.subs = a->block / KB;
     p.ng = (a->Lq + a->query_block - 1) / a->query_block;
@@ -600,8 +580,8 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
     p.max_chunks = (int)(mc < (1ll << 30) ? mc : (1ll << 30));
     const size_t bh = (size_t)a->B * a->Hk;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    size_t at = up((size_t)a->B * a->Hq * a->Lq * 4);
-    p.o_member = at; at += up(bh * p.nb * p.words * 4);
+    size_t at = up((size_t)a->B * a->Hq * a->Lq * 4) + 256;                  // delta, zeros
+    p.o_member = at; at += up(bh * p.nb * (p.words + 1) * 4);                // bits, then counts
     p.o_chunk = at; at += up(bh * (p.nb + 1) * 4);
     p.o_pkv = at; at += up(bh * p.max_chunks * p.subs * 2 * KB * a->D * 4);
     p.o_pbias = at; at += a->num_buckets ? up(bh * p.ng * p.chunks * a->num_buckets * (a->Hq / a->Hk) * 8) : 0;
@@ -611,21 +591,22 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
 size_t attn_backward_workspace(const scipnp_block_attn_args* a) { return bwd_plan(a).total; }
 
 template <typename T, int DP, int RW>
-static int dq_launch(const Attn& p, unsigned grid, hipStream_t st) {
-    using C = DqCfg<T, DP, RW>;
-    const size_t lds = (size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + bias_lds(p.nbuckets, p.maxd, p.G) + (size_t)4 * p.nbuckets * HROW * 4;
-    if (lds > 163840) return fail(SCIPNP_EINVAL, "block_attn_backward: %zu bytes of LDS needed (fewer buckets or a smaller n_sel)", lds);
+static int dq_launch(const Attn& p, hipStream_t st) {
+    using C = DqCfg<T, DP>;
+    const size_t set = ((size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + (size_t)(p.nbuckets * p.G + 3) / 4 * 16 + (size_t)RW * p.nbuckets * HROW * 4 + 15) / 16 * 16;
+    const size_t shared = bias_lut_bytes(p.nbuckets, p.maxd) + 16;
+    int sets = 4 / RW;
+    while (sets > 1 && shared + sets * set > 163840) sets >>= 1;
+    if (shared + sets * set > 163840) return fail(SCIPNP_EINVAL, "block_attn_backward: %zu bytes of LDS needed (fewer buckets or a smaller n_sel)", shared + set);
     static LdsAttrOnce once;
     if (const int rc = once.ensure((const void*)block_attn_dq_kernel<T, DP, RW>, 163840, "block_attn_dq")) return rc;
-    block_attn_dq_kernel<T, DP, RW><<<grid, 256, lds, st>>>(p);
+    const long long items = (long long)p.B * p.Hk * p.ng * p.chunks;
+    block_attn_dq_kernel<T, DP, RW><<<xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set);
     return SCIPNP_OK;
 }
 template <typename T, int DP>
 static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
-    const unsigned gq = xcd_grid((long long)p.B * p.Hk * p.ng * p.chunks);
-    int rc;
-    if constexpr (sizeof(T) == 4 && DP > 64) rc = bp.rw == 2 ? dq_launch<T, DP, 2>(p, gq, st) : dq_launch<T, DP, 4>(p, gq, st);
-    else rc = bp.rw == 1 ? dq_launch<T, DP, 1>(p, gq, st) : bp.rw == 2 ? dq_launch<T, DP, 2>(p, gq, st) : dq_launch<T, DP, 4>(p, gq, st);
+    const int rc = bp.rw == 1 ? dq_launch<T, DP, 1>(p, st) : bp.rw == 2 ? dq_launch<T, DP, 2>(p, st) : dq_launch<T, DP, 4>(p, st);
     if (rc) return rc;
     using C = DkvCfg<T, DP>;
     const size_t lds = (size_t)C::MAIN + (C::LIST + 8) * 4 + bias_lds(p.nbuckets, p.maxd, p.G);
@@ -639,16 +620,18 @@ static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
 
 template <typename T>
 static int bwd_run(const Attn& p, const BwdPlan& bp, float* delta, int* chunk_start, hipStream_t st) {
-    const size_t rows = (size_t)p.B * p.Lq * p.Hq, words = (size_t)p.B * p.Hk * p.nb * p.words;
+    const size_t rows = (size_t)p.B * p.Lq * p.Hq, words = (size_t)p.B * p.Hk * p.nb * (p.words + 1);
     const size_t want = (rows + 15) / 16;
     attn_delta_kernel<T><<<(unsigned)(want < 8192 ? want : 8192), 256, 0, st>>>(p, delta, words);
     const size_t groups = (size_t)p.B * p.Hk * p.ng;
     attn_mark_kernel<<<(unsigned)((groups + 3) / 4), 256, (size_t)4 * p.n * 4, st>>>(p);
     attn_plan_kernel<<<(unsigned)(p.B * p.Hk), 256, 0, st>>>(p, chunk_start, bp.R, bp.CH);
-    const int rc = p.D <= 32 ? bwd_launch<T, 32>(p, bp, st) : p.D <= 64 ? bwd_launch<T, 64>(p, bp, st)
+    int rc;
+    if (sizeof(T) == 4 && p.D > 32 && p.D <= 48) rc = bwd_launch<T, sizeof(T) == 4 ? 48 : 64>(p, bp, st);
+    else rc = p.D <= 32 ? bwd_launch<T, 32>(p, bp, st) : p.D <= 64 ? bwd_launch<T, 64>(p, bp, st)
                  : p.D <= 96 ? bwd_launch<T, 96>(p, bp, st) : bwd_launch<T, 128>(p, bp, st);
     if (rc) return rc;
-    attn_dkv_join_kernel<T><<<dim3((unsigned)(p.nb * bp.subs), (unsigned)(p.B * p.Hk)), 256, 0, st>>>(p, bp.subs);
+    attn_dkv_join_kernel<T><<<dim3((unsigned)(p.nb * bp.subs), (unsigned)(p.B * p.Hk), (unsigned)((2 * KB * (p.D / 4) + 255) / 256)), 256, 0, st>>>(p, bp.subs);
     if (p.dbias) attn_dbias_kernel<<<(unsigned)(p.nbuckets * p.Hq), 64, 0, st>>>(p);
     return launch_status("scipnp_block_attn_backward");
 }
@@ -673,6 +656,7 @@ int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t 
     Attn p = attn_params(a);
     char* const w = (char*)a->workspace;
     p.delta = (float*)w;
+    p.zeros = (float*)(w + bp.o_member - 256);
     p.member = (unsigned*)(w + bp.o_member);
     p.words = bp.words;
     p.chunk_start = (int*)(w + bp.o_chunk);
