@@ -75,64 +75,96 @@ struct Select {
     const int32_t *qlen, *klen;
     int32_t* sel;
     int B, Lq, Lk, Hq, Hk, D, block, qb, n, sink, local, causal, nb, ng;
-    int gpw, tiles, spare;                                // groups of a workgroup, workgroups of a (sequence, key head), LDS words behind the keys
+    int gpw, tiles, hist_at;                              // groups of a workgroup, workgroups of a (sequence, key head), LDS offset
 };
 
-constexpr int SEL_MAX_BLOCKS = 8192;                      // 64 KB of scores
+constexpr int SEL_MAX_BLOCKS = 8192;
 
-// A double as a whole number of the same order: NaN lowest (1), 0 is free for "not a candidate"
+// A number as a whole number of the same order (64 and 32 bits): NaN lowest (1), 0 is free for "no candidate", all ones for "always"
 __device__ __forceinline__ unsigned long long order_key(double v) {
     const unsigned long long u = __builtin_bit_cast(unsigned long long, v + 0.0);          // (-0 becomes +0: they are equal)
     if (v != v) return 1;
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
+__device__ __forceinline__ unsigned order_key(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v + 0.f);
+    if (v != v) return 1;
+    return (u >> 31) ? ~u : (u | 0x80000000u);
+}
 
-// the keys of 0 .. nb-1 are in LDS (0: no candidate): one wave writes the n best of them, ascending; ties to the lower index.
-// Radix selection from the top byte over a histogram of its own: at most 8 counting passes, none once a byte's bucket is taken whole
-// (scores that differ in their first 20 bits need three).
-__device__ void select_best(const unsigned long long* keys, int nb, int n, int32_t* out, int* hist, int lane) {
+// One counting pass of a radix selection, from the greatest byte down: of the keys with `prefix` above the byte, the byte of the
+// need-th greatest, how many are still needed among those with that byte, and how many there are.  key(j): 0 where there is none.
+template <typename K, typename F>
+__device__ __forceinline__ void radix_pass(F key, int nb, int shift, K& prefix, K& mask, int& need, bool& all, int* hist, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hist[lane + 64 * i] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int j = lane; j < nb; j += 64) {
+        const K k = key(j);
+        if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);          // (counts: no order)
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int c[4], s = 0;                                       // sums from the greatest byte down, four counts a lane
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; s += c[i]; }
+    int incl = s;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += o;
+    }
+    int before = incl - s, byte = -1, rest = 0, have = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (before < need && before + c[i] >= need) { byte = 255 - (4 * lane + i); rest = need - before; have = c[i]; }
+        before += c[i];
+    }
+    const int src = __ffsll((unsigned long long)__ballot(byte >= 0)) - 1;                          // exactly one lane has it
+    prefix |= (K)__shfl(byte, src, 64) << shift;
+    mask |= (K)255 << shift;
+    need = __shfl(rest, src, 64);
+    all = need == __shfl(have, src, 64);
+}
+
+// One wave writes the n best of the candidates 0 .. nb-1, ascending; ties to the lower index.  The scores are compared as fp32 keys
+// first (half the LDS, at most four passes); only where the n-th and the next share one are those candidates compared in fp64,
+// recomputed by exact(j).
+template <typename F>
+__device__ void select_best(const unsigned* keys, int nb, int n, int32_t* out, int* hist, int lane, F exact) {
     int cand = 0;
     for (int base = 0; base < nb; base += 64) cand += __popcll(__ballot(base + lane < nb && keys[base + lane] != 0));
-    unsigned long long prefix = 0, mask = 0;               // the threshold's known upper bytes
+    unsigned prefix = 0, mask = 0;                         // the threshold's known upper bytes
     int need = min(n, cand);                               // still to take among the keys with that prefix
     bool all = need == cand;                               // take every key with the prefix (and every greater one)
-    for (int shift = 56; shift >= 0 && !all; shift -= 8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) hist[lane + 64 * i] = 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int shift = 24; shift >= 0 && !all; shift -= 8)
+        radix_pass<unsigned>([&](int j) { return keys[j]; }, nb, shift, prefix, mask, need, all, hist, lane);
+    unsigned long long prefix64 = 0, mask64 = 0;
+    if (!all && prefix != ~0u && prefix != 1) {            // (the always chosen and the NaNs are equal among themselves)
+        auto key64 = [&](int j) -> unsigned long long { return keys[j] == prefix ? order_key(exact(j)) : 0; };
+        unsigned long long lo = ~0ull, hi = 0;
         for (int j = lane; j < nb; j += 64) {
-            const unsigned long long k = keys[j];
-            if (k != 0 && (k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);      // (counts: no order)
+            const unsigned long long k = key64(j);
+            if (k) { lo = min(lo, k); hi = max(hi, k); }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        // sums from the greatest byte down, four counts a lane
-        int c[4], s = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { c[i] = hist[255 - (4 * lane + i)]; s += c[i]; }
-        int incl = s;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(incl, off, 64);
-            if (lane >= off) incl += o;
+        for (int off = 32; off > 0; off >>= 1) {
+            lo = min(lo, (unsigned long long)__shfl_xor((long long)lo, off, 64));
+            hi = max(hi, (unsigned long long)__shfl_xor((long long)hi, off, 64));
         }
-        int before = incl - s, byte = -1, rest = 0, have = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (before < need && before + c[i] >= need) { byte = 255 - (4 * lane + i); rest = need - before; have = c[i]; }
-            before += c[i];
-        }
-        const int src = __ffsll((unsigned long long)__ballot(byte >= 0)) - 1;                      // exactly one lane has it
-        prefix |= (unsigned long long)__shfl(byte, src, 64) << shift;
-        mask |= 255ull << shift;
-        need = __shfl(rest, src, 64);
-        all = need == __shfl(have, src, 64);
+        if (lo != hi)
+            for (int shift = 56; shift >= 0 && !all; shift -= 8) radix_pass<unsigned long long>(key64, nb, shift, prefix64, mask64, need, all, hist, lane);
     }
-    // greater than the prefix: in; equal: the first `need` of them
+    // greater than the threshold: in; equal: the first `need` of them
     int eqs = 0, at = 0;
     for (int base = 0; base < nb; base += 64) {
         const int j = base + lane;
-        const unsigned long long k = j < nb ? keys[j] : 0, below = (1ull << lane) - 1;
-        const bool eq = k != 0 && (k & mask) == prefix, gt = k != 0 && (k & mask) > prefix;
+        const unsigned k = j < nb ? keys[j] : 0;
+        const unsigned long long below = (1ull << lane) - 1;
+        bool eq = k != 0 && (k & mask) == prefix, gt = k != 0 && (k & mask) > prefix;
+        if (mask64 != 0 && eq) {
+            const unsigned long long e = order_key(exact(j));
+            eq = (e & mask64) == prefix64;
+            gt = (e & mask64) > prefix64;
+        }
         const unsigned long long be = __ballot(eq);
         const bool in = gt || (eq && (all || eqs + __popcll(be & below) < need));
         const unsigned long long bi = __ballot(in);
@@ -158,30 +190,44 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
     extern __shared__ __attribute__((aligned(16))) char smem_s[];
     const int qst = a.D + 2;                               // (rows two banks apart)
     double* const qs = (double*)smem_s;                    // [groups][qst]
-    unsigned long long* const keys = (unsigned long long*)(qs + a.gpw * qst);      // [groups][nb]; before that the parts of step 1
-    int* const hists = (int*)(keys + (size_t)a.gpw * a.nb + a.spare);
+    double* const scratch = qs + a.gpw * qst;              // step 1: the parts; then the keys [groups][nb]
+    unsigned* const keys = (unsigned*)scratch;
+    int* const hists = (int*)(smem_s + a.hist_at);
     const long long total = (long long)a.B * a.Hk * a.tiles, item = xcd_item(blockIdx.x, total);
     if (item < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int g0 = (int)(item % a.tiles) * a.gpw, bh = (int)(item / a.tiles), hk = bh % a.Hk, b = bh / a.Hk;
     const int ngr = min(a.gpw, a.ng - g0);
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Lq) : a.Lq, klen = a.klen ? min(max(a.klen[b], 0), a.Lk) : a.Lk;
-    const int G = a.Hq / a.Hk, nc = a.D / E, parts = 64 / nc;
+    const int G = a.Hq / a.Hk, nc = a.D / E, parts = 64 / nc;              // (D <= 256: at most 64 pieces of a row)
     for (int i = wave; i < a.gpw; i += SEL_WAVES) {
-        const int q0 = (g0 + i) * a.qb, rows = i < ngr ? min(a.qb, qlen - q0) * G : 0;
-        const int c = lane % nc, part = lane / nc;         // (D <= 256: at most 64 pieces of a row)
+        const int q0 = (g0 + i) * a.qb, toks = i < ngr ? min(a.qb, qlen - q0) : 0;
+        const int c = lane % nc, part = lane / nc;
         double s[E] = {};
         if (part < parts) {
-            const T* base = (const T*)a.q + b * a.sq.b + c * E;
-#pragma unroll 4
-            for (int r = part; r < rows; r += parts) {
-                __attribute__((aligned(16))) T v[E];
-                *(f32x4a*)v = *(const f32x4a*)(base + (long long)(q0 + r / G) * a.sq.t + (hk * G + r % G) * a.sq.h);
+            const T* base = (const T*)a.q + b * a.sq.b + (long long)q0 * a.sq.t + hk * G * a.sq.h + c * E;
+            int tok = part / G, h = part - tok * G;
+            const int dt = parts / G, dh = parts - dt * G;
+            while (tok < toks) {
+                __attribute__((aligned(16))) T v[8][E];
+                int m = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e) s[e] += (double)(float)v[e];
+                for (int u = 0; u < 8; ++u) {              // eight rows under way
+                    const bool ok = tok < toks;
+                    *(f32x4a*)v[u] = ok ? *(const f32x4a*)(base + (long long)tok * a.sq.t + h * a.sq.h) : f32x4a{0.f, 0.f, 0.f, 0.f};
+                    m += ok;
+                    h += dh;
+                    tok += dt;
+                    if (h >= G) { h -= G; ++tok; }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (u < m)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) s[e] += (double)(float)v[u][e];
             }
         }
-        double* const mine = (double*)keys + (size_t)wave * 64 * E;        // (the keys come later)
+        double* const mine = scratch + (size_t)wave * 64 * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) mine[lane * E + e] = s[e];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -193,22 +239,25 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __syncthreads();
-    // key position of the group's last query (this lane's column), and what the tile's last group may see
+    // key position of the group's last query (this lane's column)
     const int col = lane & 15, kq = lane >> 4, gc = g0 + col;
     const bool group = col < ngr && gc * a.qb < qlen;
     const int last = klen - qlen + min((gc + 1) * a.qb, qlen) - 1;
     const int own = last >= 0 ? last / a.block : (last - a.block + 1) / a.block;
+    const int seen = min((klen + a.block - 1) / a.block, !a.causal ? a.nb : last < 0 ? 0 : last / a.block + 1);        // blocks it may choose
     const int nt = (a.nb + 15) / 16;
     const double* const qrow = qs + (col < a.gpw ? col : 0) * qst + 4 * kq;
+    const float* const means = a.summary + ((size_t)b * a.nb * a.Hk + hk) * a.D;
     for (int jt = wave; jt < nt; jt += SEL_WAVES) {
         const int j = jt * 16 + col;                       // (A's row)
         f32x4a m[ND];
-        const float* const row = a.summary + (((size_t)b * a.nb + (j < a.nb ? j : 0)) * a.Hk + hk) * a.D + 4 * kq;
+        const float* const row = means + (size_t)(j < a.nb ? j : 0) * a.Hk * a.D + 4 * kq;
 #pragma unroll
         for (int d = 0; d < ND; ++d) m[d] = j < a.nb && 16 * d + 4 * kq < a.D ? *(const f32x4a*)(row + 16 * d) : f32x4a{0.f, 0.f, 0.f, 0.f};
         f64x4a s0 = {0.0, 0.0, 0.0, 0.0}, s1 = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
+            if (16 * d >= a.D) continue;                   // (uniform)
             double q[4] = {0.0, 0.0, 0.0, 0.0};
             if (16 * d + 4 * kq < a.D)
 #pragma unroll
@@ -223,14 +272,22 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
             for (int r = 0; r < 4; ++r) {
                 const int jj = jt * 16 + 4 * r + kq;
                 if (jj >= a.nb) continue;
-                const bool may = group && (long long)jj * a.block < klen && (!a.causal || (long long)jj * a.block <= last);
                 const bool must = jj < a.sink || abs(jj - own) < a.local;
-                keys[(size_t)col * a.nb + jj] = !may ? 0 : must ? ~0ull : order_key(s0[r] + s1[r]);
+                keys[(size_t)col * a.nb + jj] = !group || jj >= seen ? 0u : must ? ~0u : order_key((float)(s0[r] + s1[r]));
             }
     }
     __syncthreads();
     for (int i = wave; i < ngr; i += SEL_WAVES)
-        select_best(keys + (size_t)i * a.nb, a.nb, a.n, a.sel + ((size_t)bh * a.ng + g0 + i) * a.n, hists + wave * 256, lane);
+        select_best(keys + (size_t)i * a.nb, a.nb, a.n, a.sel + ((size_t)bh * a.ng + g0 + i) * a.n, hists + wave * 256, lane, [&](int j) {
+            const float* m = means + (size_t)j * a.Hk * a.D;
+            double s = 0.0;
+            for (int d = 0; d < a.D; d += 4) {
+                const f32x4a v = *(const f32x4a*)(m + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s = fma(qs[i * qst + d + e], (double)v[e], s);
+            }
+            return s;
+        });
 #endif
 }
 
@@ -299,15 +356,15 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s) {
     p.n = a->n_sel; p.sink = a->sink; p.local = a->local; p.causal = a->causal;
     p.ng = (a->Lq + a->query_block - 1) / a->query_block;
     // groups of a workgroup: up to 16 (the columns of a matrix instruction) with at most 64 KB of scores, two workgroups a CU
-    p.gpw = 65536 / (p.nb * 8);
-    p.gpw = p.gpw > 16 ? 16 : p.gpw < 1 ? 1 : p.gpw;
+    p.gpw = 65536 / (p.nb * 4);
+    p.gpw = p.gpw > 16 ? 16 : p.gpw;
     if (p.gpw > p.ng) p.gpw = p.ng;
     p.tiles = (p.ng + p.gpw - 1) / p.gpw;
-    const int parts_words = SEL_WAVES * 64 * (16 / (int)attn_esize(a->dtype)), key_words = p.gpw * p.nb;
-    p.spare = parts_words > key_words ? parts_words - key_words : 0;
+    const size_t parts_bytes = (size_t)SEL_WAVES * 64 * (16 / attn_esize(a->dtype)) * 8, key_bytes = ((size_t)p.gpw * p.nb * 4 + 15) / 16 * 16;
+    p.hist_at = (int)((size_t)p.gpw * (a->D + 2) * 8 + (parts_bytes > key_bytes ? parts_bytes : key_bytes));
     const long long items = (long long)a->B * a->Hk * p.tiles;
     SCIPNP_REQUIRE(items < (1ll << 22) && (long long)p.ng * a->query_block < (1ll << 30), "too many query groups");
-    const size_t lds = (size_t)p.gpw * (a->D + 2) * 8 + (size_t)(key_words + p.spare) * 8 + SEL_WAVES * 256 * 4;
+    const size_t lds = (size_t)p.hist_at + SEL_WAVES * 256 * 4;
     return a->dtype == SCIPNP_BF16 ? select_launch<__bf16>(p, lds, xcd_grid(items), (hipStream_t)s) : select_launch<float>(p, lds, xcd_grid(items), (hipStream_t)s);
 }
 

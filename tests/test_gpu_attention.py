@@ -143,6 +143,20 @@ def test_selection_ties_nan_and_infinities(A):
         assert torch.equal(got.cpu(), O.select(q.cpu(), s, n, 1, 4, 600, False, None, None, 0, 0)), n
 
 
+@pytest.mark.parametrize('step', [2.0 ** -30, 2.0 ** -45])
+def test_selection_of_scores_that_one_float32_holds(A, step):
+    """neighbours in the order closer than fp32 can tell, a few of them and hundreds"""
+    gen = torch.Generator().manual_seed(5)
+    q = torch.ones(1, 2, 1, 8)
+    s = torch.zeros(1, 700, 1, 8)
+    s[0, :, 0, 0] = 1.0
+    s[0, :, 0, 1] = torch.randperm(700, generator=gen).float() * step
+    s[0, 100:200, 0, 0] = 3.0
+    for n in (1, 50, 99, 101, 400, 699):
+        got = A.select_blocks(cu(q), cu(s), n, block=1, query_block=2, sink=0, local=0)
+        assert torch.equal(got.cpu(), O.select(q, s, n, 1, 2, 700, False, None, None, 0, 0)), n
+
+
 def test_summary_of_the_newest_tokens(A):
     gen = torch.Generator().manual_seed(9)
     B, Lk, Hk, D, block = 3, 500, 2, 64, 64
