@@ -214,7 +214,7 @@ class BlockAttnArgs(C.Structure):
     """scipnp_block_attn_args of include/scipnp.h"""
     _fields_ = ([('struct_size', C.c_size_t)]
                 + [(n, C.c_int) for n in ('dtype', 'B', 'Lq', 'Lk', 'Hq', 'Hk', 'D', 'block', 'query_block', 'n_sel', 'causal', 'num_buckets',
-                                          'max_distance')]
+                                          'max_distance', 'zero_rest')]
                 + [('scale', C.c_float)] + [(n, C.c_void_p) for n in ('q', 'k', 'v', 'out')]
                 + [(n + '_stride', _st3) for n in ('q', 'k', 'v', 'out')]
                 + [(n, C.c_void_p) for n in ('sel', 'qlen', 'klen', 'bucket_of', 'q_pos', 'k_pos', 'bias', 'lse', 'out32', 'dout')]

@@ -32,7 +32,7 @@ _F32, _F64, _I32 = torch.float32, torch.float64, torch.int32
 # forty ctypes assignments (a decoding step is five such calls).
 _NORM = struct.Struct('@N9if10P24q6PN')
 _SELECT = struct.Struct('@N13iP3q4P')
-_ATTN = struct.Struct('@N13if4P12q10P3q5PN')
+_ATTN = struct.Struct('@N14if4P12q10P3q5PN')
 assert (_NORM.size, _SELECT.size, _ATTN.size) == tuple(C.sizeof(s) for s in (_lib.HeadNormArgs, _lib.SelectArgs, _lib.BlockAttnArgs))
 _NONE4 = (0, 0, 0, 0)
 
@@ -278,13 +278,13 @@ def _attn_args(q, k, v, sel, block, query_block, scale, causal, qlen, klen, buck
     elif q_pos is not None or k_pos is not None:
         raise ValueError('q_pos and k_pos are positions for the bias')
     _on_device(('q', q), ('k', k), ('v', v), ('sel', sel), ('qlen', qlen), ('klen', klen), ('bias', bias), ('bucket_of', bucket_of), ('q_pos', q_pos), ('k_pos', k_pos))
-    front = (_ATTN.size, _DT[dt], B, Lq, Lk, Hq, Hk, D, block, query_block, n, bool(causal), nbuckets, maxd,
-             1.0 / math.sqrt(D) if scale is None else scale, qa[0], ka[0], va[0])
+    front = (_ATTN.size, _DT[dt], B, Lq, Lk, Hq, Hk, D, block, query_block, n, bool(causal), nbuckets, maxd)
+    inputs = (1.0 / math.sqrt(D) if scale is None else scale, qa[0], ka[0], va[0])
     strides = (*qa[1:], *ka[1:], *va[1:])
     middle = (sel_, ql, kl, bucket_, qp, kp, bias_)
 
-    def pack(out=_NONE4, lse=0, out32=0, dout=_NONE4, grads=_NONE4, ws=0, size=0):
-        return _ATTN.pack(*front, out[0], *strides, *out[1:], *middle, lse, out32, *dout, *grads, ws, size)
+    def pack(out=_NONE4, lse=0, out32=0, dout=_NONE4, grads=_NONE4, ws=0, size=0, zero_rest=False):
+        return _ATTN.pack(*front, zero_rest, *inputs, out[0], *strides, *out[1:], *middle, lse, out32, *dout, *grads, ws, size)
     return pack, front
 
 
@@ -315,8 +315,9 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
     the saved fp32 result carries the gradient (out is the same up to its rounding)."""
     pack, front = _attn_args(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos)
     n, dt, dev = q.shape, q.dtype, q.device
-    if out is None:
-        out = (torch.empty_like if qlen is None else torch.zeros_like)(q)
+    fresh = out is None
+    if fresh:
+        out = torch.empty_like(q)
     oa = _tokens(out, 'out', n, dt)
     _on_device(('out', out))
     saved = None
@@ -328,7 +329,7 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
     if size:
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
         ws_ = ws.data_ptr()
-    _call('scipnp_block_attn', pack(oa, lse, out32, ws=ws_, size=size))
+    _call('scipnp_block_attn', pack(oa, lse, out32, ws=ws_, size=size, zero_rest=fresh))
     return (out, saved) if save else out
 
 

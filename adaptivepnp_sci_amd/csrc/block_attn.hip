@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         if (any) {
             const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
             const int far = a.causal ? min(sq.klen, sq.shift + g * a.qb + (rows_end - 1) / a.G + 1) : sq.klen;
-            c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
+            c = live_tiles(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
         }
         if (lane == 0) *nlist = c;
     }
@@ -64,14 +64,14 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
     const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
-    const int min_lim = wave_min(live ? lim : INT_MAX), max_lim = wave_max(lim);
+    const int min_lim = wave_min(live ? lim : INT_MAX);
     const unsigned ks = (unsigned)(a.sk.t * (long long)sizeof(T)), vs = (unsigned)(a.sv.t * (long long)sizeof(T));
     DmaOffsets<T, DP, RW> ko, vo;
     ko.init(rw, lane, ks, a.D);
     vo.init(rw, lane, vs, a.D);
     __syncthreads();
 
-    const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist) * tpb;
+    const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist);
     const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, count = max(0, min(ntiles, t_begin + per) - t_begin);
     int trips = count;                                    // sets that share a barrier take the same number of trips
     if constexpr (RW > 1) {
@@ -93,7 +93,6 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
     };
     auto issue = [&](int key0, int buf) {
         const int there = min(KT, sq.klen - key0);
-        if (there <= 0) return;                           // (the rest of a block behind the last key)
         char* const tile = smem + buf * C::TILE;
         ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
         vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
@@ -113,7 +112,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         key0 = next_key();
         issue(key0, 0);
     }
-    for (int t = 0; t < trips; ++t) {
+    for (int t = 0; t < count; ++t) {
         const int buf = t & 1, cur = key0;
         int* const kp = kp_lds + buf * KT;
         if (a.k_pos && tset < KT) kp[tset] = kpr;
@@ -122,7 +121,6 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
             key0 = next_key();
             issue(key0, buf ^ 1);
         }
-        if (t >= count || cur > max_lim) continue;
         const char* const kt = smem + buf * C::TILE;
         f32x16a s = dma_rows<T, DP>(kt, qf, lane);
         ColTile<T, DP> vt;
@@ -174,10 +172,17 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
         vt.template mma<SAVE>(s, o);
     }
+    for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     l += __shfl_xor(l, 32, 64);
 
-    if (!live) return;
     const size_t id = ((size_t)b * a.Lq + tok) * a.Hq + head;
+    if (!live) {                                          // (a row behind qlen; the join takes care of it where there is one)
+        if (there_is && a.zero_rest && a.splits == 1 && row < R && tok < a.Lq) {
+            T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
+            for (int d = 4 * hi; d < a.D; d += 8) store_four(out + d, f32x4a{0.f, 0.f, 0.f, 0.f});
+        }
+        return;
+    }
     if (a.splits > 1) {
         const size_t rows = (size_t)a.B * a.Lq * a.Hq;
         if (hi == 0) *(float2*)(a.pml + 2 * (part * rows + id)) = make_float2(m, l);
@@ -201,25 +206,40 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
 #endif
 }
 
-// joins the parts of a row's keys: one wave a row
+// joins the parts of a row's keys (at most 64: a lane each for their maxima and sums): one wave a row, the parts in order
 template <typename T>
 __global__ void __launch_bounds__(256) block_attn_join_kernel(Attn a) {
     const size_t rows = (size_t)a.B * a.Lq * a.Hq, id = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (id >= rows) return;
     const int lane = threadIdx.x & 63, head = (int)(id % a.Hq), tok = (int)(id / a.Hq % a.Lq), b = (int)(id / a.Hq / a.Lq);
-    if (tok >= seq_of(a, b).qlen) return;
-    float M = -INFINITY;
-    for (int p = 0; p < a.splits; ++p) M = fmaxf(M, a.pml[2 * (p * rows + id)]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, s[2] = {0.f, 0.f};
-    for (int p = 0; p < a.splits; ++p) {
-        const float2 ml = *(const float2*)(a.pml + 2 * (p * rows + id));
-        const float f = __builtin_amdgcn_exp2f(ml.x - Ms);
-        L = fmaf(ml.y, f, L);
-        const float* po = a.po + (p * rows + id) * a.D;
+    T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
+    if (tok >= seq_of(a, b).qlen) {
+        if (a.zero_rest)
+            for (int d = lane; d < a.D; d += 64) out[d] = (T)0.f;
+        return;
+    }
+    const float2 ml = lane < a.splits ? *(const float2*)(a.pml + 2 * (lane * rows + id)) : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 64 * i < a.D) s[i] = fmaf(po[lane + 64 * i], f, s[i]);
+    for (int off = 1; off < 64; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    const float Ms = M == -INFINITY ? 0.f : M, f = __builtin_amdgcn_exp2f(ml.x - Ms);
+    float L = ml.y * f;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) L += __shfl_xor(L, off, 64);
+    const float* po = a.po + id * a.D;
+    float s[2] = {0.f, 0.f};
+    for (int p0 = 0; p0 < a.splits; p0 += 8) {
+        float v[8][2];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[u][i] = p0 + u < a.splits && lane + 64 * i < a.D ? po[(p0 + u) * rows * a.D + lane + 64 * i] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float w = __shfl(f, p0 + u, 64);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[i] = p0 + u < a.splits ? fmaf(v[u][i], w, s[i]) : s[i];
+        }
     }
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
 #pragma unroll
@@ -227,7 +247,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(Attn a) {
         const int d = lane + 64 * i;
         if (d >= a.D) continue;
         const float v = s[i] * inv;
-        ((T*)a.out)[b * a.so.b + (long long)tok * a.so.t + head * a.so.h + d] = (T)v;
+        out[d] = (T)v;
         if (a.out32) a.out32[id * a.D + d] = v;
     }
     if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
@@ -283,6 +303,7 @@ Attn attn_params(const scipnp_block_attn_args* a) {
     p.chunks = p.splits = 1;
     p.scale = a->scale;
     p.scale2 = a->scale * LOG2E;
+    p.zero_rest = a->zero_rest;
     p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.dout = a->dout;
     p.sq = strides_of(a->q_stride); p.sk = strides_of(a->k_stride); p.sv = strides_of(a->v_stride); p.so = strides_of(a->out_stride);
     p.sdo = strides_of(a->dout_stride);

@@ -87,32 +87,39 @@ struct DmaOffsets {
     }
 };
 
-// score products: A B^T, A = row li of the tile.  All of a half's reads are under way before its first product
+// score products: A B^T, A = row li of the tile.  read() brings the rows into registers (all reads under way at once), mma() multiplies
 template <typename T, int DP>
-__device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int lane) {
-    constexpr int LC = DmaTile<T, DP>::LC, N = DP / Mat<T>::K, H = N <= 8 ? N : N / 2;
-    const int li = lane & 31, x = (lane >> 5) ^ swz<T, LC>(li);
-    const char* row = tile + li * LC * 16;
-    f32x16a acc;
+struct RowTile {
+    static constexpr int LC = DmaTile<T, DP>::LC, N = DP / Mat<T>::K;
+    typename Mat<T>::Frag a[N];
+    __device__ __forceinline__ void read(const char* tile, int lane) {
+        const int li = lane & 31, x = (lane >> 5) ^ swz<T, LC>(li);
+        const char* row = tile + li * LC * 16;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+        for (int s = 0; s < N; ++s) a[s] = *(const typename Mat<T>::Frag*)(row + ((x ^ (2 * s)) << 4));
+    }
+    __device__ __forceinline__ f32x16a mma(const typename Mat<T>::Frag (&b)[N]) const {
+        f32x16a acc;
 #pragma unroll
-    for (int h = 0; h < N; h += H) {
-        typename Mat<T>::Frag a[H];
+        for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
-        for (int s = 0; s < H; ++s) a[s] = *(const typename Mat<T>::Frag*)(row + ((x ^ (2 * (h + s))) << 4));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < H; ++s) {
+        for (int s = 0; s < N; ++s) {
             if constexpr (sizeof(T) == 2) {
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s], b[h + s], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s], b[s], acc, 0, 0, 0);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], b[h + s][j], acc, 0, 0, 0);
+                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], b[s][j], acc, 0, 0, 0);
             }
         }
+        return acc;
     }
-    return acc;
+};
+template <typename T, int DP>
+__device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int lane) {
+    RowTile<T, DP> r;
+    r.read(tile, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    return r.mma(b);
 }
 
 // second products: acc += X^T P over the tile's 32 rows (P in an accumulator's registers, rounded to T), NB column blocks of 32.
@@ -295,7 +302,7 @@ __device__ __forceinline__ void dma_wait() {
 // ---- what every kernel knows of the call
 struct Attn {
     int B, Lq, Lk, Hq, Hk, G, D, block, qb, n, causal, nbuckets, maxd, nb, ng;
-    int chunks, splits;                                   // forward: row chunks of a group, parts of its keys
+    int zero_rest, chunks, splits;                                 // forward: row chunks of a group, parts of its keys
     float scale, scale2;                                  // scale2 = scale * log2(e)
     const void *q, *k, *v, *dout;
     void* out;
@@ -349,6 +356,13 @@ __device__ __forceinline__ int live_blocks(const Attn& a, const int32_t* sel, in
     return count;
 }
 
+// ... and the number of their tiles with a wanted key (the last block may end behind the limit)
+__device__ __forceinline__ int live_tiles(const Attn& a, const int32_t* sel, int limit, int* list, int lane) {
+    const int c = live_blocks(a, sel, limit, list, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return c == 0 ? 0 : (c - 1) * (a.block / KT) + (min(a.block, limit - list[c - 1] * a.block) + KT - 1) / KT;
+}
+
 // ---- scores of a tile: 32 keys of a lane's row, masked, with the bias
 struct Bias {                                             // in LDS: the bucket of each clamped distance, the workgroup's heads
     const unsigned char* lut;
@@ -385,10 +399,20 @@ __device__ __forceinline__ int tile_distance(const Attn& a, RowRange q, int key0
     return lo == hi ? lo : -1;
 }
 // the bias of 16 scores of a lane's row, position by position
+__device__ __forceinline__ void tile_buckets(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int hi, int (&d)[16]) {
+    if (kp) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[r] = kp[tile_key(r, hi)];
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[r] = key0 + tile_key(r, hi);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) d[r] = s.lut[clamp_dist(d[r] - qp, a.maxd)];
+}
 __device__ __forceinline__ void tile_bias(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int gl, int hi, float (&x)[16]) {
     int d[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) d[r] = s.lut[clamp_dist((kp ? kp[tile_key(r, hi)] : key0 + tile_key(r, hi)) - qp, a.maxd)];
+    tile_buckets(a, s, key0, kp, qp, hi, d);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = s.tbl[d[r] * a.G + gl];
 }

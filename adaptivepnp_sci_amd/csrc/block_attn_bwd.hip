@@ -98,15 +98,15 @@ __global__ void __launch_bounds__(256) attn_plan_kernel(Attn a, int* chunk_start
     if (tid == 0) cs[a.nb] = carry;
 }
 
-// ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums of a lane's row: one LDS word a bucket and lane, the two ends
-// (where most tiles lie) in registers
+// ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
+// most tiles lie) in registers
 template <typename T, int DP>
 struct DqCfg {
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
     static constexpr int MAIN = 2 * TILE;
     static constexpr int KP = 2 * KT * 4;
 };
-constexpr int HROW = 65;                                  // a bucket's 64 lane sums, rows shifted by a bank
+constexpr int HROW = 33;                                  // a bucket's sums of 32 rows, shifted by a bank
 
 template <typename T, int DP, int RW>
 __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes) {
@@ -139,15 +139,16 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     float* const tbl = (float*)(smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16);
     const Bias bias = load_bias(a, lut, tbl, hk, tset, 64 * RW);
     float* const hist = tbl + (a.nbuckets * a.G + 3) / 4 * 4;
-    float* const mine = hist + rw * a.nbuckets * HROW + lane;
-    for (int i = 0; i < a.nbuckets; ++i) mine[i * HROW] = 0.f;
+    float* const mine = hist + rw * a.nbuckets * HROW + li;
+    if (hi == 0)
+        for (int i = 0; i < a.nbuckets; ++i) mine[i * HROW] = 0.f;
     if (threadIdx.x == 0) *longest = 0;
     if (rw == 0) {
         int c = 0;
         if (any) {
             const int rows_end = min(min(R, r0 + 32 * RW), (sq.qlen - g * a.qb) * a.G);
             const int far = a.causal ? min(sq.klen, sq.shift + g * a.qb + (rows_end - 1) / a.G + 1) : sq.klen;
-            c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
+            c = live_tiles(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
         }
         if (lane == 0) *nlist = c;
     }
@@ -158,14 +159,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     const float lse = live ? a.lse[stat] * LOG2E : 0.f, delta = live ? a.delta[stat] : 0.f;
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
     const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
-    const int min_lim = wave_min(live ? lim : INT_MAX), max_lim = wave_max(lim);
+    const int min_lim = wave_min(live ? lim : INT_MAX);
     const unsigned ks = (unsigned)(a.sk.t * (long long)sizeof(T)), vs = (unsigned)(a.sv.t * (long long)sizeof(T));
     DmaOffsets<T, DP, RW> ko, vo;
     ko.init(rw, lane, ks, a.D);
     vo.init(rw, lane, vs, a.D);
     __syncthreads();
 
-    const int tpb = a.block / KT, count = __builtin_amdgcn_readfirstlane(*nlist) * tpb;
+    const int count = __builtin_amdgcn_readfirstlane(*nlist);
     int trips = count;                                    // sets that share a barrier take the same number of trips
     if constexpr (RW > 1) {
         if (sets > 1) {
@@ -185,7 +186,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     };
     auto issue = [&](int key0, int buf) {
         const int there = min(KT, sq.klen - key0);
-        if (there <= 0) return;
         char* const tile = smem + buf * C::TILE;
         ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
         vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
@@ -194,6 +194,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     const int far = 2 * a.maxd;
     const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
     float sum_lo = 0.f, sum_hi = 0.f;
+    auto add_bucket = [&](int n, float v) {
+        v += __shfl_xor(v, 32, 64);
+        if (hi == 0) mine[n * HROW] += v;
+    };
     f32x16a o[NB];
 #pragma unroll
     for (int db = 0; db < NB; ++db)
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
         key0 = next_key();
         issue(key0, 0);
     }
-    for (int t = 0; t < trips; ++t) {
+    for (int t = 0; t < count; ++t) {
         const int buf = t & 1, cur = key0;
         int* const kp = kp_lds + buf * KT;
         if (a.k_pos && tset < KT) kp[tset] = kpr;
@@ -214,26 +218,24 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
             key0 = next_key();
             issue(key0, buf ^ 1);
         }
-        if (t >= count || cur > max_lim) continue;
         const char* const kt = smem + buf * C::TILE;
         f32x16a s = dma_rows<T, DP>(kt, qf, lane);
         const f32x16a dp = dma_rows<T, DP>(kt + DmaTile<T, DP>::BYTES, gf, lane);
         ColTile<T, DP> kc;
         kc.read(kt, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
-        float x[16];
+        float c = a.scale2, add = -lse;
         if (dist >= 0) {
-            float add = 0.f;
-            if (a.nbuckets) add = dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = add - lse;
+            if (a.nbuckets) add += dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
         } else {
+            float x[16];
             tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] -= lse;
+            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, x[r]);
+            c = 1.f;
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, x[r])) * (dp[r] - delta);
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, add)) * (dp[r] - delta);
         if (cur + KT - 1 > min_lim) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : 0.f;
@@ -244,20 +246,23 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
                                   (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
                 if (dist == 0) sum_lo += sum;
                 else if (dist == far) sum_hi += sum;
-                else mine[bias.lut[dist] * HROW] += sum;
+                else add_bucket(bias.lut[dist], sum);
             } else {
+                int d[16];
+                tile_buckets(a, bias, cur, a.k_pos ? kp : nullptr, qp, hi, d);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int k = a.k_pos ? kp[tile_key(r, hi)] : cur + tile_key(r, hi);
-                    mine[bias.lut[clamp_dist(k - qp, a.maxd)] * HROW] += s[r];
-                }
+                for (int half = 0; half < 2; ++half)      // (the two lanes of a row share its words: one after the other)
+                    if (hi == half)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) mine[d[r] * HROW] += s[r];
             }
         }
         kc.mma(s, o);
     }
+    for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     if (a.dbias) {                                        // the set's sums: a (bucket, head) adds its lanes in order, in fp64
-        mine[bias.lut[0] * HROW] += sum_lo;
-        mine[bias.lut[far] * HROW] += sum_hi;
+        add_bucket(bias.lut[0], sum_lo);
+        add_bucket(bias.lut[far], sum_hi);
         __syncthreads();
         if (there_is)
             for (int i = tset; i < a.nbuckets * a.G; i += 64 * RW) {
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
                 for (int w = 0; w < RW; ++w) {
                     const int at = (r0 + w * 32) % a.G;
                     for (int y = (h - at + a.G) % a.G; y < 32; y += a.G)
-                        sum += (double)hist[(w * a.nbuckets + n) * HROW + y] + (double)hist[(w * a.nbuckets + n) * HROW + y + 32];
+                        sum += (double)hist[(w * a.nbuckets + n) * HROW + y];
                 }
                 a.pbias[(size_t)item * a.nbuckets * a.G + i] = sum;
             }
@@ -304,9 +309,8 @@ __global__ void __launch_bounds__(64) attn_dbias_kernel(Attn a) {
 template <typename T, int DP>
 struct DkvCfg {
     static constexpr int INFO = KT * 20 + 16;             // bias - lse (or - lse), delta, last key, position, head of each row; flags
-    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES + INFO;
+    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES + INFO + KT * 16;   // ... and where the rows of q and dout begin
     static constexpr int MAIN = 4 * TILE;                 // two row tiles, two buffers
-    static constexpr int OST = DP + 4;
     static constexpr int JOIN = 2 * 32 * ((DP + 31) / 32 * 32 + 4) * 4;
     static_assert(JOIN <= MAIN, "the join reuses the tiles");
     static constexpr int LIST = 1032;                     // query groups of a chunk
@@ -319,10 +323,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32, LC = DmaTile<T, DP>::LC, PIECES = DmaTile<T, DP>::PIECES, MINE = (PIECES + 1) / 2, BYTES = DmaTile<T, DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const long long total = (long long)a.B * a.Hk * a.max_chunks * subs, item = xcd_item(blockIdx.x, total);
-    if (item < 0) return;
-    const unsigned it0 = (unsigned)item;
-    const int sub = it0 % subs, c = it0 / subs % a.max_chunks, bh = it0 / subs / a.max_chunks, hk = bh % a.Hk, b = bh / a.Hk;
+    // (chunks in turn over the XCDs: the last of a sequence and key head's slots are empty)
+    const int sub = blockIdx.x % subs, c = blockIdx.x / subs % a.max_chunks, bh = blockIdx.x / subs / a.max_chunks, hk = bh % a.Hk, b = bh / a.Hk;
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     if (c >= cs[a.nb]) return;                            // (uniform)
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hi = lane >> 5;
@@ -397,41 +399,62 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     };
     const T* const qb0 = (const T*)a.q + b * a.sq.b + hk * a.G * a.sq.h;
     const T* const gb0 = (const T*)a.dout + b * a.sdo.b + hk * a.G * a.sdo.h;
+    // The first 32 threads of a row half keep the books of its tiles: where row x begins (a tile ahead), what it brings besides
     float iadd = 0.f, idelta = 0.f;
-    int ilim = -1, iqp = 0, ig = 0;
-    auto load = [&](unsigned x, int buf) {                // rows x .. x + 31
-        char* const tile = main + (rs * 2 + buf) * C::TILE;
+    int ilim = -1, iqp = 0, ig = 0, tok = -1, gl = 0;     // (tok, gl: of the row of the next tile)
+    auto tile_at = [&](int it) -> char* { return main + (rs * 2 + (it & 1)) * C::TILE; };
+    auto put_rows = [&](int it) {
+        long long* const off = (long long*)(tile_at(it) + 2 * BYTES + C::INFO);
+        off[tsplit] = tok < 0 ? -1 : tok * a.sq.t + gl * a.sq.h;
+        off[KT + tsplit] = tok < 0 ? -1 : tok * a.sdo.t + gl * a.sdo.h;
+    };
+    auto get_info = [&]() {
+        ilim = -1;
+        iadd = idelta = 0.f;
+        iqp = 0;
+        ig = gl;
+        if (tok >= 0) {
+            const size_t stat = ((size_t)b * a.Hq + hk * a.G + gl) * a.Lq + tok;
+            iadd = a.lse[stat];
+            idelta = a.delta[stat];
+            ilim = a.causal ? min(sq.shift + tok, sq.klen - 1) : sq.klen - 1;
+            iqp = a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : sq.shift + tok;
+        }
+    };
+    int chunk_at[MINE];                                   // elements into a row of this lane's 16 bytes, -1: past D
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int y = (kw + 2 * i) * 64 + lane, ch = (y % LC) ^ swz<T, LC>(y / LC);
+        chunk_at[i] = ch * Mat<T>::E < a.D ? ch * Mat<T>::E : -1;
+    }
+    auto issue = [&](int it) {
+        char* const tile = tile_at(it);
+        const long long* const off = (const long long*)(tile + 2 * BYTES + C::INFO);
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
             const int piece = kw + 2 * i;
             if (PIECES % 2 == 0 || piece < PIECES) {
-                const int y = piece * 64 + lane, r = y / LC, ch = (y % LC) ^ swz<T, LC>(r);
-                int tok, gl;
-                row_of(x + r, tok, gl);
-                const bool ok = tok >= 0 && ch * Mat<T>::E < a.D;
-                const T* const qa = ok ? qb0 + tok * a.sq.t + gl * a.sq.h + ch * Mat<T>::E : (const T*)a.zeros;
-                const T* const ga = ok ? gb0 + tok * a.sdo.t + gl * a.sdo.h + ch * Mat<T>::E : (const T*)a.zeros;
+                const long long oq = off[piece * 64 / LC + lane / LC], og = off[KT + piece * 64 / LC + lane / LC];
+                const bool ok = oq >= 0 && chunk_at[i] >= 0;
+                const T* const qa = ok ? qb0 + oq + chunk_at[i] : (const T*)a.zeros;
+                const T* const ga = ok ? gb0 + og + chunk_at[i] : (const T*)a.zeros;
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)qa, (__attribute__((address_space(3))) void*)(tile + 1024 * piece), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ga, (__attribute__((address_space(3))) void*)(tile + BYTES + 1024 * piece), 16, 0, 0);
             }
         }
-        if (tsplit < KT) {
-            int tok, gl;
-            row_of(x + tsplit, tok, gl);
-            ilim = -1; iadd = idelta = 0.f; iqp = 0; ig = gl;
-            if (tok >= 0) {
-                const size_t stat = ((size_t)b * a.Hq + hk * a.G + gl) * a.Lq + tok;
-                iadd = a.lse[stat];
-                idelta = a.delta[stat];
-                ilim = a.causal ? min(sq.shift + tok, sq.klen - 1) : sq.klen - 1;
-                iqp = a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : sq.shift + tok;
-            }
-        }
     };
     const int iters = (int)((x1 - x0 + 2 * KT - 1) / (2 * KT));
-    load(x0 + rs * KT, 0);
+    const unsigned xs = x0 + rs * KT + tsplit;
+    if (tsplit < KT) {
+        row_of(xs, tok, gl);
+        put_rows(0);
+        get_info();
+        row_of(xs + 2 * KT, tok, gl);
+    }
+    __syncthreads();
+    issue(0);
     for (int it = 0; it < iters; ++it) {
-        char* const at = main + (rs * 2 + (it & 1)) * C::TILE;
+        char* const at = tile_at(it);
         float* const info = (float*)(at + 2 * BYTES);
         if (tsplit < KT) {
             float add = -iadd * LOG2E;
@@ -449,9 +472,16 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             ((int*)info)[3 * KT + tsplit] = iqp;
             ((int*)info)[4 * KT + tsplit] = ig;
             if (tsplit == 0) ((int*)info)[5 * KT] = (all_one ? 1 : 0) | (open ? 2 : 0);
+            put_rows(it + 1);
         }
         dma_wait<4>();
-        if (it + 1 < iters) load(x0 + (it + 1) * 2 * KT + rs * KT, (it + 1) & 1);
+        if (it + 1 < iters) {
+            issue(it + 1);
+            if (tsplit < KT) {
+                get_info();
+                row_of(xs + (it + 2) * 2 * KT, tok, gl);
+            }
+        }
         const int flags = __builtin_amdgcn_readfirstlane(((int*)info)[5 * KT]);
         f32x16a s = dma_rows<T, DP>(at, kf, lane);
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
@@ -613,7 +643,7 @@ static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
     if (lds > 163840) return fail(SCIPNP_EINVAL, "block_attn_backward: %zu bytes of LDS needed", lds);
     static LdsAttrOnce once;
     if (const int rc2 = once.ensure((const void*)block_attn_dkv_kernel<T, DP>, 163840, "block_attn_dkv")) return rc2;
-    const unsigned gk = xcd_grid((long long)p.B * p.Hk * p.max_chunks * bp.subs);
+    const unsigned gk = (unsigned)((long long)p.B * p.Hk * p.max_chunks * bp.subs);
     block_attn_dkv_kernel<T, DP><<<gk, 256, lds, st>>>(p, bp.CH, bp.subs, div_magic(bp.R), div_magic(p.G));
     return SCIPNP_OK;
 }
