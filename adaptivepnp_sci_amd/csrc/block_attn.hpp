@@ -294,8 +294,11 @@ __device__ __forceinline__ void each_four(int hi, F f) {
 template <int WAVES>
 __device__ __forceinline__ void dma_wait() {
 #if defined(__HIP_DEVICE_COMPILE__)
-    if constexpr (WAVES == 1) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // (the builtins, so that the compiler knows these loads to be done and puts no wait for all of them further on)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);                   // vmcnt(0) lgkmcnt(0)
+    if constexpr (WAVES > 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 #endif
 }
 

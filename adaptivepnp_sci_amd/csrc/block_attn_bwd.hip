@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     if (c >= cs[a.nb]) return;                            // (uniform)
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, hi = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave & 1, rs = wave >> 1, tsplit = kw * 64 + lane;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave & 1, rs = wave >> 1;
     char* const main = smem;
     int* const list = (int*)(smem + C::MAIN);
     int* const misc = list + C::LIST;                     // block, scan
@@ -399,14 +399,14 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     };
     const T* const qb0 = (const T*)a.q + b * a.sq.b + hk * a.G * a.sq.h;
     const T* const gb0 = (const T*)a.dout + b * a.sdo.b + hk * a.G * a.sdo.h;
-    // The first 32 threads of a row half keep the books of its tiles: where row x begins (a tile ahead), what it brings besides
+    // Each row half's first wave keeps where the rows of the next tile begin, its second what they bring besides (32 lanes each)
     float iadd = 0.f, idelta = 0.f;
     int ilim = -1, iqp = 0, ig = 0, tok = -1, gl = 0;     // (tok, gl: of the row of the next tile)
     auto tile_at = [&](int it) -> char* { return main + (rs * 2 + (it & 1)) * C::TILE; };
     auto put_rows = [&](int it) {
         long long* const off = (long long*)(tile_at(it) + 2 * BYTES + C::INFO);
-        off[tsplit] = tok < 0 ? -1 : tok * a.sq.t + gl * a.sq.h;
-        off[KT + tsplit] = tok < 0 ? -1 : tok * a.sdo.t + gl * a.sdo.h;
+        off[lane] = tok < 0 ? -1 : tok * a.sq.t + gl * a.sq.h;
+        off[KT + lane] = tok < 0 ? -1 : tok * a.sdo.t + gl * a.sdo.h;
     };
     auto get_info = [&]() {
         ilim = -1;
@@ -444,11 +444,11 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
         }
     };
     const int iters = (int)((x1 - x0 + 2 * KT - 1) / (2 * KT));
-    const unsigned xs = x0 + rs * KT + tsplit;
-    if (tsplit < KT) {
+    const unsigned xs = x0 + rs * KT + lane;
+    if (lane < KT) {
         row_of(xs, tok, gl);
-        put_rows(0);
-        get_info();
+        if (kw == 0) put_rows(0);
+        else get_info();
         row_of(xs + 2 * KT, tok, gl);
     }
     __syncthreads();
@@ -456,61 +456,69 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     for (int it = 0; it < iters; ++it) {
         char* const at = tile_at(it);
         float* const info = (float*)(at + 2 * BYTES);
-        if (tsplit < KT) {
-            float add = -iadd * LOG2E;
-            bool one = true;                              // every key has the same bucket for this row
-            if (a.nbuckets && ilim >= 0) {
-                const int lo = clamp_dist(klo - iqp, a.maxd);
-                one = lo == clamp_dist(khi - iqp, a.maxd);
-                if (one) add += bias.tbl[bias.lut[lo] * a.G + ig];
+        if (lane < KT) {
+            if (kw == 0) {
+                put_rows(it + 1);
+            } else {
+                float add = -iadd * LOG2E;
+                bool one = true;                          // every key has the same bucket for this row
+                if (a.nbuckets && ilim >= 0) {
+                    const int lo = clamp_dist(klo - iqp, a.maxd);
+                    one = lo == clamp_dist(khi - iqp, a.maxd);
+                    if (one) add += bias.tbl[bias.lut[lo] * a.G + ig];
+                }
+                const bool all_one = __ballot(!one) == 0, open = __ballot(ilim < k64 + KB - 1) == 0;
+                if (!all_one) add = -iadd * LOG2E;
+                info[lane] = add;
+                info[KT + lane] = idelta;
+                info[2 * KT + lane] = __int_as_float(ilim);
+                info[3 * KT + lane] = __int_as_float(iqp);
+                info[4 * KT + lane] = __int_as_float(ig);
+                if (lane == 0) info[5 * KT] = __int_as_float((all_one ? 0 : 1) | (open ? 0 : 2));
             }
-            const bool all_one = __ballot(!one) == 0, open = __ballot(ilim < k64 + KB - 1) == 0;
-            if (!all_one) add = -iadd * LOG2E;
-            info[tsplit] = add;
-            info[KT + tsplit] = idelta;
-            ((int*)info)[2 * KT + tsplit] = ilim;
-            ((int*)info)[3 * KT + tsplit] = iqp;
-            ((int*)info)[4 * KT + tsplit] = ig;
-            if (tsplit == 0) ((int*)info)[5 * KT] = (all_one ? 1 : 0) | (open ? 2 : 0);
-            put_rows(it + 1);
         }
         dma_wait<4>();
         if (it + 1 < iters) {
-            issue(it + 1);
-            if (tsplit < KT) {
-                get_info();
+            if (lane < KT) {                              // (before the tile is asked for: its wait is no wait for the tile)
+                if (kw != 0) get_info();
                 row_of(xs + (it + 2) * 2 * KT, tok, gl);
             }
+            issue(it + 1);
         }
-        const int flags = __builtin_amdgcn_readfirstlane(((int*)info)[5 * KT]);
+        const int flags = __builtin_amdgcn_readfirstlane(__float_as_int(info[5 * KT]));
         f32x16a s = dma_rows<T, DP>(at, kf, lane);
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
         ColTile<T, DP> gc, qc;
         gc.read(at + BYTES, lane);
         qc.read(at, lane);
+        const float* const mine = info + 4 * hi;
+        if (flags & 1) {                                  // the bias key by key
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4a qp = *(const f32x4a*)(mine + 3 * KT + 8 * q), gh = *(const f32x4a*)(mine + 4 * KT + 8 * q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[4 * q + e] = fmaf(s[4 * q + e], a.scale2, bias.tbl[bias.lut[clamp_dist(kpos - __float_as_int(qp[e]), a.maxd)] * a.G + __float_as_int(gh[e])]);
+            }
+        }
+        const float scale = flags & 1 ? 1.f : a.scale2;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int r4 = 8 * q + 4 * hi;
-            f32x4a add = *(const f32x4a*)(info + r4);
-            const f32x4a delta = *(const f32x4a*)(info + KT + r4);
-            if (!(flags & 1)) {
-                const int4 qp = *(const int4*)((int*)info + 3 * KT + r4), gh = *(const int4*)((int*)info + 4 * KT + r4);
-                const int qps[4] = {qp.x, qp.y, qp.z, qp.w}, ghs[4] = {gh.x, gh.y, gh.z, gh.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) add[e] += bias.tbl[bias.lut[clamp_dist(kpos - qps[e], a.maxd)] * a.G + ghs[e]];
-            }
+            const f32x4a add = *(const f32x4a*)(mine + 8 * q), delta = *(const f32x4a*)(mine + KT + 8 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * q + e;
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, add[e]));
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, add[e]));
                 dp[r] = s[r] * (dp[r] - delta[e]);
             }
-            if (!(flags & 2)) {
-                const int4 lim = *(const int4*)((int*)info + 2 * KT + r4);
-                const int lims[4] = {lim.x, lim.y, lim.z, lim.w};
+        }
+        if (flags & 2) {                                  // some row does not see some key
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4a lim = *(const f32x4a*)(mine + 2 * KT + 8 * q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool see = key <= lims[e];
+                    const bool see = key <= __float_as_int(lim[e]);
                     s[4 * q + e] = see ? s[4 * q + e] : 0.f;
                     dp[4 * q + e] = see ? dp[4 * q + e] : 0.f;
                 }
