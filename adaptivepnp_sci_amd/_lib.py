@@ -122,6 +122,8 @@ SIGNATURES = {
     'scipnp_block_attn_workspace_bytes': (_sz, [_vp, _int]),
     'scipnp_block_attn': (_int, [_vp, _vp]),
     'scipnp_block_attn_backward': (_int, [_vp, _vp]),
+    'scipnp_patch_tokens': (_int, [_vp, _vp, _int, _int, _int, _int, _int, C.c_float, C.c_float, _int, _vp]),
+    'scipnp_patch_frames': (_int, [_vp, _vp, _int, _int, _int, _int, _int, _vp]),
     'scipnp_host_legacy_normal': (_int, [_vp, C.POINTER(_int), C.POINTER(_int), C.POINTER(C.c_double), C.c_double, C.c_double,
                                         _vp, _sz]),
     'scipnp_twostage_ffdnet_iterate': (_int, [_vp, C.POINTER(_int), _vp]),

@@ -1,7 +1,8 @@
 """Non-local attention over selected key blocks: thin wrappers over the C ABI (include/scipnp.h), like ops.py.
 
 A query group picks the key blocks that resemble it by a cheap score and attends to those blocks only: the block matching of
-non-local video restoration in the form of attention, for tokens of any kind.  Four operators, used together:
+non-local video restoration in the form of attention, for tokens of any kind (the solver's 'nonlocal_color' prior is built of them,
+nonlocal_prior.py).  Four operators, used together:
 
     head_norm_rotate   norm of every query and key head with its learned weight, and the rotation by the token's position, in one
                        pass; writes into a cache when given slots                          (+ head_norm_rotate_backward)

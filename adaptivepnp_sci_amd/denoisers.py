@@ -2,6 +2,7 @@
 
 ffdnet_rgb_denoise_full_tensor      <- packages/ffdnet/test_ffdnet_ipol.py:240-359
 fastdvdnet_denoiser_full_tensor_v2  <- packages/fastdvdnet/test_fastdvdnet.py:325-500
+nonlocal_denoiser_full_tensor       the non-local prior with the same signature (no counterpart in the reference)
 test_ddnet                          <- packages/DDnet/DDnet_test.py:218-321 (deep demosaicking)
 
 Both take / return the reference's (H, W, 3, B) colour cube as a CUDA(ROCm) tensor.  The solver
@@ -78,6 +79,21 @@ def fastdvdnet_denoiser_full_tensor_v2(vnoisy, sigma, y_bayer=None, Phi=None, mo
         y_pm = y_bayer.permute(2, 0, 1).contiguous()
         Phi_pm = Phi.permute(2, 3, 0, 1).contiguous()
         fastdvdnet_online_finetune(model, eng, frames, y_pm, Phi_pm, sigma, lr_, update_per_iter)
+        return ops.rgb_to_cube(eng.forward(frames, sigma)), model
+    return ops.rgb_to_cube(eng.forward(frames, sigma))
+
+
+def nonlocal_denoiser_full_tensor(vnoisy, sigma, y_bayer=None, Phi=None, model=None, useGPU=True, lr_=0.000001, updata_=False,
+                                  update_per_iter=1):
+    """vnoisy (H,W,3,B) CUDA tensor -> denoised (H,W,3,B) by the non-local prior `model` (nonlocal_prior.NonLocalPrior); with `updata_`
+    first adapts it to the measurement (y_bayer / Phi as Bayer planes (M,N,4) / (M,N,B,4)) and returns (out, model)."""
+    from .nonlocal_prior import NonLocalEngine, nonlocal_online_finetune
+    H, W, _, B = vnoisy.shape
+    frames = ops.cube_to_rgb(vnoisy.float().contiguous())
+    eng = NonLocalEngine(model, B, H, W, vnoisy.device)
+    if updata_:
+        nonlocal_online_finetune(model, eng, frames, y_bayer.permute(2, 0, 1).contiguous(), Phi.permute(2, 3, 0, 1).contiguous(), sigma, lr_,
+                                 update_per_iter)
         return ops.rgb_to_cube(eng.forward(frames, sigma)), model
     return ops.rgb_to_cube(eng.forward(frames, sigma))
 

@@ -680,6 +680,20 @@ def fastdvd_noisy_input(v, noise_f64):
     return out
 
 
+def patch_tokens(frames, tokens, units, shifts, constant, scale=1.0, replicate=True):
+    """planar frames (B,3,H,W) -> patch tokens (units * shifts, L, 1, 56) of the non-local prior (nonlocal_prior.py)"""
+    B, _, H, W = frames.shape
+    _call('scipnp_patch_tokens', _p(frames, 'frames'), _p(tokens, 'tokens'), B, H, W, units, shifts, float(constant), float(scale), int(replicate), _stream())
+    return tokens
+
+
+def patch_frames(tokens, frames, units, shifts):
+    """patch tokens -> planar frames (B,3,H,W), the mean over the shifted grids"""
+    B, _, H, W = frames.shape
+    _call('scipnp_patch_frames', _p(tokens, 'tokens'), _p(frames, 'frames'), B, H, W, units, shifts, _stream())
+    return frames
+
+
 def sum_rows_f64(part, out=None):
     """row sums of a contiguous fp64 table [rows][n] (or one row [n]) on the device, fixed summation order"""
     t = part.reshape(1, -1) if part.dim() == 1 else part

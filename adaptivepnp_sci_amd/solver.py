@@ -37,7 +37,7 @@ F32 = torch.float32
 # extra layout kernel per iteration when set; None in production.
 ITERATE_HOOK = None
 
-DENOISERS = ('tv', 'ffdnet_color', 'fastdvd_color')
+DENOISERS = ('tv', 'ffdnet_color', 'fastdvd_color', 'nonlocal_color')
 
 
 class _NullLog:
@@ -250,8 +250,12 @@ class AdmmRun:
                         from .finetune import _FFDNetTrainer
                         self.eng._ft_trainer = _FFDNetTrainer(model, self.eng)
                 else:
-                    from .fastdvd import FastDVDEngine
-                    self.eng = FastDVDEngine(model, B, H, W, self.device, precision=conv_precision, units=U)
+                    if denoiser == 'nonlocal_color':
+                        from .nonlocal_prior import NonLocalEngine
+                        self.eng = NonLocalEngine(model, B, H, W, self.device, units=U)
+                    else:
+                        from .fastdvd import FastDVDEngine
+                        self.eng = FastDVDEngine(model, B, H, W, self.device, precision=conv_precision, units=U)
                     self.rgb_w = torch.empty_like(self.x_rgb)
                 self.dd = None
                 if model_demosaic is not None:   # deep demosaicking instead of Malvar (reference :192-194 / :242-244)
@@ -363,7 +367,10 @@ class AdmmRun:
                 via_mosaic = True
             else:
                 ops.pm_pre_denoise(self.x, b_in, w, self.x_rgb, None, None, inv_rho, inv_tau, nsig)
-            if gate and self.two_stage and (self.update_i < self.update_times or self.update_times < 0):
+            if gate and self.denoiser == 'nonlocal_color':
+                from .nonlocal_prior import nonlocal_online_finetune
+                nonlocal_online_finetune(self.model, self.eng, net_in, self.y, self.Phi, nsig, self.lr_, self.update_per_iter, logf=self.logf)
+            elif gate and self.two_stage and (self.update_i < self.update_times or self.update_times < 0):
                 from .finetune import fastdvdnet_online_finetune
                 fastdvdnet_online_finetune(self.model, self.eng, net_in, self.y, self.Phi, nsig, self.lr_,
                                            self.update_per_iter, logf=self.logf,
@@ -475,7 +482,7 @@ class AdmmRun:
                     src = getattr(self, name)
                     if src is not None:
                         getattr(r, name).copy_(src.view(B, U, 3, H, W)[:, u])
-                if self.denoiser == 'fastdvd_color':        # (the closed-form update reads the engine's last denoised frames)
+                if self.denoiser != 'ffdnet_color':        # (the closed-form update reads the engine's last denoised frames)
                     r.eng.out.copy_(self.eng.out.view(B, U, 3, H, W)[:, u])
         return runs
 

@@ -781,6 +781,14 @@ size_t scipnp_block_attn_workspace_bytes(const scipnp_block_attn_args* a, int ba
 int scipnp_block_attn(const scipnp_block_attn_args* a, scipnp_stream_t s);
 int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t s);
 
+/* tokens of the non-local prior: `units` clips of B / units frames (B, 3, H, W; frame t of clip u at t * units + u), each cut with
+ * `shifts` (1, 2, 4) grids moved by half a patch.  tokens (units * shifts, T * ty * tx * 64, 56): 4 x 4 x 3 values times scale, `constant`,
+ * zeros; 64 patches a tile of 32 x 32 pixels, ty = ceil((H + 2 [shifts > 1]) / 32).  Outside the frame: replicated, or zero.
+ * patch_frames: the mean of the shifts' values at every pixel (its adjoint is patch_tokens with scale 1 / shifts, zeros outside). */
+int scipnp_patch_tokens(const float* frames, float* tokens, int B, int H, int W, int units, int shifts, float constant, float scale,
+                        int replicate, scipnp_stream_t s);
+int scipnp_patch_frames(const float* tokens, float* frames, int B, int H, int W, int units, int shifts, scipnp_stream_t s);
+
 /* HOST function (no GPU involved): n deviates of NumPy's LEGACY normal stream -- np.random.normal(loc, scale, n) on the
  * global RandomState, bit for bit -- from / to a generator state in np.random.get_state() form (key[624], pos,
  * has_gauss, cached_gaussian).  The reference draws its FastDVDnet finetune noise from that stream
