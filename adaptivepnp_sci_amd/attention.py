@@ -310,8 +310,9 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
     """softmax(scale * q k^T + bias) v over the keys of each group's selected blocks (select_blocks; an entry outside the blocks, or
     not greater than those before it, is ignored).  scale None: 1 / sqrt(D).  causal: keys behind the query are masked.  bias
     (buckets, Hq) float32 by the relative position of key and query, bucket_of from bucket_table; q_pos (B, Lq), k_pos (B, Lk) int32
-    name the positions (None: the key positions), e.g. the frame of each token of a video; differences must fit 32 bits.  A query
-    without a visible key gives zeros.  Rows behind qlen are zeros, or left as they were in a given `out`.
+    name the positions (None: the key positions), e.g. the frame of each token of a video; differences must fit 32 bits.  A bias below
+    -1e30 (-inf, a type's lowest value) masks its keys.  A query without a visible key gives zeros; what a key holds that a query does
+    not see -- NaN, infinity -- does not reach it.  Rows behind qlen are zeros, or left as they were in a given `out`.
     save=True returns (out, saved) for block_attention_backward; bfloat16 probabilities are then multiplied whole, not rounded, so that
     the saved fp32 result carries the gradient (out is the same up to its rounding)."""
     pack, front = _attn_args(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos)
@@ -337,7 +338,8 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
 def block_attention_backward(dout, q, k, v, sel, saved, block=64, query_block=64, scale=None, causal=False, qlen=None, klen=None,
                              bucket_of=None, bias=None, q_pos=None, k_pos=None):
     """(dq, dk, dv, dbias) of block_attention called with the same arguments and save=True; rows behind qlen / klen are zeros, dbias
-    (buckets, Hq) float32 is None without a bias.  The selection is not differentiated."""
+    (buckets, Hq) float32 is None without a bias.  The selection is not differentiated.  q, k, v and dout of the live rows must be finite:
+    here a NaN or an infinity reaches every gradient of its block of 64."""
     pack, _ = _attn_args(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos)
     n, dev = q.shape, q.device
     da = _tokens(dout, 'dout', n, q.dtype)

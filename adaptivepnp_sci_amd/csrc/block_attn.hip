@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
     float m = -INFINITY, l = 0.f;
+    bool spoilt = false;
 
     int key0 = 0;
     if (count > 0) {
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         vt.read(kt + DmaTile<T, DP>::BYTES, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
         const bool masked = cur + KT - 1 > min_lim;
+        bool skip = false;
         float c = a.scale2, add = 0.f;
         if (dist >= 0 && a.nbuckets) add = dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
         if (dist < 0 || masked || c < 0.f) {              // the scores one by one
@@ -140,6 +142,10 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
                 for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, add);
             }
             if (masked) {
+                if (!vt.finite()) {                       // (what its values add comes behind the loop, key by key)
+                    spoilt = skip = true;
+                    vt.clear();
+                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : -INFINITY;
             }
@@ -170,39 +176,73 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // P rounded to bf16 is off by 2^-8 of each probability, of the order of the output's own rounding; with out32 wanted it is
         // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
+        if constexpr (sizeof(T) == 4) {
+            if (skip) continue;
+        }
         vt.template mma<SAVE>(s, o);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     l += __shfl_xor(l, 32, 64);
+    const Attn& z = late_args();                          // (what only the end needs is read again there: the loop's scalars fit the registers)
+    // Tiles with masked keys and values that are not numbers: only rows that see a key take its value, by plain loads
+    if (spoilt) {
+        const T* const qr = (const T*)z.q + b * z.sq.b + tok * z.sq.t + head * z.sq.h;
+        for (int t = t_begin; t < t_begin + count; ++t) {
+            const int cur = __builtin_amdgcn_readfirstlane(list[t / tpb]) * z.block + t % tpb * KT, there = min(KT, sq.klen - cur);
+            if (cur + KT - 1 <= min_lim) continue;
+            bool bad = false;
+            for (int j = 0; j < there; ++j)
+                for (int d = lane; d < z.D; d += 64) bad |= !(fabsf((float)vb[(cur + j) * z.sv.t + d]) < INFINITY);
+            if (!__ballot(bad)) continue;
+            for (int j = 0; j < there; ++j) {
+                if (!live || cur + j > lim) continue;
+                const T* const kr = kb + (cur + j) * z.sk.t;
+                const T* const vr = vb + (cur + j) * z.sv.t;
+                float x = 0.f;
+                for (int d = 0; d < z.D; ++d) x = fmaf((float)kr[d], (float)qr[d], x);
+                x *= z.scale2;
+                if (z.nbuckets) {
+                    const int kp = z.k_pos ? z.k_pos[(size_t)b * z.Lk + cur + j] : cur + j;
+                    x += bias.tbl[bias.lut[clamp_dist(kp - qp, z.maxd)] * z.G + gl];
+                }
+                const float p = __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
+                each_four<T, NB>(hi, [&](int d, auto at) {
+                    if (d >= z.D) return;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[at(e) >> 4][at(e) & 15] = fmaf(p, (float)vr[d + e], o[at(e) >> 4][at(e) & 15]);
+                });
+            }
+        }
+    }
 
-    const size_t id = ((size_t)b * a.Lq + tok) * a.Hq + head;
+    const size_t id = ((size_t)b * z.Lq + tok) * z.Hq + head;
     if (!live) {                                          // (a row behind qlen; the join takes care of it where there is one)
-        if (there_is && a.zero_rest && a.splits == 1 && row < R && tok < a.Lq) {
-            T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
-            for (int d = 4 * hi; d < a.D; d += 8) store_four(out + d, f32x4a{0.f, 0.f, 0.f, 0.f});
+        if (there_is && z.zero_rest && z.splits == 1 && row < R && tok < z.Lq) {
+            T* const out = (T*)z.out + b * z.so.b + (long long)tok * z.so.t + head * z.so.h;
+            for (int d = 4 * hi; d < z.D; d += 8) store_four(out + d, f32x4a{0.f, 0.f, 0.f, 0.f});
         }
         return;
     }
-    if (a.splits > 1) {
-        const size_t rows = (size_t)a.B * a.Lq * a.Hq;
-        if (hi == 0) *(float2*)(a.pml + 2 * (part * rows + id)) = make_float2(m, l);
-        float* const po = a.po + (part * rows + id) * a.D;
+    if (z.splits > 1) {
+        const size_t rows = (size_t)z.B * z.Lq * z.Hq;
+        if (hi == 0) *(float2*)(z.pml + 2 * (part * rows + id)) = make_float2(m, l);
+        float* const po = z.po + (part * rows + id) * z.D;
         each_four<T, NB>(hi, [&](int d, auto at) {
-            if (d < a.D) *(f32x4a*)(po + d) = f32x4a{o[at(0) >> 4][at(0) & 15], o[at(1) >> 4][at(1) & 15], o[at(2) >> 4][at(2) & 15], o[at(3) >> 4][at(3) & 15]};
+            if (d < z.D) *(f32x4a*)(po + d) = f32x4a{o[at(0) >> 4][at(0) & 15], o[at(1) >> 4][at(1) & 15], o[at(2) >> 4][at(2) & 15], o[at(3) >> 4][at(3) & 15]};
         });
         return;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);             // (a NaN sum stays one)
-    T* const out = (T*)a.out + b * a.so.b + (long long)tok * a.so.t + head * a.so.h;
+    T* const out = (T*)z.out + b * z.so.b + (long long)tok * z.so.t + head * z.so.h;
     each_four<T, NB>(hi, [&](int d, auto at) {
-        if (d >= a.D) return;
+        if (d >= z.D) return;
         f32x4a v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = o[at(e) >> 4][at(e) & 15] * inv;
         store_four(out + d, v);
-        if constexpr (SAVE) *(f32x4a*)(a.out32 + id * a.D + d) = v;
+        if constexpr (SAVE) *(f32x4a*)(z.out32 + id * z.D + d) = v;
     });
-    if (a.lse && hi == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (z.lse && hi == 0) z.lse[((size_t)b * z.Hq + head) * z.Lq + tok] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 #endif
 }
 

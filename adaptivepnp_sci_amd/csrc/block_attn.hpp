@@ -216,6 +216,39 @@ struct ColTile {
                          : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
     }
 #endif
+    // No infinity and no NaN in the tile: a masked weight of 0 would carry it into rows that do not see it (0 x inf)
+    __device__ __forceinline__ bool finite() const {
+        float sum = 0.f;                                  // of x * 0
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (sizeof(T) == 2) {
+            const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{u[db][k].v[2 * i], u[db][k].v[2 * i + 1]}, zero, sum, false);
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < DmaTile<T, DP>::PIECES; ++i) {
+                const f32x4a x = *(const f32x4a*)(tile + i * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = fmaf(x[e], 0.f, sum);
+            }
+        }
+#endif
+        return __ballot(sum != 0.f) == 0;
+    }
+    __device__ __forceinline__ void clear() {             // (bf16, where the columns are in registers)
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[db][k].v[i] = (__bf16)0.f;
+        }
+    }
     template <bool EXACT = false>
     __device__ __forceinline__ void mma(const f32x16a& p, f32x16a (&acc)[NB]) const {
         if constexpr (sizeof(T) == 2) {
@@ -326,6 +359,16 @@ struct Attn {
     float* pkv;                                           // partial dk, dv
     double* pbias;
 };
+// the kernel's first argument, read once more from memory where this is called: nothing of it is held in registers until then
+__device__ __forceinline__ const Attn& late_args() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto p = (const __attribute__((address_space(4))) Attn*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Attn*)p;
+#else
+    return *(const Attn*)nullptr;
+#endif
+}
 
 struct Seq { int qlen, klen, shift; };                    // shift: key position of query 0
 __device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
@@ -371,11 +414,9 @@ struct Bias {                                             // in LDS: the bucket 
     const unsigned char* lut;
     const float* tbl;
 };
-// scores are kept in units of ln 2 (exp2 needs no product); a finite bias stays finite
-__device__ __forceinline__ float bias_log2(float b) {
-    const float x = b * LOG2E;
-    return __builtin_isinf(x) && !__builtin_isinf(b) ? copysignf(3.402823466e38f, b) : x;
-}
+// scores are kept in units of ln 2 (exp2 needs no product).  A bias below -1e30 -- a type's lowest value as much as -inf -- masks its
+// keys: at that size a score's own digits are lost in it, and a row with nothing else has no weights to tell apart
+__device__ __forceinline__ float bias_log2(float b) { return b < -1e30f ? -INFINITY : fminf(b * LOG2E, 3.402823466e38f) + (b - b); }
 __host__ __device__ inline int bias_lut_bytes(int nbuckets, int maxd) { return nbuckets ? (2 * maxd + 1 + 15) / 16 * 16 : 0; }
 // the table of buckets by the whole workgroup, a key head's biases by `n` threads
 __device__ __forceinline__ Bias load_bias(const Attn& a, unsigned char* lut, float* tbl, int hk, int t, int n) {

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     const int row = r0 + rw * 32 + li, tok = g * a.qb + row / a.G, gl = row % a.G, head = hk * a.G + gl;
     const bool live = there_is && row < R && tok < sq.qlen;
     const int qkey = sq.shift + tok;
-    const int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;
+    int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;
     const bool any = there_is && g * a.qb + r0 / a.G < sq.qlen;             // a live row in this chunk
 
     unsigned char* const lut = (unsigned char*)smem_all;
@@ -156,7 +156,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     load_frags<T, DP>(live ? (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + head * a.sdo.h : nullptr, a.D, hi, gf);
     const size_t stat = ((size_t)b * a.Hq + head) * a.Lq + tok;
-    const float lse = live ? a.lse[stat] * LOG2E : 0.f, delta = live ? a.delta[stat] : 0.f;
+    float lse = live ? a.lse[stat] * LOG2E : 0.f;
+    if (lse == -INFINITY) {                               // (a row that saw nothing: of its keys, or because the bias masks them)
+        lse = 0.f;
+        lim = -1;
+    }
+    const float delta = live ? a.delta[stat] : 0.f;
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
     const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
     const int min_lim = wave_min(live ? lim : INT_MAX);
@@ -460,6 +465,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             if (kw == 0) {
                 put_rows(it + 1);
             } else {
+                if (iadd == -INFINITY) {                  // (a row that saw nothing)
+                    iadd = 0.f;
+                    ilim = -1;
+                }
                 float add = -iadd * LOG2E;
                 bool one = true;                          // every key has the same bucket for this row
                 if (a.nbuckets && ilim >= 0) {

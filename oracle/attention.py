@@ -74,6 +74,13 @@ def visible(sel_row, block, Lk, klen, causal, qkey):
     return m
 
 
+def weigh(P, V, mask):
+    """P V over the visible keys only: what a masked key holds does not matter"""
+    if torch.isfinite(V).all():
+        return P @ V
+    return torch.stack([P[i, m] @ V[m] for i, m in enumerate(mask)])
+
+
 def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None, bias=None, q_pos=None, k_pos=None, dout=None):
     """float64 results and element-wise bounds of the error of a computation whose products and sums are fp32 and whose probabilities
     and score gradients are rounded to the inputs' type in front of the second products:
@@ -107,6 +114,7 @@ def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None
                 kp = torch.arange(Lk) if k_pos is None else k_pos[b].long()
                 md = bucket_of.numel() // 2
                 bucket = bucket_of.long()[(kp[None] - qp[:, None]).clamp(-md, md) + md]
+                mask &= bias[:, h][bucket] >= -1e30                             # (lower ones mask)
                 S = S + bias[:, h].double()[bucket]
                 eS = eS + 2 * U32 * S.abs()
             S = S.masked_fill(~mask, -math.inf)
@@ -119,8 +127,7 @@ def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None
             worst = eS.amax(1, keepdim=True)
             n = mask.sum(1, keepdim=True)
             eP = 2 * worst + (n + 16) * U32                                    # relative, of a probability (its sum included)
-            O = P @ V
-            A = P @ V.abs()
+            O, A = weigh(P, V, mask), weigh(P, V.abs(), mask)
             val['out'][b, :ql, h] = O
             err['out'][b, :ql, h] = A * (u * (q.dtype != torch.float32) + eP + (n + 16) * U32) + u * O.abs()
             val['lse'][b, h, :ql] = torch.where(some, top[:, 0] + L[:, 0].log(), torch.tensor(-math.inf, dtype=torch.float64))

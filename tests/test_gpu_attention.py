@@ -246,6 +246,50 @@ def test_block_attention(A, case, dt):
 
 
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('B,L,Hq,Hk,D,qb,new', [(1, 130, 2, 1, 64, 16, 0), (2, 96, 1, 1, 128, 64, 0), (1, 70, 3, 3, 48, 8, 0), (1, 200, 2, 2, 96, 200, 0),
+                                                (2, 90, 8, 2, 128, 1, 3), (1, 300, 4, 1, 8, 3, 5)])
+def test_what_a_later_key_holds_does_not_reach_an_earlier_query(A, B, L, Hq, Hk, D, qb, new, dt):
+    """infinities and NaN in keys and values of causal sequences: the queries that see them, and only those, show them"""
+    gen = torch.Generator().manual_seed(L)
+    Lq, T = new or L, DT[dt]
+    q, k, v = randn(gen, B, Lq, Hq, D, dtype=T), randn(gen, B, L, Hk, D, dtype=T), randn(gen, B, L, Hk, D, dtype=T)
+    at = [L - 2, L - 1] if new else [L // 2, L // 2 + 1, L - 1]
+    v[0, at[0], 0, 3], v[0, at[1], 0, D - 1], v[-1, at[-1], -1, 0] = math.inf, -math.inf, math.nan
+    k[0, L - 1, -1, 1] = math.nan
+    nb, ng = -(-L // 64), -(-Lq // qb)
+    sel = torch.arange(nb, dtype=torch.int32).expand(B, Hk, ng, nb).contiguous()
+    from adaptivepnp_sci_amd.attention import bucket_table
+    how = dict(block=64, query_block=qb, scale=0.3 / math.sqrt(D), causal=True, qlen=None, klen=None, bucket_of=bucket_table(8, 40, False),
+               bias=0.3 * randn(gen, 8, Hq), q_pos=None, k_pos=None)
+    val, err = reference(q, k, v, sel, how)['out']
+    assert torch.isfinite(val).any() and not torch.isfinite(val).all()
+    got = A.block_attention(cu(q), cu(k), cu(v), cu(sel), **on_gpu(how)).double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(val)) and torch.equal(torch.isinf(got), torch.isinf(val))
+    within(got.nan_to_num(nan=0.0), val.nan_to_num(nan=0.0), err.nan_to_num(nan=0.0), 'out')
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('low', [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min])
+def test_a_bias_of_the_lowest_value_masks(A, low, dt):
+    """some buckets masked for one head, every one for another: zeros there, and no gradient"""
+    gen = torch.Generator().manual_seed(17)
+    T = DT[dt]
+    q, k, v, g = randn(gen, 1, 100, 2, 64, dtype=T), randn(gen, 1, 100, 1, 64, dtype=T), randn(gen, 1, 100, 1, 64, dtype=T), randn(gen, 1, 100, 2, 64, dtype=T)
+    sel = torch.tensor([0, 1], dtype=torch.int32).expand(1, 1, 7, 2).contiguous()
+    from adaptivepnp_sci_amd.attention import bucket_table
+    bias = randn(gen, 8, 2)
+    bias[2:, 0], bias[:, 1] = low, low
+    how = dict(block=64, query_block=16, scale=0.2, causal=False, qlen=None, klen=None, bucket_of=bucket_table(8, 20), bias=bias, q_pos=None, k_pos=None)
+    want = reference(q, k, v, sel, how, dout=g)
+    args = [cu(t) for t in (q, k, v, sel)]
+    out, saved = A.block_attention(*args, save=True, **on_gpu(how))
+    within(out, *want['out'], 'out')
+    assert not out[:, :, 1].any() and torch.equal(saved[0][:, 1].cpu(), torch.full((1, 100), -math.inf))
+    for name, t in zip(('dq', 'dk', 'dv', 'dbias'), A.block_attention_backward(cu(g), *args, saved, **on_gpu(how))):
+        within(t, *want[name], name)
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
 @pytest.mark.parametrize('case', ATTN)
 def test_block_attention_backward(A, case, dt):
     q, k, v, g, sel, how = problem(case, dt, torch.Generator().manual_seed(case[1] * 3 + case[2]))
