@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         if constexpr (sizeof(T) == 4) {
             if (skip) continue;
         }
-        vt.template mma<SAVE>(s, o);
+        vt.template mma<SAVE ? 3 : 1>(s, o);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     l += __shfl_xor(l, 32, 64);

@@ -126,7 +126,7 @@ __device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat
 // bf16: read() brings the transposed tile into registers, early, so that the reads overlap the score products and the softmax;
 //   the 16 lanes of a group supply 4 rows x 16 columns (8 bytes each) and receive a column's 4 rows.  Assembly because the compiler
 //   takes the builtin for a reader of every request in flight and waits for the NEXT tile in front of it; the block waits for its reads.
-//   Column 32 db + m is row m of block db.  EXACT: P as three bf16 numbers that add up to its 24 bits, three products.
+//   Column 32 db + m is row m of block db.  PARTS: the bf16 numbers that P is split into, a product each; 3 hold its 24 bits, 2 hold 16.
 // fp32: with 2 or 4 blocks a lane reads 2 or 4 neighbouring columns at once: column NB m + db is row m of block db.
 typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
 template <typename T, int DP>
@@ -249,7 +249,7 @@ struct ColTile {
                     for (int i = 0; i < 8; ++i) u[db][k].v[i] = (__bf16)0.f;
         }
     }
-    template <bool EXACT = false>
+    template <int PARTS = 1>
     __device__ __forceinline__ void mma(const f32x16a& p, f32x16a (&acc)[NB]) const {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -259,20 +259,20 @@ struct ColTile {
                 for (int i = 0; i < 8; ++i) {
                     const float x = p[8 * k + i];
                     pb[i] = (__bf16)x;
-                    if constexpr (EXACT) {
+                    if constexpr (PARTS > 1) {
                         const float r1 = x - (float)pb[i];
                         p1[i] = (__bf16)r1;
-                        p2[i] = (__bf16)(r1 - (float)p1[i]);
+                        if constexpr (PARTS > 2) p2[i] = (__bf16)(r1 - (float)p1[i]);
                     }
                 }
 #pragma unroll
                 for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, pb, acc[db], 0, 0, 0);
-                if constexpr (EXACT) {
+                if constexpr (PARTS > 1)
 #pragma unroll
                     for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p1, acc[db], 0, 0, 0);
+                if constexpr (PARTS > 2)
 #pragma unroll
                     for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[db], 0, 0, 0);
-                }
             }
         } else {
             constexpr int W = NB == 3 ? 1 : NB;            // floats of a read

@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
                         for (int r = 0; r < 16; ++r) mine[d[r] * HROW] += s[r];
             }
         }
-        kc.mma(s, o);
+        kc.template mma<2>(s, o);                         // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     if (a.dbias) {                                        // the set's sums: a (bucket, head) adds its lanes in order, in fp64
