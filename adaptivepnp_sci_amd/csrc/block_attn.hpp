@@ -350,10 +350,10 @@ struct Attn {
     float* dbias;
     float *po, *pml;                                      // forward, splits > 1: partial results, their maxima and sums
     // backward
-    const float* delta;
+    float* delta;
     float* zeros;                                         // 256 bytes
-    unsigned* member;                                     // [b, hk][key block][ng bits], then [b, hk][key block] counts
-    int words;
+    unsigned* member;                                     // [b, hk][32 groups][nb4 key blocks], a bit a group
+    int words, nb4;
     const int* chunk_start;                               // [b, hk][key block + 1]
     int max_chunks;
     float* pkv;                                           // partial dk, dv

@@ -21,78 +21,76 @@ __device__ __forceinline__ unsigned fast_div(unsigned x, unsigned d, unsigned m,
 }
 static inline unsigned div_magic(int d) { return d <= 1 ? 0xFFFFFFFFu : (unsigned)((1ull << 32) / (unsigned)d); }
 
-// ---- delta of every live row (16 lanes a row), and the membership bits (and counts) cleared for the launch behind it
-template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(Attn a, float* delta, size_t member_words) {
-    const size_t rows = (size_t)a.B * a.Lq * a.Hq;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < member_words; i += (size_t)gridDim.x * 256) a.member[i] = 0;
-    if (blockIdx.x == 0 && threadIdx.x < 64) a.zeros[threadIdx.x] = 0;      // what the rows that do not exist are read from
-    for (size_t id = (size_t)blockIdx.x * 16 + (threadIdx.x >> 4); id < rows; id += (size_t)gridDim.x * 16) {
-        const int head = (int)(id % a.Hq), tok = (int)(id / a.Hq % a.Lq), b = (int)(id / a.Hq / a.Lq), l16 = threadIdx.x & 15;
-        float s = 0.f;
-        if (tok < seq_of(a, b).qlen) {
-            const T* g = (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + head * a.sdo.h;
-            for (int d = 4 * l16; d < a.D; d += 64) {
-                const f32x4a o = *(const f32x4a*)(a.out32 + id * a.D + d);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s = fmaf((float)g[d + e], o[e], s);
+// ---- the selection the other way round: a workgroup gathers 32 query groups, a bit each in a word for every key block.  No word is
+// written twice, so nothing has to be cleared before; and the zeros that rows that do not exist are read from
+constexpr int MARK_WAVES = 16, MARK_CAP = 16384;          // (key blocks in LDS at a time)
+__global__ void __launch_bounds__(64 * MARK_WAVES) attn_mark_kernel(Attn a, int cap) {
+    extern __shared__ unsigned bits[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, word = blockIdx.x, bh = blockIdx.y;
+    int* const list = (int*)(bits + cap) + wave * a.n;
+    const Seq s = seq_of(a, bh / a.Hk);
+    if (word == 0 && bh == 0 && tid < 64) a.zeros[tid] = 0.f;
+    for (int base = 0; base < a.nb; base += cap) {
+        const int m = min(cap, a.nb - base);
+        for (int i = tid; i < m; i += 64 * MARK_WAVES) bits[i] = 0;
+        __syncthreads();
+        for (int g = 32 * word + wave; g < min(a.ng, 32 * word + 32); g += MARK_WAVES) {
+            const int q0 = g * a.qb, nq = min(a.qb, s.qlen - q0);
+            if (nq <= 0) break;
+            const int far = a.causal ? min(s.klen, s.shift + q0 + nq) : s.klen;
+            const int c = live_blocks(a, a.sel + ((size_t)bh * a.ng + g) * a.n, far, list, lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int i = lane; i < c; i += 64) {
+                const int e = list[i] - base;
+                if (e >= 0 && e < m) atomicOr(&bits[e], 1u << (g & 31));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        __syncthreads();
+        for (int i = tid; i < m; i += 64 * MARK_WAVES) a.member[((size_t)bh * a.words + word) * a.nb4 + base + i] = bits[i];
+        __syncthreads();
+    }
+}
+
+// ---- chunks of every key block of one (sequence, key head), by one workgroup: chunk_start[j] = chunks of the blocks before j
+__device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH, int* lds) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    int* const wsum = lds;
+    int* const cs = (int*)a.chunk_start + (size_t)bh * (a.nb + 1);
+    int carry = 0;
+    for (int base = 0; base < a.nb; base += 4 * blockDim.x) {     // four neighbouring blocks a thread
+        const int j = base + 4 * tid;
+        int n[4] = {0, 0, 0, 0};
+        if (j < a.nb) {
+            const uint4* p = (const uint4*)(a.member + (size_t)bh * a.words * a.nb4 + j);
+#pragma unroll 16
+            for (int w = 0; w < a.words; ++w) {
+                const uint4 x = p[(size_t)w * (a.nb4 / 4)];
+                n[0] += __popc(x.x), n[1] += __popc(x.y), n[2] += __popc(x.z), n[3] += __popc(x.w);
             }
         }
-        s += __shfl_xor(s, 8, 16);
-        s += __shfl_xor(s, 4, 16);
-        s += __shfl_xor(s, 2, 16);
-        s += __shfl_xor(s, 1, 16);
-        if (l16 == 0) delta[((size_t)b * a.Hq + head) * a.Lq + tok] = s;
-    }
-}
-
-// ---- the selection the other way round: one wave a query group sets its bit in each of its blocks and counts itself (whole numbers: no order)
-__global__ void __launch_bounds__(256) attn_mark_kernel(Attn a) {
-    extern __shared__ int lists[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long item = (long long)blockIdx.x * 4 + wave;
-    if (item >= (long long)a.B * a.Hk * a.ng) return;
-    int* const list = lists + wave * a.n;
-    const int g = (int)(item % a.ng), bh = (int)(item / a.ng);
-    const Seq s = seq_of(a, bh / a.Hk);
-    const int q0 = g * a.qb, nq = min(a.qb, s.qlen - q0);
-    if (nq <= 0) return;
-    const int far = a.causal ? min(s.klen, s.shift + q0 + nq) : s.klen;
-    const int c = live_blocks(a, a.sel + (size_t)item * a.n, far, list, lane);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    unsigned* const counts = a.member + (size_t)a.B * a.Hk * a.nb * a.words;
-    for (int i = lane; i < c; i += 64) {
-        atomicOr(&a.member[((size_t)bh * a.nb + list[i]) * a.words + (g >> 5)], 1u << (g & 31));
-        atomicAdd(&counts[(size_t)bh * a.nb + list[i]], 1u);
-    }
-}
-
-// ---- chunks of every key block of one (sequence, key head): chunk_start[j] = chunks of the blocks before j
-__global__ void __launch_bounds__(256) attn_plan_kernel(Attn a, int* chunk_start, int R, int CH) {
-    __shared__ int wsum[4], carry;
-    const int bh = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int* const cs = chunk_start + (size_t)bh * (a.nb + 1);
-    if (tid == 0) carry = 0;
-    __syncthreads();
-    for (int base = 0; base < a.nb; base += 256) {
-        const int j = base + tid;
-        int c = 0;
-        if (j < a.nb) {
-            const unsigned* counts = a.member + (size_t)a.B * a.Hk * a.nb * a.words;
-            c = (int)(((long long)counts[(size_t)bh * a.nb + j] * R + CH - 1) / CH);
+        int sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = j + e < a.nb ? (int)(((long long)n[e] * R + CH - 1) / CH) : 0;
+            n[e] = sum;
+            sum += c;
         }
-        int incl = c;
+        int incl = sum;
         for (int off = 1; off < 64; off <<= 1) {
             const int o = __shfl_up(incl, off, 64);
             if (lane >= off) incl += o;
         }
         if (lane == 63) wsum[wave] = incl;
         __syncthreads();
-        int at = carry + incl - c;
-        for (int w = 0; w < wave; ++w) at += wsum[w];
-        if (j < a.nb) cs[j] = at;
-        __syncthreads();
-        if (tid == 0) carry += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+        int at = carry + incl - sum;
+        for (int w = 0; w < waves; ++w) {
+            if (w < wave) at += wsum[w];
+            carry += wsum[w];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < a.nb) cs[j + e] = at + n[e];
         __syncthreads();
     }
     if (tid == 0) cs[a.nb] = carry;
@@ -109,13 +107,17 @@ struct DqCfg {
 constexpr int HROW = 33;                                  // a bucket's sums of 32 rows, shifted by a bank
 
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes) {
+__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes, int plans, int CH) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DqCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32;
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
-    const long long total = (long long)a.B * a.Hk * a.ng * a.chunks, first = xcd_item(blockIdx.x, (total + sets - 1) / sets);
+    if (blockIdx.x < plans) {                             // the first workgroups cut the chunks of the launch behind this one
+        plan_chunks(a, blockIdx.x, a.qb * a.G, CH, (int*)smem_all);
+        return;
+    }
+    const long long total = (long long)a.B * a.Hk * a.ng * a.chunks, first = xcd_item(blockIdx.x - plans, (total + sets - 1) / sets);
     if (first < 0) return;
     const int lane = threadIdx.x & 63, li = lane & 31, hi = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int set = wave / RW, rw = wave % RW, tset = rw * 64 + lane;
@@ -161,7 +163,20 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
         lse = 0.f;
         lim = -1;
     }
-    const float delta = live ? a.delta[stat] : 0.f;
+    // delta of the row, in fp64: each half of a row's lanes has half of it
+    double dsum = 0.0;
+    if (live) {
+        const float* const orow = a.out32 + (((size_t)b * a.Lq + tok) * a.Hq + head) * a.D;
+#pragma unroll
+        for (int s = 0; s < DP / Mat<T>::K; ++s) {
+            const int c = Mat<T>::K * s + Mat<T>::E * hi;
+            if (c < a.D)
+#pragma unroll
+                for (int i = 0; i < Mat<T>::E; ++i) dsum = fma((double)(float)gf[s][i], (double)orow[c + i], dsum);
+        }
+    }
+    const float delta = (float)(dsum + __shfl_xor(dsum, 32, 64));
+    if (live && hi == 0) a.delta[stat] = delta;
     const int qp = a.nbuckets && live ? (a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : qkey) : 0;
     const RowRange range = {wave_min(live ? qp : INT_MAX), wave_max(live ? qp : INT_MIN)};
     const int min_lim = wave_min(live ? lim : INT_MAX);
@@ -293,18 +308,6 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
 #endif
 }
 
-// dbias[n][head]: one wave sums the workgroups' partials, every 64th a lane
-__global__ void __launch_bounds__(64) attn_dbias_kernel(Attn a) {
-    const int n = blockIdx.x / a.Hq, head = blockIdx.x % a.Hq, hk = head / a.G, h = head % a.G, lane = threadIdx.x;
-    const size_t per = (size_t)a.ng * a.chunks, row = (size_t)a.nbuckets * a.G;
-    double s = 0.0;
-    for (int b = 0; b < a.B; ++b) {
-        const double* p = a.pbias + ((size_t)(b * a.Hk + hk) * per) * row + (size_t)n * a.G + h;
-        for (size_t i = lane; i < per; i += 64) s += p[i * row];
-    }
-    s = wave_sum_f64(s);
-    if (lane == 0) a.dbias[(size_t)n * a.Hq + head] = (float)s;
-}
 
 // ---- dK, dV of 64 keys over one chunk of the query rows that chose their block.  Waves: two halves of the keys x two of the row tiles;
 // a wave keeps its 32 keys and values in registers (the B operands) and streams rows, which the memory system writes to LDS
@@ -349,10 +352,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     const unsigned x0 = (unsigned)(c - cs[j]) * CH;
     int count = 0;
     {
-        const unsigned* w = a.member + ((size_t)bh * a.nb + j) * a.words;
+        const unsigned* w = a.member + (size_t)bh * a.words * a.nb4 + j;
         const int e0 = (int)(x0 / R), e1 = (int)((x0 + CH + R - 1) / R);
         for (int base = 0; base < a.words; base += 256) {
-            const unsigned bits = base + tid < a.words ? w[base + tid] : 0;
+            const unsigned bits = base + tid < a.words ? w[(size_t)(base + tid) * a.nb4] : 0;
             const int n = __popc(bits);
             int incl = n;
             for (int off = 1; off < 64; off <<= 1) {
@@ -578,14 +581,33 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
 #endif
 }
 
+// dbias[n][head]: one wave sums the workgroups' partials, every 64th a lane
+__device__ __forceinline__ void dbias_pair(const Attn& a, int pair) {
+    const int n = pair / a.Hq, head = pair % a.Hq, hk = head / a.G, h = head % a.G, lane = threadIdx.x & 63;
+    const size_t per = (size_t)a.ng * a.chunks, row = (size_t)a.nbuckets * a.G;
+    double s = 0.0;
+    for (int b = 0; b < a.B; ++b) {
+        const double* p = a.pbias + ((size_t)(b * a.Hk + hk) * per) * row + (size_t)n * a.G + h;
+        for (size_t i = lane; i < per; i += 64) s += p[i * row];
+    }
+    s = wave_sum_f64(s);
+    if (lane == 0) a.dbias[(size_t)n * a.Hq + head] = (float)s;
+}
+
 // blocks that more than one chunk worked on (their partials in order), and blocks that nobody chose (zeros)
 template <typename T>
-__global__ void __launch_bounds__(256) attn_dkv_join_kernel(Attn a, int subs) {
-    const int j = blockIdx.x / subs, sub = blockIdx.x % subs, bh = blockIdx.y, hk = bh % a.Hk, b = bh / a.Hk;
+__global__ void __launch_bounds__(256) attn_end_kernel(Attn a, int subs, unsigned joins) {
+    if (blockIdx.x >= joins) {
+        const int pair = (blockIdx.x - joins) * 4 + (threadIdx.x >> 6);
+        if (pair < a.nbuckets * a.Hq) dbias_pair(a, pair);
+        return;
+    }
+    const unsigned parts = (2 * KB * (a.D / 4) + 255) / 256, x = blockIdx.x / parts;
+    const int sub = x % subs, j = x / subs % a.nb, bh = x / subs / a.nb, hk = bh % a.Hk, b = bh / a.Hk;
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     const int c0 = cs[j], n = cs[j + 1] - c0;
     if (n == 1) return;
-    const int per = a.D / 4, i = blockIdx.z * 256 + threadIdx.x, which = i / (KB * per), k = i / per % KB, d = 4 * (i % per);
+    const int per = a.D / 4, i = blockIdx.x % parts * 256 + threadIdx.x, which = i / (KB * per), k = i / per % KB, d = 4 * (i % per);
     const int key = j * a.block + sub * KB + k;
     if (which > 1 || key >= a.Lk) return;
     f32x4a s = {0.f, 0.f, 0.f, 0.f};
@@ -628,7 +650,7 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
     const size_t bh = (size_t)a->B * a->Hk;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     size_t at = up((size_t)a->B * a->Hq * a->Lq * 4) + 256;                  // delta, zeros
-    p.o_member = at; at += up(bh * p.nb * (p.words + 1) * 4);                // bits, then counts
+    p.o_member = at; at += up(bh * ((p.nb + 3) / 4 * 4) * p.words * 4);
     p.o_chunk = at; at += up(bh * (p.nb + 1) * 4);
     p.o_pkv = at; at += up(bh * p.max_chunks * p.subs * 2 * KB * a->D * 4);
     p.o_pbias = at; at += a->num_buckets ? up(bh * p.ng * p.chunks * a->num_buckets * (a->Hq / a->Hk) * 8) : 0;
@@ -638,7 +660,7 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
 size_t attn_backward_workspace(const scipnp_block_attn_args* a) { return bwd_plan(a).total; }
 
 template <typename T, int DP, int RW>
-static int dq_launch(const Attn& p, hipStream_t st) {
+static int dq_launch(const Attn& p, int CH, hipStream_t st) {
     using C = DqCfg<T, DP>;
     const size_t set = ((size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + (size_t)(p.nbuckets * p.G + 3) / 4 * 16 + (size_t)RW * p.nbuckets * HROW * 4 + 15) / 16 * 16;
     const size_t shared = bias_lut_bytes(p.nbuckets, p.maxd) + 16;
@@ -648,12 +670,13 @@ static int dq_launch(const Attn& p, hipStream_t st) {
     static LdsAttrOnce once;
     if (const int rc = once.ensure((const void*)block_attn_dq_kernel<T, DP, RW>, 163840, "block_attn_dq")) return rc;
     const long long items = (long long)p.B * p.Hk * p.ng * p.chunks;
-    block_attn_dq_kernel<T, DP, RW><<<xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set);
+    const unsigned plans = (unsigned)(p.B * p.Hk);
+    block_attn_dq_kernel<T, DP, RW><<<plans + xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set, (int)plans, CH);
     return SCIPNP_OK;
 }
 template <typename T, int DP>
 static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
-    const int rc = bp.rw == 1 ? dq_launch<T, DP, 1>(p, st) : bp.rw == 2 ? dq_launch<T, DP, 2>(p, st) : dq_launch<T, DP, 4>(p, st);
+    const int rc = bp.rw == 1 ? dq_launch<T, DP, 1>(p, bp.CH, st) : bp.rw == 2 ? dq_launch<T, DP, 2>(p, bp.CH, st) : dq_launch<T, DP, 4>(p, bp.CH, st);
     if (rc) return rc;
     using C = DkvCfg<T, DP>;
     const size_t lds = (size_t)C::MAIN + (C::LIST + 8) * 4 + bias_lds(p.nbuckets, p.maxd, p.G);
@@ -666,20 +689,18 @@ static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
 }
 
 template <typename T>
-static int bwd_run(const Attn& p, const BwdPlan& bp, float* delta, int* chunk_start, hipStream_t st) {
-    const size_t rows = (size_t)p.B * p.Lq * p.Hq, words = (size_t)p.B * p.Hk * p.nb * (p.words + 1);
-    const size_t want = (rows + 15) / 16;
-    attn_delta_kernel<T><<<(unsigned)(want < 8192 ? want : 8192), 256, 0, st>>>(p, delta, words);
-    const size_t groups = (size_t)p.B * p.Hk * p.ng;
-    attn_mark_kernel<<<(unsigned)((groups + 3) / 4), 256, (size_t)4 * p.n * 4, st>>>(p);
-    attn_plan_kernel<<<(unsigned)(p.B * p.Hk), 256, 0, st>>>(p, chunk_start, bp.R, bp.CH);
+static int bwd_run(const Attn& p, const BwdPlan& bp, hipStream_t st) {
+    static LdsAttrOnce once;
+    if (const int rc = once.ensure((const void*)attn_mark_kernel, 163840, "attn_mark")) return rc;
+    const int cap = p.nb < MARK_CAP ? p.nb : MARK_CAP;
+    attn_mark_kernel<<<dim3((unsigned)bp.words, (unsigned)(p.B * p.Hk)), 64 * MARK_WAVES, (size_t)(cap + MARK_WAVES * p.n) * 4, st>>>(p, cap);
     int rc;
     if (sizeof(T) == 4 && p.D > 32 && p.D <= 48) rc = bwd_launch<T, sizeof(T) == 4 ? 48 : 64>(p, bp, st);
     else rc = p.D <= 32 ? bwd_launch<T, 32>(p, bp, st) : p.D <= 64 ? bwd_launch<T, 64>(p, bp, st)
                  : p.D <= 96 ? bwd_launch<T, 96>(p, bp, st) : bwd_launch<T, 128>(p, bp, st);
     if (rc) return rc;
-    attn_dkv_join_kernel<T><<<dim3((unsigned)(p.nb * bp.subs), (unsigned)(p.B * p.Hk), (unsigned)((2 * KB * (p.D / 4) + 255) / 256)), 256, 0, st>>>(p, bp.subs);
-    if (p.dbias) attn_dbias_kernel<<<(unsigned)(p.nbuckets * p.Hq), 64, 0, st>>>(p);
+    const unsigned joins = (unsigned)(p.nb * bp.subs) * (unsigned)(p.B * p.Hk) * (unsigned)((2 * KB * (p.D / 4) + 255) / 256);
+    attn_end_kernel<T><<<joins + (p.dbias ? (p.nbuckets * p.Hq + 3) / 4 : 0), 256, 0, st>>>(p, bp.subs, joins);
     return launch_status("scipnp_block_attn_backward");
 }
 
@@ -706,13 +727,14 @@ int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t 
     p.zeros = (float*)(w + bp.o_member - 256);
     p.member = (unsigned*)(w + bp.o_member);
     p.words = bp.words;
+    p.nb4 = (p.nb + 3) / 4 * 4;
     p.chunk_start = (int*)(w + bp.o_chunk);
     p.max_chunks = bp.max_chunks;
     p.pkv = (float*)(w + bp.o_pkv);
     p.pbias = (double*)(w + bp.o_pbias);
     p.chunks = bp.chunks;
-    return a->dtype == SCIPNP_BF16 ? bwd_run<__bf16>(p, bp, (float*)w, (int*)(w + bp.o_chunk), (hipStream_t)s)
-                                   : bwd_run<float>(p, bp, (float*)w, (int*)(w + bp.o_chunk), (hipStream_t)s);
+    return a->dtype == SCIPNP_BF16 ? bwd_run<__bf16>(p, bp, (hipStream_t)s)
+                                   : bwd_run<float>(p, bp, (hipStream_t)s);
 }
 
 }
