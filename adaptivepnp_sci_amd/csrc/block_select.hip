@@ -75,7 +75,7 @@ struct Select {
     const int32_t *qlen, *klen;
     int32_t* sel;
     int B, Lq, Lk, Hq, Hk, D, block, qb, n, sink, local, causal, nb, ng;
-    int gpw, tiles, hist_at;                              // groups of a workgroup, workgroups of a (sequence, key head), LDS offset
+    int gpw, tiles, kst, hist_at;                         // groups of a workgroup, workgroups of a (sequence, key head), keys of a row, LDS offset
 };
 
 constexpr int SEL_MAX_BLOCKS = 8192;
@@ -126,23 +126,80 @@ __device__ __forceinline__ void radix_pass(F key, int nb, int shift, K& prefix, 
     all = need == __shfl(have, src, 64);
 }
 
-// One wave writes the n best of the candidates 0 .. nb-1, ascending; ties to the lower index.  The scores are compared as fp32 keys
-// first (half the LDS, at most four passes); only where the n-th and the next share one are those candidates compared in fp64,
-// recomputed by exact(j).
+// the need-th greatest of the keys that count(t) counts from t on, bit by bit
 template <typename F>
-__device__ void select_best(const unsigned* keys, int nb, int n, int32_t* out, int* hist, int lane, F exact) {
+__device__ __forceinline__ unsigned nth_greatest(int need, F count) {
+    unsigned t = 0;
+#pragma unroll 4
+    for (int bit = 31; bit >= 0; --bit)
+        if (count(t | 1u << bit) >= need) t |= 1u << bit;
+    return t;
+}
+
+// One wave writes the n best of the candidates 0 .. nb-1, ascending; ties to the lower index.  The scores are compared as fp32 keys
+// first (half the LDS); only where the n-th and the next share one are those candidates compared in fp64, recomputed by exact(j).
+// Up to 32 wanted of more than 256: the need-th greatest of the lanes' own greatest keys is a bound that few others reach (16 of 2048:
+// about 18), and those few are sorted out in registers.  Otherwise a radix selection over all keys.  (16 of 2048 blocks, 2048 groups:
+// 56 us with the radix passes, whose counters collide, 40 us by the bound; 16 of 128: 9.4 against 10.5 us, so there they stay)
+constexpr int SHORT = 256;
+template <typename F>
+__device__ void select_best(const unsigned* keys, int nb, int n, int32_t* out, int* hist, unsigned short* list, int lane, F exact) {
+    const unsigned long long below = (1ull << lane) - 1;
     int cand = 0;
-    for (int base = 0; base < nb; base += 64) cand += __popcll(__ballot(base + lane < nb && keys[base + lane] != 0));
+    unsigned top = 0;
+    for (int j = lane; j < nb; j += 64) {
+        const unsigned k = keys[j];
+        cand += k != 0;
+        top = max(top, k);
+    }
+    for (int off = 32; off > 0; off >>= 1) cand += __shfl_xor(cand, off, 64);
+    cand = __builtin_amdgcn_readfirstlane(cand);
     unsigned prefix = 0, mask = 0;                         // the threshold's known upper bytes
     int need = min(n, cand);                               // still to take among the keys with that prefix
     bool all = need == cand;                               // take every key with the prefix (and every greater one)
-    for (int shift = 24; shift >= 0 && !all; shift -= 8)
-        radix_pass<unsigned>([&](int j) { return keys[j]; }, nb, shift, prefix, mask, need, all, hist, lane);
+    int items = nb;                                        // the candidates that are still looked at: all, or those of the list
+    bool listed = false;
+    if (!all && nb > SHORT && need <= 32) {
+        const unsigned bound = max(nth_greatest(need, [&](unsigned t) { return __popcll(__ballot(top >= t)); }), 1u);
+        int c = 0;
+        for (int base = 0; base < nb; base += 64) {
+            const int j = base + lane;
+            const bool in = j < nb && keys[j] >= bound;
+            const unsigned long long m = __ballot(in);
+            const int at = c + __popcll(m & below);
+            if (in && at < SHORT) list[at] = (unsigned short)j;
+            c += __popcll(m);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (c <= SHORT) {
+            listed = true;
+            items = c;
+            unsigned r[SHORT / 64];
+#pragma unroll
+            for (int u = 0; u < SHORT / 64; ++u) r[u] = lane + 64 * u < c ? keys[list[lane + 64 * u]] : 0;
+            auto from = [&](unsigned t) {
+                int s = __popcll(__ballot(r[0] >= t));
+                if (c > 64)
+#pragma unroll
+                    for (int u = 1; u < SHORT / 64; ++u) s += __popcll(__ballot(r[u] >= t));
+                return s;
+            };
+            prefix = nth_greatest(need, from);
+            mask = ~0u;
+            const int more = prefix == ~0u ? 0 : from(prefix + 1);
+            all = need == from(prefix);
+            need -= more;
+        }
+    }
+    if (!listed)
+        for (int shift = 24; shift >= 0 && !all; shift -= 8)
+            radix_pass<unsigned>([&](int j) { return keys[j]; }, nb, shift, prefix, mask, need, all, hist, lane);
+    auto at_item = [&](int i) { return listed ? (int)list[i] : i; };
     unsigned long long prefix64 = 0, mask64 = 0;
     if (!all && prefix != ~0u && prefix != 1) {            // (the always chosen and the NaNs are equal among themselves)
-        auto key64 = [&](int j) -> unsigned long long { return keys[j] == prefix ? order_key(exact(j)) : 0; };
+        auto key64 = [&](int i) -> unsigned long long { const int j = at_item(i); return keys[j] == prefix ? order_key(exact(j)) : 0; };
         unsigned long long lo = ~0ull, hi = 0;
-        for (int j = lane; j < nb; j += 64) {
+        for (int j = lane; j < items; j += 64) {
             const unsigned long long k = key64(j);
             if (k) { lo = min(lo, k); hi = max(hi, k); }
         }
@@ -151,14 +208,13 @@ __device__ void select_best(const unsigned* keys, int nb, int n, int32_t* out, i
             hi = max(hi, (unsigned long long)__shfl_xor((long long)hi, off, 64));
         }
         if (lo != hi)
-            for (int shift = 56; shift >= 0 && !all; shift -= 8) radix_pass<unsigned long long>(key64, nb, shift, prefix64, mask64, need, all, hist, lane);
+            for (int shift = 56; shift >= 0 && !all; shift -= 8) radix_pass<unsigned long long>(key64, items, shift, prefix64, mask64, need, all, hist, lane);
     }
     // greater than the threshold: in; equal: the first `need` of them
     int eqs = 0, at = 0;
-    for (int base = 0; base < nb; base += 64) {
-        const int j = base + lane;
-        const unsigned k = j < nb ? keys[j] : 0;
-        const unsigned long long below = (1ull << lane) - 1;
+    for (int base = 0; base < items; base += 64) {
+        const int j = base + lane < items ? at_item(base + lane) : 0;
+        const unsigned k = base + lane < items ? keys[j] : 0;
         bool eq = k != 0 && (k & mask) == prefix, gt = k != 0 && (k & mask) > prefix;
         if (mask64 != 0 && eq) {
             const unsigned long long e = order_key(exact(j));
@@ -190,9 +246,10 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
     extern __shared__ __attribute__((aligned(16))) char smem_s[];
     const int qst = a.D + 2;                               // (rows two banks apart)
     double* const qs = (double*)smem_s;                    // [groups][qst]
-    double* const scratch = qs + a.gpw * qst;              // step 1: the parts; then the keys [groups][nb]
+    double* const scratch = qs + a.gpw * qst;              // step 1: the parts; then the keys [groups][kst]
     unsigned* const keys = (unsigned*)scratch;
     int* const hists = (int*)(smem_s + a.hist_at);
+    unsigned short* const lists = (unsigned short*)(hists + SEL_WAVES * 256);
     const long long total = (long long)a.B * a.Hk * a.tiles, item = xcd_item(blockIdx.x, total);
     if (item < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -245,23 +302,38 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
     const int last = klen - qlen + min((gc + 1) * a.qb, qlen) - 1;
     const int own = last >= 0 ? last / a.block : (last - a.block + 1) / a.block;
     const int seen = min((klen + a.block - 1) / a.block, !a.causal ? a.nb : last < 0 ? 0 : last / a.block + 1);        // blocks it may choose
-    const int nt = (a.nb + 15) / 16;
+    // no group here sees a block from `nb` on (its own rows end with the last group's last query): neither scored nor looked at
+    const int lastq = min((g0 + ngr) * a.qb, qlen), end = klen - qlen + lastq;
+    const int nb = lastq <= g0 * a.qb ? 0 : min((klen + a.block - 1) / a.block, !a.causal ? a.nb : end <= 0 ? 0 : (end - 1) / a.block + 1);
+    const int nt = (nb + 15) / 16;
     const double* const qrow = qs + (col < a.gpw ? col : 0) * qst + 4 * kq;
     const float* const means = a.summary + ((size_t)b * a.nb * a.Hk + hk) * a.D;
+    auto query = [&](int d, double (&q)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = 16 * d + 4 * kq < a.D ? qrow[16 * d + e] : 0.0;
+    };
+    constexpr bool HELD = ND <= 8;                         // the sums stay in registers while the tiles go by (16 columns: 128 VGPRs, read again)
+    double held[HELD ? ND : 1][4];
+    if constexpr (HELD)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) query(d, held[d]);
     for (int jt = wave; jt < nt; jt += SEL_WAVES) {
         const int j = jt * 16 + col;                       // (A's row)
         f32x4a m[ND];
-        const float* const row = means + (size_t)(j < a.nb ? j : 0) * a.Hk * a.D + 4 * kq;
+        const float* const row = means + (size_t)(j < nb ? j : 0) * a.Hk * a.D + 4 * kq;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) m[d] = j < a.nb && 16 * d + 4 * kq < a.D ? *(const f32x4a*)(row + 16 * d) : f32x4a{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < ND; ++d) m[d] = j < nb && 16 * d + 4 * kq < a.D ? *(const f32x4a*)(row + 16 * d) : f32x4a{0.f, 0.f, 0.f, 0.f};
         f64x4a s0 = {0.0, 0.0, 0.0, 0.0}, s1 = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (16 * d >= a.D) continue;                   // (uniform)
-            double q[4] = {0.0, 0.0, 0.0, 0.0};
-            if (16 * d + 4 * kq < a.D)
+            double q[4];
+            if constexpr (HELD) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[e] = qrow[16 * d + e];
+                for (int e = 0; e < 4; ++e) q[e] = held[d][e];
+            } else {
+                query(d, q);
+            }
             s0 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][0], q[0], s0, 0, 0, 0);
             s1 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][1], q[1], s1, 0, 0, 0);
             s0 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)m[d][2], q[2], s0, 0, 0, 0);
@@ -271,14 +343,14 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int jj = jt * 16 + 4 * r + kq;
-                if (jj >= a.nb) continue;
+                if (jj >= nb) continue;
                 const bool must = jj < a.sink || abs(jj - own) < a.local;
-                keys[(size_t)col * a.nb + jj] = !group || jj >= seen ? 0u : must ? ~0u : order_key((float)(s0[r] + s1[r]));
+                keys[(size_t)col * a.kst + jj] = !group || jj >= seen ? 0u : must ? ~0u : order_key((float)(s0[r] + s1[r]));
             }
     }
     __syncthreads();
     for (int i = wave; i < ngr; i += SEL_WAVES)
-        select_best(keys + (size_t)i * a.nb, a.nb, a.n, a.sel + ((size_t)bh * a.ng + g0 + i) * a.n, hists + wave * 256, lane, [&](int j) {
+        select_best(keys + (size_t)i * a.kst, nb, a.n, a.sel + ((size_t)bh * a.ng + g0 + i) * a.n, hists + wave * 256, lists + wave * SHORT, lane, [&](int j) {
             const float* m = means + (size_t)j * a.Hk * a.D;
             double s = 0.0;
             for (int d = 0; d < a.D; d += 4) {
@@ -360,11 +432,12 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s) {
     p.gpw = p.gpw > 16 ? 16 : p.gpw;
     if (p.gpw > p.ng) p.gpw = p.ng;
     p.tiles = (p.ng + p.gpw - 1) / p.gpw;
-    const size_t parts_bytes = (size_t)SEL_WAVES * 64 * (16 / attn_esize(a->dtype)) * 8, key_bytes = ((size_t)p.gpw * p.nb * 4 + 15) / 16 * 16;
+    p.kst = (p.nb + 31) / 32 * 32 + 4;                    // (16 groups' keys of a block in different banks)
+    const size_t parts_bytes = (size_t)SEL_WAVES * 64 * (16 / attn_esize(a->dtype)) * 8, key_bytes = ((size_t)p.gpw * p.kst * 4 + 15) / 16 * 16;
     p.hist_at = (int)((size_t)p.gpw * (a->D + 2) * 8 + (parts_bytes > key_bytes ? parts_bytes : key_bytes));
     const long long items = (long long)a->B * a->Hk * p.tiles;
     SCIPNP_REQUIRE(items < (1ll << 22) && (long long)p.ng * a->query_block < (1ll << 30), "too many query groups");
-    const size_t lds = (size_t)p.hist_at + SEL_WAVES * 256 * 4;
+    const size_t lds = (size_t)p.hist_at + SEL_WAVES * (256 * 4 + SHORT * 2);
     return a->dtype == SCIPNP_BF16 ? select_launch<__bf16>(p, lds, xcd_grid(items), (hipStream_t)s) : select_launch<float>(p, lds, xcd_grid(items), (hipStream_t)s);
 }
 
