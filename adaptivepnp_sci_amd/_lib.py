@@ -219,7 +219,7 @@ class BlockAttnArgs(C.Structure):
                                           'max_distance', 'zero_rest')]
                 + [('scale', C.c_float)] + [(n, C.c_void_p) for n in ('q', 'k', 'v', 'out')]
                 + [(n + '_stride', _st3) for n in ('q', 'k', 'v', 'out')]
-                + [(n, C.c_void_p) for n in ('sel', 'qlen', 'klen', 'bucket_of', 'q_pos', 'k_pos', 'bias', 'lse', 'out32', 'dout')]
+                + [(n, C.c_void_p) for n in ('sel', 'qlen', 'klen', 'bucket_of', 'q_pos', 'k_pos', 'bias', 'lse', 'lse_rest', 'out32', 'dout')]
                 + [('dout_stride', _st3)] + [(n, C.c_void_p) for n in ('dq', 'dk', 'dv', 'dbias', 'workspace')]
                 + [('workspace_bytes', C.c_size_t)])
 

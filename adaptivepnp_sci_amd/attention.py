@@ -119,7 +119,7 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
     name the positions (None: the key positions), e.g. the frame of each token of a video; differences must fit 32 bits.  A bias below
     -1e30 (-inf, a type's lowest value) masks its keys.  A query without a visible key gives zeros; what a key holds that a query does
     not see -- NaN, infinity -- does not reach it.  Rows behind qlen are zeros, or left as they were in a given `out`.
-    save=True returns (out, saved) for block_attention_backward; bfloat16 probabilities are then multiplied whole, not rounded, so that
+    save=True returns (out, saved) for block_attention_backward, saved = (log-sum-exp (B, Hq, Lq), fp32 result, what the first was rounded by); bfloat16 probabilities are then multiplied whole, not rounded, so that
     the saved fp32 result carries the gradient (out is the same up to its rounding)."""
     return (_bound or _bind()).block_attention(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos, out, save)
 
@@ -129,6 +129,6 @@ def block_attention_backward(dout, q, k, v, sel, saved, block=64, query_block=64
     """(dq, dk, dv, dbias) of block_attention called with the same arguments and save=True; rows behind qlen / klen are zeros, dbias
     (buckets, Hq) float32 is None without a bias.  The selection is not differentiated.  q, k, v and dout of the live rows must be finite:
     here a NaN or an infinity reaches every gradient of its block of 64."""
-    lse, out32 = saved
+    lse, out32, rest = saved
     return (_bound or _bind()).block_attention_backward(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos, dout, lse,
-                                                        out32)
+                                                        out32, rest)

@@ -377,32 +377,33 @@ PyObject* block_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     ENTER(16)
     Attention c(call, o);
     const Tensor* out = given(o[14], "out");
-    Tensor made, lse, out32;
+    Tensor made, lse, rest, out32;
     if (out) call.on_device(*out, "out");
     else made = at::empty_like(c.q), out = &made, c.a.zero_rest = 1;
     tokens(*out, "out", c.q.sizes(), c.q.scalar_type()).to(c.a.out, c.a.out_stride);
     const bool save = truth(o[15]);
     if (save) {
-        lse = at::empty({c.a.B, c.a.Hq, c.a.Lq}, c.q.options().dtype(at::kFloat)), out32 = at::empty(c.q.sizes(), c.q.options().dtype(at::kFloat));
-        c.a.lse = lse.data_ptr<float>(), c.a.out32 = out32.data_ptr<float>();
+        lse = at::empty({c.a.B, c.a.Hq, c.a.Lq}, c.q.options().dtype(at::kFloat)), rest = at::empty_like(lse), out32 = at::empty(c.q.sizes(), c.q.options().dtype(at::kFloat));
+        c.a.lse = lse.data_ptr<float>(), c.a.lse_rest = rest.data_ptr<float>(), c.a.out32 = out32.data_ptr<float>();
     }
     const Tensor ws = c.workspace(0);
     const scipnp_stream_t st = call.stream();
     done(WITHOUT_GIL(attn_fn(&c.a, st)), "scipnp_block_attn");
     PyObject* const r = o[14] == Py_None ? wrap(made) : back(o[14]);
-    return save ? Py_BuildValue("N(NN)", r, wrap(lse), wrap(out32)) : r;
+    return save ? Py_BuildValue("N(NNN)", r, wrap(lse), wrap(out32), wrap(rest)) : r;
     LEAVE
 }
 
-// (the fourteen of Attention, dout, lse, out32)
+// (the fourteen of Attention, dout, lse, out32, lse_rest)
 PyObject* block_attention_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
-    ENTER(17)
+    ENTER(18)
     Attention c(call, o);
     scipnp_block_attn_args& a = c.a;
-    const Tensor &dout = needed(o[14], "dout"), &lse = needed(o[15], "saved[0]"), &out32 = needed(o[16], "saved[1]");
+    const Tensor &dout = needed(o[14], "dout"), &lse = needed(o[15], "saved[0]"), &out32 = needed(o[16], "saved[1]"), &rest = needed(o[17], "saved[2]");
     tokens(dout, "dout", c.q.sizes(), c.q.scalar_type()).to(a.dout, a.dout_stride);
     a.lse = (float*)array(&lse, "saved[0]", {a.B, a.Hq, a.Lq}, at::kFloat), a.out32 = (float*)array(&out32, "saved[1]", c.q.sizes(), at::kFloat);
-    call.on_device(dout, "dout"), call.on_device(lse, "saved[0]"), call.on_device(out32, "saved[1]");
+    a.lse_rest = (float*)array(&rest, "saved[2]", {a.B, a.Hq, a.Lq}, at::kFloat);
+    call.on_device(dout, "dout"), call.on_device(lse, "saved[0]"), call.on_device(out32, "saved[1]"), call.on_device(rest, "saved[2]");
     const Tensor dq = at::empty(c.q.sizes(), c.q.options()), dk = at::empty(c.k.sizes(), c.k.options()), dv = at::empty(c.k.sizes(), c.k.options());
     Tensor dbias;
     a.dq = dq.data_ptr(), a.dk = dk.data_ptr(), a.dv = dv.data_ptr();

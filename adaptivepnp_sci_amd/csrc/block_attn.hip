@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         store_four(out + d, v);
         if constexpr (SAVE) *(f32x4a*)(z.out32 + id * z.D + d) = v;
     });
-    if (z.lse && hi == 0) z.lse[((size_t)b * z.Hq + head) * z.Lq + tok] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (z.lse && hi == 0) store_lse(z, ((size_t)b * z.Hq + head) * z.Lq + tok, m, l);
 #endif
 }
 
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(Attn a) {
         out[d] = (T)v;
         if (a.out32) a.out32[id * a.D + d] = v;
     }
-    if (a.lse && lane == 0) a.lse[((size_t)b * a.Hq + head) * a.Lq + tok] = L == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+    if (a.lse && lane == 0) store_lse(a, ((size_t)b * a.Hq + head) * a.Lq + tok, M, L);
 }
 
 static int row_waves(const scipnp_block_attn_args* a) {
@@ -350,7 +350,7 @@ Attn attn_params(const scipnp_block_attn_args* a) {
     p.sdo = strides_of(a->dout_stride);
     p.sel = a->sel; p.qlen = a->qlen; p.klen = a->klen;
     p.bucket_of = a->bucket_of; p.q_pos = a->num_buckets ? a->q_pos : nullptr; p.k_pos = a->num_buckets ? a->k_pos : nullptr; p.bias = a->bias;
-    p.lse = a->lse; p.out32 = a->out32;
+    p.lse = a->lse; p.lse_rest = a->lse_rest; p.out32 = a->out32;
     p.dq = a->dq; p.dk = a->dk; p.dv = a->dv; p.dbias = a->num_buckets ? a->dbias : nullptr;
     return p;
 }

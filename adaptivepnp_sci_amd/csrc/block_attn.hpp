@@ -345,7 +345,7 @@ struct Attn {
     Strides sq, sk, sv, so, sdo;
     const int32_t *sel, *qlen, *klen, *bucket_of, *q_pos, *k_pos;
     const float* bias;
-    float *lse, *out32;
+    float *lse, *lse_rest, *out32;
     void *dq, *dk, *dv;
     float* dbias;
     float *po, *pml;                                      // forward, splits > 1: partial results, their maxima and sums
@@ -407,6 +407,22 @@ __device__ __forceinline__ int live_tiles(const Attn& a, const int32_t* sel, int
     const int c = live_blocks(a, sel, limit, list, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     return c == 0 ? 0 : (c - 1) * (a.block / KT) + (min(a.block, limit - list[c - 1] * a.block) + KT - 1) / KT;
+}
+
+// ln(sum of 2^score) of a row with maximum m and sum l (units of log 2), as two fp32 numbers: a row whose scores are around 50 would be
+// off by 2^-19 of every weight in the backward pass if it came back as one
+__device__ __forceinline__ void store_lse(const Attn& a, size_t at, float m, float l) {
+    const double v = l == 0.f ? -INFINITY : ((double)m + log2((double)l)) * 0.6931471805599453094;
+    const float h = (float)v;
+    a.lse[at] = h;
+    if (a.lse_rest) a.lse_rest[at] = l == 0.f ? 0.f : (float)(v - (double)h);
+}
+// minus that, in units of log 2 and in two parts again
+struct Shift { float hi, lo; };
+__device__ __forceinline__ Shift load_lse(float lse, float rest) {
+    const double v = ((double)lse + (double)rest) * 1.4426950408889634074;
+    const float h = (float)v;
+    return {-h, (float)((double)h - v)};
 }
 
 // ---- scores of a tile: 32 keys of a lane's row, masked, with the bias

@@ -158,10 +158,11 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     load_frags<T, DP>(live ? (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + head * a.sdo.h : nullptr, a.D, hi, gf);
     const size_t stat = ((size_t)b * a.Hq + head) * a.Lq + tok;
-    float lse = live ? a.lse[stat] * LOG2E : 0.f;
-    if (lse == -INFINITY) {                               // (a row that saw nothing: of its keys, or because the bias masks them)
-        lse = 0.f;
-        lim = -1;
+    Shift shift = {0.f, 0.f};                             // minus the row's log-sum-exp
+    if (live) {
+        const float lse = a.lse[stat];
+        if (lse == -INFINITY) lim = -1;                   // (a row that saw nothing: of its keys, or because the bias masks them)
+        else shift = load_lse(lse, a.lse_rest[stat]);
     }
     // delta of the row, in fp64: each half of a row's lanes has half of it
     double dsum = 0.0;
@@ -244,18 +245,27 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
         ColTile<T, DP> kc;
         kc.read(kt, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
-        float c = a.scale2, add = -lse;
+        // fp32: the large numbers, score and log-sum-exp, meet in one fused operation, and what is small is added behind it; bf16 weights
+        // are rounded to 8 bits anyway: one operation
         if (dist >= 0) {
-            if (a.nbuckets) add += dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
+            const float b = !a.nbuckets ? 0.f : dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
+            if constexpr (sizeof(T) == 4) {
+                const float rest = b + shift.lo;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, shift.hi) + rest);
+            } else {
+                const float add = b + shift.hi;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, add));
+            }
         } else {
             float x[16];
             tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, x[r]);
-            c = 1.f;
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, shift.hi) + (x[r] + shift.lo));
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, add)) * (dp[r] - delta);
+        for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
         if (cur + KT - 1 > min_lim) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : 0.f;
@@ -313,10 +323,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
 // a wave keeps its 32 keys and values in registers (the B operands) and streams rows, which the memory system writes to LDS
 // (global_load ... lds: the rows of a tile may belong to several query groups): S, dP with the rows as A, then dV += dO^T P and
 // dK += Q^T dS with the transposed rows as A and the score registers as B.
-// What a row brings besides: its last visible key, delta, and bias - lse where all 64 keys share its bucket.
+// What a row brings besides: its last visible key, delta, log-sum-exp, and its bias where all 64 keys share its bucket.
 template <typename T, int DP>
 struct DkvCfg {
-    static constexpr int INFO = KT * 20 + 16;             // bias - lse (or - lse), delta, last key, position, head of each row; flags
+    static constexpr int INFO = KT * 24 + 16;             // - lse (bf16: + bias), delta, last key, position, head, (fp32) bias - rest of lse of each row; flags
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES + INFO + KT * 16;   // ... and where the rows of q and dout begin
     static constexpr int MAIN = 4 * TILE;                 // two row tiles, two buffers
     static constexpr int JOIN = 2 * 32 * ((DP + 31) / 32 * 32 + 4) * 4;
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     const T* const qb0 = (const T*)a.q + b * a.sq.b + hk * a.G * a.sq.h;
     const T* const gb0 = (const T*)a.dout + b * a.sdo.b + hk * a.G * a.sdo.h;
     // Each row half's first wave keeps where the rows of the next tile begin, its second what they bring besides (32 lanes each)
-    float iadd = 0.f, idelta = 0.f;
+    float ilse = 0.f, irest = 0.f, idelta = 0.f;
     int ilim = -1, iqp = 0, ig = 0, tok = -1, gl = 0;     // (tok, gl: of the row of the next tile)
     auto tile_at = [&](int it) -> char* { return main + (rs * 2 + (it & 1)) * C::TILE; };
     auto put_rows = [&](int it) {
@@ -418,12 +428,13 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     };
     auto get_info = [&]() {
         ilim = -1;
-        iadd = idelta = 0.f;
+        ilse = irest = idelta = 0.f;
         iqp = 0;
         ig = gl;
         if (tok >= 0) {
             const size_t stat = ((size_t)b * a.Hq + hk * a.G + gl) * a.Lq + tok;
-            iadd = a.lse[stat];
+            ilse = a.lse[stat];
+            irest = a.lse_rest[stat];
             idelta = a.delta[stat];
             ilim = a.causal ? min(sq.shift + tok, sq.klen - 1) : sq.klen - 1;
             iqp = a.q_pos ? a.q_pos[(size_t)b * a.Lq + tok] : sq.shift + tok;
@@ -468,25 +479,27 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             if (kw == 0) {
                 put_rows(it + 1);
             } else {
-                if (iadd == -INFINITY) {                  // (a row that saw nothing)
-                    iadd = 0.f;
+                if (ilse == -INFINITY) {                  // (a row that saw nothing)
+                    ilse = 0.f;
                     ilim = -1;
                 }
-                float add = -iadd * LOG2E;
+                const Shift shift = load_lse(ilse, irest);
+                float own = 0.f;                          // its bias
                 bool one = true;                          // every key has the same bucket for this row
                 if (a.nbuckets && ilim >= 0) {
                     const int lo = clamp_dist(klo - iqp, a.maxd);
                     one = lo == clamp_dist(khi - iqp, a.maxd);
-                    if (one) add += bias.tbl[bias.lut[lo] * a.G + ig];
+                    if (one) own = bias.tbl[bias.lut[lo] * a.G + ig];
                 }
                 const bool all_one = __ballot(!one) == 0, open = __ballot(ilim < k64 + KB - 1) == 0;
-                if (!all_one) add = -iadd * LOG2E;
-                info[lane] = add;
+                if (!all_one) own = 0.f;
+                info[lane] = sizeof(T) == 4 ? shift.hi : shift.hi + own;
+                info[5 * KT + lane] = own + shift.lo;
                 info[KT + lane] = idelta;
                 info[2 * KT + lane] = __int_as_float(ilim);
                 info[3 * KT + lane] = __int_as_float(iqp);
                 info[4 * KT + lane] = __int_as_float(ig);
-                if (lane == 0) info[5 * KT] = __int_as_float((all_one ? 0 : 1) | (open ? 0 : 2));
+                if (lane == 0) info[6 * KT] = __int_as_float((all_one ? 0 : 1) | (open ? 0 : 2));
             }
         }
         dma_wait<4>();
@@ -497,30 +510,40 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             }
             issue(it + 1);
         }
-        const int flags = __builtin_amdgcn_readfirstlane(__float_as_int(info[5 * KT]));
+        const int flags = __builtin_amdgcn_readfirstlane(__float_as_int(info[6 * KT]));
         f32x16a s = dma_rows<T, DP>(at, kf, lane);
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
         ColTile<T, DP> gc, qc;
         gc.read(at + BYTES, lane);
         qc.read(at, lane);
         const float* const mine = info + 4 * hi;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4a add = *(const f32x4a*)(mine + 8 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * q + e] = fmaf(s[4 * q + e], a.scale2, add[e]);
+            if constexpr (sizeof(T) == 4) {               // (the small numbers behind the large ones, as in the pass for dQ)
+                const f32x4a rest = *(const f32x4a*)(mine + 5 * KT + 8 * q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * q + e] += rest[e];
+            }
+        }
         if (flags & 1) {                                  // the bias key by key
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x4a qp = *(const f32x4a*)(mine + 3 * KT + 8 * q), gh = *(const f32x4a*)(mine + 4 * KT + 8 * q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    s[4 * q + e] = fmaf(s[4 * q + e], a.scale2, bias.tbl[bias.lut[clamp_dist(kpos - __float_as_int(qp[e]), a.maxd)] * a.G + __float_as_int(gh[e])]);
+                    s[4 * q + e] += bias.tbl[bias.lut[clamp_dist(kpos - __float_as_int(qp[e]), a.maxd)] * a.G + __float_as_int(gh[e])];
             }
         }
-        const float scale = flags & 1 ? 1.f : a.scale2;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const f32x4a add = *(const f32x4a*)(mine + 8 * q), delta = *(const f32x4a*)(mine + KT + 8 * q);
+            const f32x4a delta = *(const f32x4a*)(mine + KT + 8 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * q + e;
-                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], scale, add[e]));
+                s[r] = __builtin_amdgcn_exp2f(s[r]);
                 dp[r] = s[r] * (dp[r] - delta[e]);
             }
         }
@@ -712,7 +735,7 @@ extern "C" {
 
 int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t s) {
     if (const int rc = attn_check(a)) return rc;
-    SCIPNP_REQUIRE(a->dout && a->dq && a->dk && a->dv && a->lse && a->out32, "backward needs dout, dq, dk, dv, lse and out32");
+    SCIPNP_REQUIRE(a->dout && a->dq && a->dk && a->dv && a->lse && a->lse_rest && a->out32, "backward needs dout, dq, dk, dv, lse, lse_rest and out32");
     SCIPNP_REQUIRE(!a->num_buckets || a->dbias, "backward with a bias needs dbias");
     SCIPNP_ALIGNED(a->dout); SCIPNP_ALIGNED(a->dq); SCIPNP_ALIGNED(a->dk); SCIPNP_ALIGNED(a->dv); SCIPNP_ALIGNED(a->out32);
     SCIPNP_STRIDES(a->dout_stride, a->dtype);

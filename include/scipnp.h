@@ -758,8 +758,9 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s);
 /* softmax(scale * q . k + bias[bucket_of[clamp(kpos - qpos, +-max_distance) + max_distance]][head]) v over the selected blocks.
  * causal: keys behind the query's position are masked.  bias fp32 (num_buckets, Hq) (NULL: none), bucket_of int32
  * (2 * max_distance + 1), q_pos (B, Lq) / k_pos (B, Lk) int32 (NULL: the key positions of query and key).  A row without a key:
- * zeros, lse = -inf.  zero_rest: rows of out behind qlen are set to zero (0: left as they are).  lse fp32 (B, Hq, Lq) and out32 fp32 (B, Lq, Hq, D) (the unrounded result) are written when given; the
- * backward pass reads them.  backward: dq, dk, dv in dtype, dbias fp32; every row is written (zeros behind qlen / klen). */
+ * zeros, lse = -inf.  zero_rest: rows of out behind qlen are set to zero (0: left as they are).  lse
+ * fp32 (B, Hq, Lq), what its rounding left in lse_rest, and out32 fp32 (B, Lq, Hq, D) (the unrounded result) are written when given;
+ * the backward pass reads them.  backward: dq, dk, dv in dtype, dbias fp32; every row is written (zeros behind qlen / klen). */
 typedef struct {
     size_t struct_size;                 /* = sizeof(scipnp_block_attn_args) */
     int dtype, B, Lq, Lk, Hq, Hk, D, block, query_block, n_sel, causal, num_buckets, max_distance, zero_rest;
@@ -769,7 +770,7 @@ typedef struct {
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
     const int32_t *sel, *qlen, *klen, *bucket_of, *q_pos, *k_pos;
     const float* bias;
-    float *lse, *out32;
+    float *lse, *lse_rest, *out32;
     const void* dout;                   /* backward: dout and the gradients; dq (B, Lq, Hq, D), dk / dv (B, Lk, Hk, D) contiguous */
     int64_t dout_stride[3];
     void *dq, *dk, *dv;

@@ -55,7 +55,7 @@ def test_attention_refusals(lib, change, word):
 
 def test_attention_backward_refusals(lib):
     refused(lib, lib.scipnp_block_attn_backward(C.byref(attn()), None), 'backward needs')
-    full = dict(dout=P, dq=P, dk=P, dv=P, lse=P, out32=P)
+    full = dict(dout=P, dq=P, dk=P, dv=P, lse=P, lse_rest=P, out32=P)
     refused(lib, lib.scipnp_block_attn_backward(C.byref(attn(**full, num_buckets=8, bias=P, bucket_of=P, max_distance=9)), None), 'dbias')
     a = attn(**full)
     need = lib.scipnp_block_attn_workspace_bytes(C.byref(a), 1)

@@ -233,7 +233,7 @@ def on_gpu(how):
 def test_block_attention(A, case, dt):
     q, k, v, _, sel, how = problem(case, dt, torch.Generator().manual_seed(case[1] + case[2]))
     want = reference(q, k, v, sel, how)
-    out, (lse, out32) = A.block_attention(cu(q), cu(k), cu(v), cu(sel), save=True, **on_gpu(how))
+    out, (lse, *_) = A.block_attention(cu(q), cu(k), cu(v), cu(sel), save=True, **on_gpu(how))
     qlen = how['qlen']
     live = torch.ones(q.shape[:2], dtype=torch.bool) if qlen is None else torch.arange(q.shape[1])[None] < qlen[:, None]
     within(out, *want['out'], 'out')
