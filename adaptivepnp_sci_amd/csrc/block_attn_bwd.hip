@@ -4,6 +4,10 @@
 // Two passes recompute S and dP (7 products of the pairs instead of 5): one per query group for dQ and dbias, one per key block for dK
 // and dV, which needs the selection the other way round: a bit for every (key block, query group), then the blocks' query rows cut
 // into chunks of equal length, since a first block is chosen by every group and most blocks by few.
+//
+// Four launches: the selection turned round; dQ, dbias, delta and the chunks; dK and dV; the chunks' sums.  2 x 4096 bf16 tokens, 16
+// heads of 64 over 4 key heads, 16 blocks of 64: 5 + 97 + 104 + 9 us behind a forward pass of 74; 65536 fp32 tokens of 48, one head:
+// 5 + 215 + 350 + 17 behind 158.  (One launch more for each of delta, the chunks and dbias: 350 us instead of 311 for the first.)
 #include "block_attn.hpp"
 
 namespace scipnp {
@@ -22,7 +26,8 @@ __device__ __forceinline__ unsigned fast_div(unsigned x, unsigned d, unsigned m,
 static inline unsigned div_magic(int d) { return d <= 1 ? 0xFFFFFFFFu : (unsigned)((1ull << 32) / (unsigned)d); }
 
 // ---- the selection the other way round: a workgroup gathers 32 query groups, a bit each in a word for every key block.  No word is
-// written twice, so nothing has to be cleared before; and the zeros that rows that do not exist are read from
+// written twice, so nothing has to be cleared before; and the zeros that rows that do not exist are read from.  Latency: 5 us, whether
+// 1024 groups choose among 64 blocks or among 1024 (atomics on words in memory: 15 us where every group chooses one block)
 constexpr int MARK_WAVES = 16, MARK_CAP = 16384;          // (key blocks in LDS at a time)
 __global__ void __launch_bounds__(64 * MARK_WAVES) attn_mark_kernel(Attn a, int cap) {
     extern __shared__ unsigned bits[];
@@ -97,7 +102,8 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
 }
 
 // ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
-// most tiles lie) in registers
+// most tiles lie) in registers.  Three products a tile and vector work of the same length: 97 us for 131072 bf16 rows of 64 with
+// about 1000 keys each, 215 us (fp32 matrix rate 60 TFLOP/s, a third of the third product padding) for 65536 x 1024 of 48 wide fp32
 template <typename T, int DP>
 struct DqCfg {
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
@@ -240,8 +246,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
             issue(key0, buf ^ 1);
         }
         const char* const kt = smem + buf * C::TILE;
+        __builtin_amdgcn_s_setprio(1);
         f32x16a s = dma_rows<T, DP>(kt, qf, lane);
         const f32x16a dp = dma_rows<T, DP>(kt + DmaTile<T, DP>::BYTES, gf, lane);
+        __builtin_amdgcn_s_setprio(0);
         ColTile<T, DP> kc;
         kc.read(kt, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
@@ -287,7 +295,9 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
                         for (int r = 0; r < 16; ++r) mine[d[r] * HROW] += s[r];
             }
         }
+        __builtin_amdgcn_s_setprio(1);
         kc.template mma<2>(s, o);                         // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
+        __builtin_amdgcn_s_setprio(0);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     if (a.dbias) {                                        // the set's sums: a (bucket, head) adds its lanes in order, in fp64
@@ -323,6 +333,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
 // a wave keeps its 32 keys and values in registers (the B operands) and streams rows, which the memory system writes to LDS
 // (global_load ... lds: the rows of a tile may belong to several query groups): S, dP with the rows as A, then dV += dO^T P and
 // dK += Q^T dS with the transposed rows as A and the score registers as B.
+// Bound by the vector work between the products: four products of 32 x 32 take 512 cycles a tile at bf16, 64 wide, the rest about
+// 900, of which the rows' books are a fifth (they were half while every lane divided for its own requests: 447 instead of 350 us in
+// fp32).  Chunks of a 2048th of all rows: larger ones leave CUs idle at the end (117 us instead of 104 at a 1024th), smaller ones pay
+// for their beginnings (110 at a 4096th).
 // What a row brings besides: its last visible key, delta, log-sum-exp, and its bias where all 64 keys share its bucket.
 template <typename T, int DP>
 struct DkvCfg {
@@ -511,8 +525,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             issue(it + 1);
         }
         const int flags = __builtin_amdgcn_readfirstlane(__float_as_int(info[6 * KT]));
+        __builtin_amdgcn_s_setprio(1);
         f32x16a s = dma_rows<T, DP>(at, kf, lane);
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
+        __builtin_amdgcn_s_setprio(0);
         ColTile<T, DP> gc, qc;
         gc.read(at + BYTES, lane);
         qc.read(at, lane);
@@ -559,8 +575,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
                 }
             }
         }
+        __builtin_amdgcn_s_setprio(1);
         gc.mma(s, dv);
         qc.mma(dp, dk);
+        __builtin_amdgcn_s_setprio(0);
     }
     // the two row halves: 1 into LDS, 0 adds
     float* const obuf = (float*)main + kw * 32 * (NB * 32 + 4);
