@@ -23,6 +23,7 @@ F32 = torch.float32
 VALUES, DIMS, BLOCK, TILE = 48, 56, 64, 32
 LIFT = 0.5 * VALUES ** 0.5               # the constant entry: as long as a patch of middle brightness
 MIN_SIGMA = 1e-3
+MAX_BLOCKS = 8192                        # of a selection
 _EPS = 1e-6
 
 
@@ -54,14 +55,16 @@ class NonLocalEngine:
         if B % units:
             raise ValueError(f'{B} frames do not split into {units} units')
         self.B, self.H, self.W, self.units, self.device = B, H, W, units, device
-        self.n_sel, self.shifts = model.n_sel, model.shifts
+        self.shifts = model.shifts
         more = 2 if self.shifts > 1 else 0
         tiles = -(-(H + more) // TILE) * -(-(W + more) // TILE)
         T, self.L = B // units, B // units * tiles * BLOCK
+        many = -(-T * tiles // MAX_BLOCKS)      # (a clip of more tiles, e.g. 1024 x 1024 x 16: blocks of several tiles, fewer of them)
+        self.block, self.n_sel = BLOCK * many, max(1, model.n_sel // many)
         seqs = units * self.shifts
         self.tokens = torch.empty(seqs, self.L, 1, DIMS, dtype=F32, device=device)
         self.q, self.k, self.o = (torch.empty_like(self.tokens) for _ in range(3))
-        self.summary = torch.empty(seqs, self.L // BLOCK, 1, DIMS, dtype=F32, device=device)
+        self.summary = torch.empty(seqs, -(-self.L // self.block), 1, DIMS, dtype=F32, device=device)
         self.frame = torch.arange(T, dtype=torch.int32, device=device).repeat_interleave(tiles * BLOCK).expand(seqs, -1).contiguous()
         self.bucket_of = A.bucket_table(model.num_buckets, model.max_distance, device=device)
         self.flat = torch.empty(2 * DIMS + model.num_buckets, dtype=F32, device=device)
@@ -76,7 +79,7 @@ class NonLocalEngine:
     def _clip(self, u, sigma, sel):
         s = slice(u * self.shifts, (u + 1) * self.shifts)
         return ((self.q[s], self.k[s], self.tokens[s], sel[s]),
-                dict(block=BLOCK, query_block=BLOCK, scale=1.0 / (DIMS * max(float(sigma), MIN_SIGMA) ** 2), bucket_of=self.bucket_of, bias=self.bias,
+                dict(block=self.block, query_block=BLOCK, scale=1.0 / (DIMS * max(float(sigma), MIN_SIGMA) ** 2), bucket_of=self.bucket_of, bias=self.bias,
                      q_pos=self.frame[s], k_pos=self.frame[s]), self.o[s])
 
     def forward(self, frames, sigma, save=False):
@@ -84,8 +87,8 @@ class NonLocalEngine:
         the backward pass needs (a single clip)"""
         ops.patch_tokens(frames, self.tokens, self.units, self.shifts, LIFT)
         A.head_norm_rotate(self.tokens, self.tokens, self.wq, self.wk, eps=_EPS, out_q=self.q, out_k=self.k)
-        A.block_summary(self.k, BLOCK, out=self.summary)
-        sel = A.select_blocks(self.q, self.summary, self.n_sel, BLOCK, BLOCK, sink=0, local=1)
+        A.block_summary(self.k, self.block, out=self.summary)
+        sel = A.select_blocks(self.q, self.summary, self.n_sel, self.block, BLOCK, keys=self.L, sink=0, local=1)
         kept = None
         for u in range(self.units):      # (a clip a call: how its work is split, and so its bits, does not depend on the other clips)
             tensors, how, o = self._clip(u, sigma, sel)

@@ -82,8 +82,10 @@ def prior(N, **kw):
 
 
 @pytest.mark.parametrize('B,H,W,shifts,n_sel', [(2, 40, 36, 2, 3), (3, 32, 64, 1, 5), (1, 20, 20, 4, 2)])
-def test_a_pass_operator_by_operator(N, B, H, W, shifts, n_sel):
-    """every operator's result, given what the one before it left"""
+@pytest.mark.parametrize('limit', [8192, 3])
+def test_a_pass_operator_by_operator(N, B, H, W, shifts, n_sel, limit, monkeypatch):
+    """every operator's result, given what the one before it left; limit: the blocks of a selection, past which they get larger"""
+    monkeypatch.setattr(N, 'MAX_BLOCKS', limit)
     m = prior(N, n_sel=n_sel, shifts=shifts)
     eng = N.NonLocalEngine(m, B, H, W, torch.device('cuda'))
     x, sigma = clip(B, H, W), 0.2
@@ -93,12 +95,15 @@ def test_a_pass_operator_by_operator(N, B, H, W, shifts, n_sel):
     for got, w in ((q, m.wq), (k, m.wk)):
         val = O.norm_rotate(tok, w.detach(), None, None)
         within(got, val, O.U32 * 1.01 * val.abs() + 2.0 ** -29 * val.abs().amax(-1, keepdim=True), 'norm')
-    want = O.summary(k, 64, None)
+    many = -(-tok.shape[1] // 64 // limit)
+    block, n_sel = 64 * many, max(1, n_sel // many)
+    assert how['block'] == block and sel.shape[-1] == n_sel
+    want = O.summary(k, block, None)
     within(eng.summary, want, O.U32 * want.abs() + 1e-15, 'summary')
     L = tok.shape[1]
-    assert torch.equal(sel, O.select(q, eng.summary.cpu(), n_sel, 64, 64, L, False, None, None, 0, 1))
+    assert torch.equal(sel, O.select(q, eng.summary.cpu(), n_sel, block, 64, L, False, None, None, 0, 1))
     h = {n: t.cpu() if isinstance(t, torch.Tensor) else t for n, t in how.items()}
-    ref = O.attention(q, k, tok, sel, 64, 64, h['scale'], False, None, None, h['bucket_of'], h['bias'], h['q_pos'], h['k_pos'])
+    ref = O.attention(q, k, tok, sel, block, 64, h['scale'], False, None, None, h['bucket_of'], h['bias'], h['q_pos'], h['k_pos'])
     within(eng.o, *ref['out'], 'attention')
     # the mean over the grids of values with those errors, plus its own roundings
     val, err = (torch.zeros(B, 3, H, W, dtype=torch.float64) for _ in range(2))
@@ -231,3 +236,17 @@ def test_entry_points_and_plug_in(N):
     assert torch.equal(cube.permute(3, 2, 0, 1), m(x, 0.1))
     with pytest.raises(ValueError, match='NonLocalPrior'):
         P.twoStageAdmm_denoise_bayer(y, Phi, denoiser='nonlocal_color', iter_max=[1], sigma=[0.1], model_denoise=torch.nn.Linear(2, 2))
+
+
+def test_a_large_cube(N):
+    """1024 x 1024 x 16: more tiles than a selection takes; a constant clip with one odd tile stays a constant clip elsewhere"""
+    x = torch.full((16, 3, 1024, 1024), 0.25, device='cuda')
+    x[3, :, 256:288, 320:352] = 0.75
+    m = N.NonLocalPrior(n_sel=6)
+    got = m(x, 0.02)
+    assert torch.isfinite(got).all()
+    # a weight across the two kinds is below exp(-|x - x'|^2 / (48 s^2) (about)): their cosine is 0.96, the scale 2500, nothing is left of it;
+    # the rest is the sum over 384 equal values and its quotient
+    far = torch.ones(1024, 1024, dtype=torch.bool, device='cuda')
+    far[224:320, 288:384] = False
+    assert (got[:, :, far] - 0.25).abs().max() <= 0.25 * 2.0 ** -24 * (4 * 64 * 6 + 8)
