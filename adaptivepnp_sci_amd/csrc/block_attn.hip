@@ -333,7 +333,7 @@ int attn_check(const scipnp_block_attn_args* a) {
     SCIPNP_REQUIRE(a->B > 0 && a->Lq > 0 && a->Lk > 0 && a->Hk > 0 && a->Hq > 0, "B, Lq, Lk, Hq, Hk must be positive");
     SCIPNP_REQUIRE(a->Hq % a->Hk == 0, "%d query heads are no multiple of %d key heads", a->Hq, a->Hk);
     SCIPNP_REQUIRE(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "head size %d: a multiple of 8 up to 128", a->D);
-    SCIPNP_REQUIRE(a->block > 0 && a->block <= 65536 && a->block % 64 == 0, "block %d: a multiple of 64", a->block);
+    SCIPNP_REQUIRE(a->block > 0 && a->block <= 65536 && a->block % 64 == 0, "block %d: a multiple of 64 up to 65536", a->block);
     SCIPNP_REQUIRE(a->query_block > 0 && a->query_block <= 1024, "query_block %d: 1 to 1024", a->query_block);
     SCIPNP_REQUIRE(a->n_sel > 0 && a->n_sel <= 1024, "n_sel %d: 1 to 1024", a->n_sel);
     SCIPNP_REQUIRE(a->Lk <= (1 << 30) && a->Lq <= (1 << 30), "sequences of at most 2^30 tokens");

@@ -360,15 +360,13 @@ struct Attn {
     double* pbias;
 };
 // the kernel's first argument, read once more from memory where this is called: nothing of it is held in registers until then
-__device__ __forceinline__ const Attn& late_args() {
 #if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ const Attn& late_args() {
     auto p = (const __attribute__((address_space(4))) Attn*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(p));
     return *(const Attn*)p;
-#else
-    return *(const Attn*)nullptr;
-#endif
 }
+#endif
 
 struct Seq { int qlen, klen, shift; };                    // shift: key position of query 0
 __device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
