@@ -6,7 +6,7 @@
 // that follows, and the keys of a cache must not depend on which call wrote them.  The kernel reads and writes each element once and
 // costs about 8 fp64 operations per element against 4 bytes of traffic in bf16: 16384 tokens of 40 bf16 heads of 128 take 76 us, 4.4
 // TB/s (a copy reaches 5.2); their arithmetic alone would take 38.  In fp32, 131072 tokens of 8 heads of 48: 89 us forward (4.5 TB/s),
-// 167 backward (3.6 TB/s) and 9 for the sum of dw over the workgroups.  One token of 16 sequences: 5.7 us, latency.  (Rows asked for while the one
+// 139 backward (4.3 TB/s) and 6 for the sum of dw over the workgroups.  One token of 16 sequences: 5.7 us, latency.  (Rows asked for while the one
 // before is computed: 121 instead of 99 us, fewer waves fit.)
 //
 // A row (one head of one token) is held by LPR = 2^k >= D / 8 lanes; a lane has two chunks of four elements, both halves of its
@@ -310,7 +310,9 @@ static int head_norm_lpr(int D) { int l = 1; while (l * 8 < D) l <<= 1; return l
 static int head_norm_bwd_groups(const scipnp_head_norm_args* a) {
     const int tt = head_norm_tokens(a, head_norm_lpr(a->D));
     const long long tiles = ((long long)a->B * a->L + tt - 1) / tt;
-    return (int)(tiles < 1024 ? tiles : 1024);            // four workgroups per CU, each with its share of dw
+    // three workgroups a CU, as many as its registers hold (four: a second round a third full, 164 + 7 instead of 139 + 6 us), each with its
+    // share of dw
+    return (int)(tiles < 768 ? tiles : 768);
 }
 
 static HeadNorm head_norm_params(const scipnp_head_norm_args* a) {
