@@ -110,11 +110,8 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
     };
     const int far = 2 * a.maxd;                           // the two ends, where most tiles lie: their bias in registers
     const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
-    f32x16a o[NB];
-#pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    Acc<T, DP> sums;
+    sums.zero();
     float m = -INFINITY, l = 0.f;
     bool spoilt = false;
 
@@ -174,10 +171,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
             const float mn = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             m = mn;
             l *= alpha;
-#pragma unroll
-            for (int db = 0; db < NB; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+            sums.scale(alpha);
         }
         const float shift = add - (m == -INFINITY ? 0.f : m);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -193,11 +187,13 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
             if (skip) continue;
         }
         __builtin_amdgcn_s_setprio(1);
-        vt.template mma<SAVE ? 3 : 1>(s, o);
+        vt.template mma<SAVE ? 3 : 1>(s, sums);
         __builtin_amdgcn_s_setprio(0);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
     l += __shfl_xor(l, 32, 64);
+    f32x16a o[NB];
+    sums.blocks(o);
     const Attn& z = late_args();                          // (what only the end needs is read again there: the loop's scalars fit the registers)
     // Tiles with masked keys and values that are not numbers: only rows that see a key take its value, by plain loads
     if (spoilt) {
@@ -221,7 +217,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
                     x += bias.tbl[bias.lut[clamp_dist(kp - qp, z.maxd)] * z.G + gl];
                 }
                 const float p = __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
-                each_four<T, NB>(hi, [&](int d, auto at) {
+                each_four<T, DP>(hi, [&](int d, auto at) {
                     if (d >= z.D) return;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[at(e) >> 4][at(e) & 15] = fmaf(p, (float)vr[d + e], o[at(e) >> 4][at(e) & 15]);
@@ -242,14 +238,14 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         const size_t rows = (size_t)z.B * z.Lq * z.Hq;
         if (hi == 0) *(float2*)(z.pml + 2 * (part * rows + id)) = make_float2(m, l);
         float* const po = z.po + (part * rows + id) * z.D;
-        each_four<T, NB>(hi, [&](int d, auto at) {
+        each_four<T, DP>(hi, [&](int d, auto at) {
             if (d < z.D) *(f32x4a*)(po + d) = f32x4a{o[at(0) >> 4][at(0) & 15], o[at(1) >> 4][at(1) & 15], o[at(2) >> 4][at(2) & 15], o[at(3) >> 4][at(3) & 15]};
         });
         return;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);             // (a NaN sum stays one)
     T* const out = (T*)z.out + b * z.so.b + (long long)tok * z.so.t + head * z.so.h;
-    each_four<T, NB>(hi, [&](int d, auto at) {
+    each_four<T, DP>(hi, [&](int d, auto at) {
         if (d >= z.D) return;
         f32x4a v;
 #pragma unroll

@@ -128,7 +128,76 @@ __device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat
 //   takes the builtin for a reader of every request in flight and waits for the NEXT tile in front of it; the block waits for its reads.
 //   Column 32 db + m is row m of block db.  PARTS: the bf16 numbers that P is split into, a product each; 3 hold its 24 bits, 2 hold 16.
 // fp32: with 2 or 4 blocks a lane reads 2 or 4 neighbouring columns at once: column NB m + db is row m of block db.
+//   With 16 columns left over (48 wide) the blocks are 16 wide and nothing is multiplied with padding: two swaps of 16 lanes bring four
+//   keys of 16 rows beside each other, which is the operand of v_mfma_f32_16x16x4_f32.
 typedef unsigned u32x2a __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void swap16(float& x, float& y) {        // lanes 16-31 and 48-63 of x with lanes 0-15 and 32-47 of y
+#if defined(__HIP_DEVICE_COMPILE__)
+    const u32x2a z = __builtin_bit_cast(u32x2a, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false));
+    x = __uint_as_float(z[0]);
+    y = __uint_as_float(z[1]);
+#endif
+}
+__device__ __forceinline__ void swap32(float& x, float& y) {        // lanes 32-63 of x with lanes 0-31 of y
+#if defined(__HIP_DEVICE_COMPILE__)
+    const u32x2a z = __builtin_bit_cast(u32x2a, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false));
+    x = __uint_as_float(z[0]);
+    y = __uint_as_float(z[1]);
+#endif
+}
+// sums of second products; blocks() gives them as column blocks of 32
+template <typename T, int DP>
+struct Acc {
+    static constexpr int NB = (DP + 31) / 32;
+    static constexpr bool N16 = sizeof(T) == 4 && DP % 32 == 16;    // [16 columns][rows 0-15, 16-31]: row lane & 15, columns 4 (lane >> 4) + i
+    f32x16a x[N16 ? 1 : NB];
+    f32x4a y[N16 ? DP / 16 : 1][2];
+    __device__ __forceinline__ void zero() {
+        if constexpr (N16)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) y[c][0] = y[c][1] = f32x4a{0.f, 0.f, 0.f, 0.f};
+        else
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[db][r] = 0.f;
+    }
+    __device__ __forceinline__ void scale(float f) {      // f: of row lane & 31
+        if constexpr (N16) {
+            float f0 = f, f1 = f;
+            swap16(f0, f1);
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { y[c][0][i] *= f0; y[c][1][i] *= f1; }
+        } else {
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[db][r] *= f;
+        }
+    }
+    __device__ __forceinline__ void blocks(f32x16a (&o)[NB]) const {
+#pragma unroll
+        for (int db = 0; db < NB; ++db) {
+            if constexpr (!N16) o[db] = x[db];
+            else
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+        }
+        if constexpr (N16)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float u = y[c][0][i], v = y[c][1][i];
+                    swap16(u, v);
+                    swap32(u, v);
+                    o[c / 2][8 * (c & 1) + i] = u;
+                    o[c / 2][8 * (c & 1) + 4 + i] = v;
+                }
+    }
+};
 template <typename T, int DP>
 struct ColTile {
     static constexpr int LC = DmaTile<T, DP>::LC, NB = (DP + 31) / 32;
@@ -250,7 +319,8 @@ struct ColTile {
         }
     }
     template <int PARTS = 1>
-    __device__ __forceinline__ void mma(const f32x16a& p, f32x16a (&acc)[NB]) const {
+    __device__ __forceinline__ void mma(const f32x16a& p, Acc<T, DP>& sums) const {
+        auto& acc = sums.x;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -273,6 +343,29 @@ struct ColTile {
                 if constexpr (PARTS > 2)
 #pragma unroll
                     for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[db], 0, 0, 0);
+            }
+        } else if constexpr (Acc<T, DP>::N16) {            // keys 8 apart share a product: its four rows lie in banks of their own
+            constexpr int NC = DP / 16;
+            const int l = lane & 15, j = lane >> 4, first = 8 * (j & 1) + 4 * (j >> 1);
+            const char* const base = tile + first * LC * 16 + 4 * (l & 3);
+            float x[2][NC];
+            auto fetch = [&](int i, float (&y)[NC]) {
+                const int row = 16 * (i >> 2) + (i & 3), f = swz<T, LC>(first + row);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) y[c] = *(const float*)(base + row * LC * 16 + ((((l >> 2) + 4 * c) ^ f) << 4));
+            };
+            fetch(0, x[0]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i < 7) fetch(i + 1, x[(i + 1) & 1]);
+                float p0 = p[8 * (i >> 2) + (i & 3)], p1 = p[8 * (i >> 2) + (i & 3) + 4];
+                swap16(p0, p1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    sums.y[c][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i & 1][c], p0, sums.y[c][0], 0, 0, 0);
+                    sums.y[c][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i & 1][c], p1, sums.y[c][1], 0, 0, 0);
+                }
             }
         } else {
             constexpr int W = NB == 3 ? 1 : NB;            // floats of a read
@@ -308,12 +401,13 @@ struct ColTile {
     }
 };
 // the accumulators of a lane's row, four neighbouring columns at a time: f(column, values, block and register of each)
-template <typename T, int NB, typename F>
+template <typename T, int DP, typename F>
 __device__ __forceinline__ void each_four(int hi, F f) {
+    constexpr int NB = Acc<T, DP>::NB;
     if constexpr (sizeof(T) == 4 && NB == 4) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) f(4 * (8 * (r >> 2) + 4 * hi + (r & 3)), [=](int e) { return e * 16 + r; });
-    } else if constexpr (sizeof(T) == 4 && NB == 2) {
+    } else if constexpr (sizeof(T) == 4 && NB == 2 && !Acc<T, DP>::N16) {
 #pragma unroll
         for (int r = 0; r < 16; r += 2) f(2 * (8 * (r >> 2) + 4 * hi + (r & 3)), [=](int e) { return (e & 1) * 16 + r + (e >> 1); });
     } else {

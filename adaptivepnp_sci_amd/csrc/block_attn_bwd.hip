@@ -225,11 +225,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
         v += __shfl_xor(v, 32, 64);
         if (hi == 0) mine[n * HROW] += v;
     };
-    f32x16a o[NB];
-#pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    Acc<T, DP> sums;
+    sums.zero();
 
     int key0 = 0;
     if (count > 0) {
@@ -296,10 +293,12 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
             }
         }
         __builtin_amdgcn_s_setprio(1);
-        kc.template mma<2>(s, o);                         // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
+        kc.template mma<2>(s, sums);                      // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
         __builtin_amdgcn_s_setprio(0);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
+    f32x16a o[NB];
+    sums.blocks(o);
     if (a.dbias) {                                        // the set's sums: a (bucket, head) adds its lanes in order, in fp64
         add_bucket(bias.lut[0], sum_lo);
         add_bucket(bias.lut[far], sum_hi);
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Att
     }
     if (!there_is || row >= R || tok >= a.Lq) return;
     T* const dst = (T*)a.dq + (((size_t)b * a.Lq + tok) * a.Hq + head) * a.D;
-    each_four<T, NB>(hi, [&](int d, auto at) {
+    each_four<T, DP>(hi, [&](int d, auto at) {
         if (d >= a.D) return;
         f32x4a v;
 #pragma unroll
@@ -413,11 +412,9 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
         khi = wave_max(k64 + lane < sq.klen ? mine : INT_MIN);
     }
 
-    f32x16a dk[NB], dv[NB];
-#pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { dk[db][r] = 0.f; dv[db][r] = 0.f; }
+    Acc<T, DP> kacc, vacc;
+    kacc.zero();
+    vacc.zero();
 
     // row x of the chunk -> token and head; tokens behind qlen: -1
     auto row_of = [&](unsigned x, int& tok, int& gl) {
@@ -576,10 +573,13 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             }
         }
         __builtin_amdgcn_s_setprio(1);
-        gc.mma(s, dv);
-        qc.mma(dp, dk);
+        gc.mma(s, vacc);
+        qc.mma(dp, kacc);
         __builtin_amdgcn_s_setprio(0);
     }
+    f32x16a dk[NB], dv[NB];
+    kacc.blocks(dk);
+    vacc.blocks(dv);
     // the two row halves: 1 into LDS, 0 adds
     float* const obuf = (float*)main + kw * 32 * (NB * 32 + 4);
     auto join = [&](f32x16a (&x)[NB]) {
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     if (rs == 1) return;
     const size_t slot = ((size_t)bh * a.max_chunks + c) * subs + sub;
     auto put = [&](const f32x16a (&x)[NB], int which, T* dst, float scale) {
-        each_four<T, NB>(hi, [&](int d, auto at) {
+        each_four<T, DP>(hi, [&](int d, auto at) {
             if (d >= a.D) return;
             f32x4a v;
 #pragma unroll
