@@ -39,17 +39,18 @@ __device__ __forceinline__ void load_frags(const T* row, int D, int hi, typename
 
 // ---- a tile that the memory system writes into LDS itself (buffer_load ... lds: no registers, no address arithmetic per tile)
 //
-// 32 rows of LC = 2^n >= DP * sizeof(T) / 16 chunks of 16 bytes, packed (a wave's request writes 1 KB in lane order); chunk c of row r
+// 32 rows of LC >= DP * sizeof(T) / 16 chunks of 16 bytes, LC a power of two or 12, packed (a wave's request writes 1 KB in lane order); chunk c of row r
 // lies at chunk c ^ swz(r), so that both ways of reading meet every bank once: 16 rows at one chunk (the A operand of a score product),
 // and, transposed, 4 rows x 4 chunks (bf16) or two rows 4 apart x 8 chunks (fp32).  Rows past the live ones and columns past D
 // come back as zeros (requests outside the buffer descriptor), whatever lies behind them in memory.
 template <typename T, int DP> constexpr int lds_chunks() {
     const int n = DP * (int)sizeof(T) / 16;
-    return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32;
+    return n <= 4 ? 4 : n <= 8 ? 8 : sizeof(T) == 4 && n == 12 ? 12 : n <= 16 ? 16 : 32;
 }
 template <typename T, int LC>
 __device__ __forceinline__ int swz(int row) {
-    if constexpr (sizeof(T) == 4) return LC >= 16 ? ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3) : (row >> 1) & 7;
+    if constexpr (LC == 12) return (row >> 2) & 3;        // (rows begin 48 banks apart: four of them meet every 16th)
+    else if constexpr (sizeof(T) == 4) return LC >= 16 ? ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3) : (row >> 1) & 7;
     else return LC >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : LC == 8 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
 }
 template <typename T, int DP>
@@ -344,13 +345,13 @@ struct ColTile {
 #pragma unroll
                     for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[db], 0, 0, 0);
             }
-        } else if constexpr (Acc<T, DP>::N16) {            // keys 8 apart share a product: its four rows lie in banks of their own
+        } else if constexpr (Acc<T, DP>::N16) {
             constexpr int NC = DP / 16;
-            const int l = lane & 15, j = lane >> 4, first = 8 * (j & 1) + 4 * (j >> 1);
+            const int l = lane & 15, j = lane >> 4, first = (j & 1) + 4 * (j >> 1);
             const char* const base = tile + first * LC * 16 + 4 * (l & 3);
             float x[2][NC];
             auto fetch = [&](int i, float (&y)[NC]) {
-                const int row = 16 * (i >> 2) + (i & 3), f = swz<T, LC>(first + row);
+                const int row = 8 * (i >> 1) + 2 * (i & 1), f = swz<T, LC>(first + row);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) y[c] = *(const float*)(base + row * LC * 16 + ((((l >> 2) + 4 * c) ^ f) << 4));
             };
@@ -358,7 +359,7 @@ struct ColTile {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (i < 7) fetch(i + 1, x[(i + 1) & 1]);
-                float p0 = p[8 * (i >> 2) + (i & 3)], p1 = p[8 * (i >> 2) + (i & 3) + 4];
+                float p0 = p[2 * i], p1 = p[2 * i + 1];
                 swap16(p0, p1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

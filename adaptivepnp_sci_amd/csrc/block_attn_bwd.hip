@@ -464,7 +464,8 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
         for (int i = 0; i < MINE; ++i) {
             const int piece = kw + 2 * i;
             if (PIECES % 2 == 0 || piece < PIECES) {
-                const long long oq = off[piece * 64 / LC + lane / LC], og = off[KT + piece * 64 / LC + lane / LC];
+                const int at = (piece * 64 + lane) / LC;
+                const long long oq = off[at], og = off[KT + at];
                 const bool ok = oq >= 0 && chunk_at[i] >= 0;
                 const T* const qa = ok ? qb0 + oq + chunk_at[i] : (const T*)a.zeros;
                 const T* const ga = ok ? gb0 + og + chunk_at[i] : (const T*)a.zeros;
