@@ -449,7 +449,7 @@ struct Attn {
     float* zeros;                                         // 256 bytes
     unsigned* member;                                     // [b, hk][32 groups][nb4 key blocks], a bit a group
     int words, nb4;
-    const int* chunk_start;                               // [b, hk][key block + 1]
+    int *chunk_start, *chunk_rows;                        // [b, hk][key block + 1], [b, hk][key block]
     int max_chunks;
     float* pkv;                                           // partial dk, dv
     double* pbias;

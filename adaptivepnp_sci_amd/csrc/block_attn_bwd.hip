@@ -57,11 +57,13 @@ __global__ void __launch_bounds__(64 * MARK_WAVES) attn_mark_kernel(Attn a, int 
     }
 }
 
-// ---- chunks of every key block of one (sequence, key head), by one workgroup: chunk_start[j] = chunks of the blocks before j
+// ---- chunks of every key block of one (sequence, key head), by one workgroup: chunk_start[j] = chunks of the blocks before j; a block's
+// chunks are of one length, chunk_rows[j] <= CH (a multiple of 64; the last may be shorter)
 __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH, int* lds) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
     int* const wsum = lds;
-    int* const cs = (int*)a.chunk_start + (size_t)bh * (a.nb + 1);
+    int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
+    int* const cr = a.chunk_rows + (size_t)bh * a.nb;
     int carry = 0;
     for (int base = 0; base < a.nb; base += 4 * blockDim.x) {     // four neighbouring blocks a thread
         const int j = base + 4 * tid;
@@ -77,7 +79,9 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
         int sum = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int c = j + e < a.nb ? (int)(((long long)n[e] * R + CH - 1) / CH) : 0;
+            const long long rows = (long long)n[e] * R;
+            const int c = j + e < a.nb ? (int)((rows + CH - 1) / CH) : 0;
+            if (c > 0) cr[j + e] = (int)(((rows + c - 1) / c + 63) / 64 * 64);
             n[e] = sum;
             sum += c;
         }
@@ -348,7 +352,7 @@ struct DkvCfg {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(Attn a, int CH, int subs, unsigned magic_r, unsigned magic_g) {
+__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(Attn a, int subs, unsigned magic_r, unsigned magic_g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DkvCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
@@ -372,11 +376,11 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
     const int R = a.qb * a.G;
     const Seq sq = seq_of(a, b);
     // the chunk's rows are x0 .. x1 of the block's groups laid end to end; their groups into the list
-    const unsigned x0 = (unsigned)(c - cs[j]) * CH;
+    const unsigned len = (unsigned)a.chunk_rows[(size_t)bh * a.nb + j], x0 = (unsigned)(c - cs[j]) * len;
     int count = 0;
     {
         const unsigned* w = a.member + (size_t)bh * a.words * a.nb4 + j;
-        const int e0 = (int)(x0 / R), e1 = (int)((x0 + CH + R - 1) / R);
+        const int e0 = (int)(x0 / R), e1 = (int)((x0 + len + R - 1) / R);
         for (int base = 0; base < a.words; base += 256) {
             const unsigned bits = base + tid < a.words ? w[(size_t)(base + tid) * a.nb4] : 0;
             const int n = __popc(bits);
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
         }
         __syncthreads();
     }
-    const unsigned x1 = (unsigned)min((long long)x0 + CH, (long long)count * R);
+    const unsigned x1 = (unsigned)min((long long)x0 + len, (long long)count * R);
     const int e0 = (int)(x0 / R);
 
     const int k64 = j * a.block + sub * KB, kbase = k64 + kw * 32, key = kbase + li;
@@ -693,7 +697,7 @@ static BwdPlan bwd_plan(const scipnp_block_attn_args* a) {
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     size_t at = up((size_t)a->B * a->Hq * a->Lq * 4) + 256;                  // delta, zeros
     p.o_member = at; at += up(bh * ((p.nb + 3) / 4 * 4) * p.words * 4);
-    p.o_chunk = at; at += up(bh * (p.nb + 1) * 4);
+    p.o_chunk = at; at += up(bh * (2 * p.nb + 1) * 4);
     p.o_pkv = at; at += up(bh * p.max_chunks * p.subs * 2 * KB * a->D * 4);
     p.o_pbias = at; at += a->num_buckets ? up(bh * p.ng * p.chunks * a->num_buckets * (a->Hq / a->Hk) * 8) : 0;
     p.total = at;
@@ -726,7 +730,7 @@ static int bwd_launch(const Attn& p, const BwdPlan& bp, hipStream_t st) {
     static LdsAttrOnce once;
     if (const int rc2 = once.ensure((const void*)block_attn_dkv_kernel<T, DP>, 163840, "block_attn_dkv")) return rc2;
     const unsigned gk = (unsigned)((long long)p.B * p.Hk * p.max_chunks * bp.subs);
-    block_attn_dkv_kernel<T, DP><<<gk, 256, lds, st>>>(p, bp.CH, bp.subs, div_magic(bp.R), div_magic(p.G));
+    block_attn_dkv_kernel<T, DP><<<gk, 256, lds, st>>>(p, bp.subs, div_magic(bp.R), div_magic(p.G));
     return SCIPNP_OK;
 }
 
@@ -771,6 +775,7 @@ int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t 
     p.words = bp.words;
     p.nb4 = (p.nb + 3) / 4 * 4;
     p.chunk_start = (int*)(w + bp.o_chunk);
+    p.chunk_rows = p.chunk_start + (size_t)a->B * a->Hk * (p.nb + 1);
     p.max_chunks = bp.max_chunks;
     p.pkv = (float*)(w + bp.o_pkv);
     p.pbias = (double*)(w + bp.o_pbias);
