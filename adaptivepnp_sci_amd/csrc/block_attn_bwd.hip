@@ -106,8 +106,9 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
 }
 
 // ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
-// most tiles lie) in registers.  Three products a tile and vector work of the same length: 97 us for 131072 bf16 rows of 64 with
-// about 1000 keys each, 215 us (fp32 matrix rate 60 TFLOP/s, a third of the third product padding) for 65536 x 1024 of 48 wide fp32
+// most tiles lie) in registers.  Three products a tile and vector work of twice their length: 77 us for 131072 bf16 rows of 64 with
+// about 1000 keys each (three waves a SIMD; with two, and no register in scratch outside the loop, 98), 196 us for 65536 x 1024 of 48
+// wide fp32 (99 TFLOP/s)
 template <typename T, int DP>
 struct DqCfg {
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
@@ -117,7 +118,7 @@ struct DqCfg {
 constexpr int HROW = 33;                                  // a bucket's sums of 32 rows, shifted by a bank
 
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes, int plans, int CH) {
+__global__ void __launch_bounds__(256, DP > 64 ? 1 : sizeof(T) == 2 ? 3 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes, int plans, int CH) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DqCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
