@@ -107,7 +107,7 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
 
 // ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
 // most tiles lie) in registers.  Three products a tile and vector work of twice their length: 77 us for 131072 bf16 rows of 64 with
-// about 1000 keys each (three waves a SIMD; with two, and no register in scratch outside the loop, 98), 196 us for 65536 x 1024 of 48
+// about 1000 keys each (three waves a SIMD; with two, and no register in scratch outside the loop, 98; 128 wide two instead of one: 72 us less), 196 us for 65536 x 1024 of 48
 // wide fp32 (99 TFLOP/s)
 template <typename T, int DP>
 struct DqCfg {
@@ -118,7 +118,7 @@ struct DqCfg {
 constexpr int HROW = 33;                                  // a bucket's sums of 32 rows, shifted by a bank
 
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : sizeof(T) == 2 ? 3 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes, int plans, int CH) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP > 64 ? 1 : 2) block_attn_dq_kernel(Attn a, int sets, int set_bytes, int plans, int CH) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DqCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
@@ -351,13 +351,16 @@ struct DkvCfg {
     static_assert(JOIN <= MAIN, "the join reuses the tiles");
     static constexpr int LIST = 1032;                     // query groups of a chunk
 };
+// bf16: the transposed rows are read early, under the vector work, up to 64 wide (103 us, late 106).  96 wide they would leave one wave a
+// SIMD; read late, there are two (the whole backward pass of 131072 rows: 376 us instead of 497)
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(Attn a, int subs, unsigned magic_r, unsigned magic_g) {
+__global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) block_attn_dkv_kernel(Attn a, int subs, unsigned magic_r, unsigned magic_g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = DkvCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32, LC = DmaTile<T, DP>::LC, PIECES = DmaTile<T, DP>::PIECES, MINE = (PIECES + 1) / 2, BYTES = DmaTile<T, DP>::BYTES;
+    constexpr bool LATE = DP > 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // (chunks in turn over the XCDs: the last of a sequence and key head's slots are empty)
     const int sub = blockIdx.x % subs, c = blockIdx.x / subs % a.max_chunks, bh = blockIdx.x / subs / a.max_chunks, hk = bh % a.Hk, b = bh / a.Hk;
@@ -533,8 +536,10 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
         __builtin_amdgcn_s_setprio(0);
         ColTile<T, DP> gc, qc;
-        gc.read(at + BYTES, lane);
-        qc.read(at, lane);
+        if constexpr (!LATE) {
+            gc.read(at + BYTES, lane);
+            qc.read(at, lane);
+        }
         const float* const mine = info + 4 * hi;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -579,7 +584,9 @@ __global__ void __launch_bounds__(256, DP > 64 ? 1 : 2) block_attn_dkv_kernel(At
             }
         }
         __builtin_amdgcn_s_setprio(1);
+        if constexpr (LATE) gc.read(at + BYTES, lane);
         gc.mma(s, vacc);
+        if constexpr (LATE) qc.read(at, lane);
         qc.mma(dp, kacc);
         __builtin_amdgcn_s_setprio(0);
     }
