@@ -19,21 +19,30 @@
 
 namespace scipnp {
 
-template <typename T, int DP>
+// LEAN, bf16 of 96 and 128 columns: three waves a SIMD instead of two (417 instead of 460 us for the first case above, kernel alone; 139
+// instead of 155 at 8192 queries of 32 heads of 96 in groups of 16).  V is read behind the softmax, 64 columns at a time, which saves the
+// registers; and of V there is one buffer where only two waves share a pair of tiles, which saves the LDS: it is asked for when its
+// tile's scores begin.  Not where there is no third workgroup for a CU (52 us instead of 49 at 4096 queries of 16 heads of 128), nor
+// with P in three parts of 128 columns (30 registers would go to scratch in the loop), nor for one wave a set (LDS).
+template <typename T, int DP, int RW, bool SAVE>
+constexpr bool can_be_lean() { return sizeof(T) == 2 && DP > 64 && RW > 1 && !(SAVE && DP == 128); }
+template <typename T, int DP, int RW, bool LEAN>
 struct FwdCfg {
-    static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
-    static constexpr int MAIN = 2 * TILE;
+    static constexpr bool ONE_V = LEAN && RW == 2;
+    static constexpr int BYTES = DmaTile<T, DP>::BYTES;
+    static constexpr int MAIN = (ONE_V ? 3 : 4) * BYTES;                      // two K, one or two V
     static constexpr int KP = 2 * KT * 4;
 };
 
 // A workgroup holds `sets` sets of RW waves, each with work of its own: four waves a workgroup land one on each SIMD of a CU, where
 // workgroups of one or two leave some SIMDs with three waves and some with one.
-template <typename T, int DP, int RW, bool SAVE>           // SAVE: out32 wanted (a training pass)
-__global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
+template <typename T, int DP, int RW, bool SAVE, bool LEAN>          // SAVE: out32 wanted (a training pass)
+__global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    using C = FwdCfg<T, DP>;
+    using C = FwdCfg<T, DP, RW, LEAN>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32;
+    constexpr bool ONE_V = C::ONE_V;
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
     const long long total = (long long)a.B * a.Hk * a.ng * a.chunks * a.splits;
     const long long first = xcd_item(blockIdx.x, (total + sets - 1) / sets);
@@ -103,9 +112,8 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
     };
     auto issue = [&](int key0, int buf) {
         const int there = min(KT, sq.klen - key0);
-        char* const tile = smem + buf * C::TILE;
-        ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, tile, rw);
-        vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, tile + DmaTile<T, DP>::BYTES, rw);
+        ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, smem + buf * C::BYTES, rw);
+        if constexpr (!ONE_V) vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, smem + (2 + buf) * C::BYTES, rw);
         if (a.k_pos && tset < KT) kpr = tset < there ? a.k_pos[(size_t)b * a.Lk + key0 + tset] : 0;
     };
     const int far = 2 * a.maxd;                           // the two ends, where most tiles lie: their bias in registers
@@ -125,22 +133,25 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         int* const kp = kp_lds + buf * KT;
         if (a.k_pos && tset < KT) kp[tset] = kpr;
         dma_wait<RW>();                                   // this tile has landed, and everyone is done with the other buffer
+        if constexpr (ONE_V) vo.issue(vb + (long long)cur * a.sv.t, min(KT, sq.klen - cur), vs, a.D, smem + 2 * C::BYTES, rw);
         if (t + 1 < count) {
             key0 = next_key();
             issue(key0, buf ^ 1);
         }
-        const char* const kt = smem + buf * C::TILE;
+        const char* const kt = smem + buf * C::BYTES;
+        const char* const v_at = smem + (ONE_V ? 2 : 2 + buf) * C::BYTES;
         // (a wave with products to issue goes before one in its softmax: 73.6 -> 69.5 us in training at 2 x 4096 tokens, 16 heads of 64)
         __builtin_amdgcn_s_setprio(1);
-        f32x16a s = dma_rows<T, DP>(kt, qf, lane);
+        f32x16a s = dma_rows<T, DP, LEAN>(kt, qf, lane);
         __builtin_amdgcn_s_setprio(0);
-        ColTile<T, DP> vt;
-        vt.read(kt + DmaTile<T, DP>::BYTES, lane);
+        ColTile<T, DP, LEAN && NB == 4 ? 2 : NB> vt;
+        if constexpr (LEAN) vt.at(v_at, lane);
+        else vt.read(v_at, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
         const bool masked = cur + KT - 1 > min_lim;
         bool skip = false;
         float c = a.scale2, add = 0.f;
-        if (dist >= 0 && a.nbuckets) add = dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
+        if (dist >= 0 && a.nbuckets) add = !LEAN && dist == 0 ? bias_lo : !LEAN && dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
         if (dist < 0 || masked || c < 0.f) {              // the scores one by one
             if (dist < 0) {
                 float x[16];
@@ -152,7 +163,7 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
                 for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, add);
             }
             if (masked) {
-                if (!vt.finite()) {                       // (what its values add comes behind the loop, key by key)
+                if (!LEAN && !vt.finite()) {                       // (what its values add comes behind the loop, key by key)
                     spoilt = skip = true;
                     vt.clear();
                 }
@@ -186,11 +197,26 @@ __global__ void __launch_bounds__(256, 2) block_attn_kernel(Attn a, int sets, in
         if constexpr (sizeof(T) == 4) {
             if (skip) continue;
         }
+        if constexpr (ONE_V) dma_wait_but<DmaOffsets<T, DP, RW>::N>(t + 1 < count);
+        if constexpr (LEAN) {
+            if (masked && !vt.template finite<false>()) {
+                spoilt = true;
+                continue;
+            }
+        }
         __builtin_amdgcn_s_setprio(1);
+        if constexpr (LEAN) vt.read(v_at, lane);
         vt.template mma<SAVE ? 3 : 1>(s, sums);
+        if constexpr (LEAN && NB == 4) {
+            vt.read(v_at, lane, 2);
+            vt.template mma<SAVE ? 3 : 1>(s, sums, 2);
+        }
         __builtin_amdgcn_s_setprio(0);
     }
-    for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
+    for (int t = count; t < trips; ++t) {                 // (the other sets' barriers)
+        dma_wait<RW>();
+        if constexpr (ONE_V) dma_wait<RW>();
+    }
     l += __shfl_xor(l, 32, 64);
     f32x16a o[NB];
     sums.blocks(o);
@@ -367,23 +393,30 @@ Attn attn_params(const scipnp_block_attn_args* a) {
     return p;
 }
 
-template <typename T, int DP, int RW, bool SAVE>
+template <typename T, int DP, int RW, bool SAVE, bool LEAN>
 static int fwd_launch(const Attn& p, hipStream_t st) {
-    using C = FwdCfg<T, DP>;
+    using C = FwdCfg<T, DP, RW, LEAN>;
     const size_t set = ((size_t)C::MAIN + C::KP + (size_t)(p.n + 4) / 4 * 16 + (size_t)p.nbuckets * p.G * 4 + 15) / 16 * 16;
     const size_t shared = bias_lut_bytes(p.nbuckets, p.maxd) + 16;
     int sets = 4 / RW;
     while (sets > 1 && shared + sets * set > 163840) sets >>= 1;
     static LdsAttrOnce once;
-    if (const int rc = once.ensure((const void*)block_attn_kernel<T, DP, RW, SAVE>, 163840, "block_attn")) return rc;
+    if (const int rc = once.ensure((const void*)block_attn_kernel<T, DP, RW, SAVE, LEAN>, 163840, "block_attn")) return rc;
     const long long items = (long long)p.B * p.Hk * p.ng * p.chunks * p.splits;
-    block_attn_kernel<T, DP, RW, SAVE><<<xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set);
+    block_attn_kernel<T, DP, RW, SAVE, LEAN><<<xcd_grid((items + sets - 1) / sets), 64 * RW * sets, shared + sets * set, st>>>(p, sets, (int)set);
     return SCIPNP_OK;
+}
+template <typename T, int DP, int RW, bool SAVE>
+static int fwd_pick(const Attn& p, hipStream_t st) {
+    if constexpr (can_be_lean<T, DP, RW, SAVE>()) {        // (more than two workgroups of four waves for each of 256 CUs)
+        if ((long long)p.B * p.Hk * p.ng * p.chunks * p.splits > 512 * (4 / RW)) return fwd_launch<T, DP, RW, SAVE, true>(p, st);
+    }
+    return fwd_launch<T, DP, RW, SAVE, false>(p, st);
 }
 template <typename T, int DP>
 static int fwd_rows(const Attn& p, int rw, hipStream_t st) {
-    if (p.out32) return rw == 1 ? fwd_launch<T, DP, 1, true>(p, st) : rw == 2 ? fwd_launch<T, DP, 2, true>(p, st) : fwd_launch<T, DP, 4, true>(p, st);
-    return rw == 1 ? fwd_launch<T, DP, 1, false>(p, st) : rw == 2 ? fwd_launch<T, DP, 2, false>(p, st) : fwd_launch<T, DP, 4, false>(p, st);
+    if (p.out32) return rw == 1 ? fwd_pick<T, DP, 1, true>(p, st) : rw == 2 ? fwd_pick<T, DP, 2, true>(p, st) : fwd_pick<T, DP, 4, true>(p, st);
+    return rw == 1 ? fwd_pick<T, DP, 1, false>(p, st) : rw == 2 ? fwd_pick<T, DP, 2, false>(p, st) : fwd_pick<T, DP, 4, false>(p, st);
 }
 template <typename T>
 static int fwd_dim(const Attn& p, int rw, hipStream_t st) {

@@ -115,11 +115,11 @@ struct RowTile {
         return acc;
     }
 };
-template <typename T, int DP>
+template <typename T, int DP, bool LEAN = false>          // LEAN: the compiler may read a part at a time, in fewer registers
 __device__ __forceinline__ f32x16a dma_rows(const char* tile, const typename Mat<T>::Frag (&b)[DP / Mat<T>::K], int lane) {
     RowTile<T, DP> r;
     r.read(tile, lane);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!LEAN) __builtin_amdgcn_sched_barrier(0);
     return r.mma(b);
 }
 
@@ -199,29 +199,32 @@ struct Acc {
                 }
     }
 };
-template <typename T, int DP>
+template <typename T, int DP, int PART = (DP + 31) / 32>   // PART: column blocks held at a time (bf16)
 struct ColTile {
-    static constexpr int LC = DmaTile<T, DP>::LC, NB = (DP + 31) / 32;
+    static constexpr int LC = DmaTile<T, DP>::LC, NB = PART;
     union Pair { u32x2a s[2]; bf16x8 v; };
     Pair u[sizeof(T) == 2 ? NB : 1][2];
     const char* tile;
     int lane;
-    __device__ __forceinline__ void read(const char* tile_, int lane_) {
+    __device__ __forceinline__ void at(const char* tile_, int lane_) {
         tile = tile_;
         lane = lane_;
+    }
+    __device__ __forceinline__ void read(const char* tile_, int lane_, int first = 0) {
+        at(tile_, lane_);
 #if defined(__HIP_DEVICE_COMPILE__)
         if constexpr (sizeof(T) == 2) {
             const int q = (lane >> 2) & 3, c0 = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), r0 = 4 * (lane >> 5) + q;
             const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) const char*)tile + r0 * LC * 16 + 8 * (lane & 1);
             const int f0 = c0 ^ swz<T, LC>(r0), f1 = c0 ^ swz<T, LC>(r0 + 8);
             constexpr int STEP = 16 * LC * 16, DOWN = 8 * LC * 16;         // 16 rows, 8 rows
-            unsigned at[2 * NB];
+            unsigned from[2 * NB];
 #pragma unroll
             for (int db = 0; db < NB; ++db) {
-                at[2 * db] = base + ((f0 ^ (4 * db)) << 4);
-                at[2 * db + 1] = base + ((f1 ^ (4 * db)) << 4);
+                from[2 * db] = base + ((f0 ^ (4 * (first + db))) << 4);
+                from[2 * db + 1] = base + ((f1 ^ (4 * (first + db))) << 4);
             }
-            read_blocks<STEP, DOWN>(at);
+            read_blocks<STEP, DOWN>(from);
         }
 #endif
     }
@@ -287,10 +290,19 @@ struct ColTile {
     }
 #endif
     // No infinity and no NaN in the tile: a masked weight of 0 would carry it into rows that do not see it (0 x inf)
+    template <bool READ = true>
     __device__ __forceinline__ bool finite() const {
         float sum = 0.f;                                  // of x * 0
 #if defined(__HIP_DEVICE_COMPILE__)
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 && !READ) {
+            const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
+#pragma unroll 2
+            for (int i = 0; i < DmaTile<T, DP>::PIECES; ++i) {
+                const bf16x8 x = *(const bf16x8*)(tile + i * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * e], x[2 * e + 1]}, zero, sum, false);
+            }
+        } else if constexpr (sizeof(T) == 2) {
             const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
 #pragma unroll
             for (int db = 0; db < NB; ++db)
@@ -320,7 +332,7 @@ struct ColTile {
         }
     }
     template <int PARTS = 1>
-    __device__ __forceinline__ void mma(const f32x16a& p, Acc<T, DP>& sums) const {
+    __device__ __forceinline__ void mma(const f32x16a& p, Acc<T, DP>& sums, int first = 0) const {
         auto& acc = sums.x;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -337,13 +349,13 @@ struct ColTile {
                     }
                 }
 #pragma unroll
-                for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, pb, acc[db], 0, 0, 0);
+                for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, pb, acc[first + db], 0, 0, 0);
                 if constexpr (PARTS > 1)
 #pragma unroll
-                    for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p1, acc[db], 0, 0, 0);
+                    for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p1, acc[first + db], 0, 0, 0);
                 if constexpr (PARTS > 2)
 #pragma unroll
-                    for (int db = 0; db < NB; ++db) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[db], 0, 0, 0);
+                    for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[first + db], 0, 0, 0);
             }
         } else if constexpr (Acc<T, DP>::N16) {
             constexpr int NC = DP / 16;
@@ -426,6 +438,19 @@ __device__ __forceinline__ void dma_wait() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0070);                   // vmcnt(0) lgkmcnt(0)
     if constexpr (WAVES > 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#endif
+}
+
+// ... all but the last N requests, where there were any behind them; every wave's
+template <int N>
+__device__ __forceinline__ void dma_wait_but(bool more) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    static_assert(N < 16, "the low four bits of the count");
+    asm volatile("" ::: "memory");
+    if (more) __builtin_amdgcn_s_waitcnt(0x0F70 | N);     // vmcnt(N)
+    else __builtin_amdgcn_s_waitcnt(0x0F70);
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #endif
 }

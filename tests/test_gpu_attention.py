@@ -268,6 +268,52 @@ def test_what_a_later_key_holds_does_not_reach_an_earlier_query(A, B, L, Hq, Hk,
     within(got.nan_to_num(nan=0.0), val.nan_to_num(nan=0.0), err.nan_to_num(nan=0.0), 'out')
 
 
+def again(t, times):
+    return t.repeat(times, *[1] * (t.dim() - 1))
+
+
+def of_all(how, times):
+    return on_gpu({n: again(t, times) if n in ('qlen', 'klen', 'q_pos', 'k_pos') and t is not None else t for n, t in how.items()})
+
+
+@pytest.mark.parametrize('times,case', [
+    (37, (2, 100, 300, 8, 2, 128, 64, 16, 4, True, True, 32, 128, False)),
+    (210, (1, 65, 257, 3, 1, 112, 64, 16, 3, False, True, 16, 16, True)),
+    (33, (1, 200, 300, 8, 2, 128, 64, 64, 3, True, False, 0, 0, False)),
+    (26, (2, 130, 400, 5, 1, 96, 128, 32, 3, True, True, 8, 60, False)),
+    (86, (1, 150, 150, 4, 1, 72, 64, 13, 3, True, False, 4, 16, False)),
+])
+def test_more_workgroups_than_two_a_cu(A, times, case):
+    """wide bf16 heads have a kernel of their own there: the same sequences many times over, each with the result of the first"""
+    q, k, v, _, sel, how = problem(case, 'bf16', torch.Generator().manual_seed(case[1] + case[2]))
+    want = reference(q, k, v, sel, how)['out']
+    args = [cu(again(t, times)) for t in (q, k, v, sel)]
+    for save in (False, True):
+        got = A.block_attention(*args, save=save, **of_all(how, times))
+        got = (got[0] if save else got).unflatten(0, (times, q.shape[0]))
+        within(got[0], *want, 'out')
+        assert torch.equal(got, got[:1].expand_as(got))
+
+
+@pytest.mark.parametrize('times,L,Hq,Hk,D,qb', [(58, 130, 8, 2, 128, 16), (90, 140, 4, 1, 96, 64), (60, 130, 4, 1, 128, 64)])
+def test_values_that_are_not_numbers_with_more_workgroups_than_two_a_cu(A, times, L, Hq, Hk, D, qb):
+    gen = torch.Generator().manual_seed(L)
+    q, k, v = (randn(gen, 1, L, h, D, dtype=torch.bfloat16) for h in (Hq, Hk, Hk))
+    v[0, L // 2, 0, 3], v[0, L // 2 + 1, 0, D - 1], v[0, L - 1, -1, 0] = math.inf, -math.inf, math.nan
+    nb, ng = -(-L // 64), -(-L // qb)
+    sel = torch.arange(nb, dtype=torch.int32).expand(1, Hk, ng, nb).contiguous()
+    from adaptivepnp_sci_amd.attention import bucket_table
+    how = dict(block=64, query_block=qb, scale=0.3 / math.sqrt(D), causal=True, qlen=None, klen=None, bucket_of=bucket_table(8, 40, False),
+               bias=0.3 * randn(gen, 8, Hq), q_pos=None, k_pos=None)
+    val, err = reference(q, k, v, sel, how)['out']
+    assert torch.isfinite(val).any() and not torch.isfinite(val).all()
+    got = A.block_attention(*(cu(again(t, times)) for t in (q, k, v, sel)), **of_all(how, times)).double().cpu()
+    for one in (got[:1], got[-1:]):
+        assert torch.equal(torch.isnan(one), torch.isnan(val)) and torch.equal(torch.isinf(one), torch.isinf(val))
+        within(one.nan_to_num(nan=0.0), val.nan_to_num(nan=0.0), err.nan_to_num(nan=0.0), 'out')
+    assert torch.equal(got.nan_to_num(nan=0.0), got[:1].nan_to_num(nan=0.0).expand_as(got))
+
+
 @pytest.mark.parametrize('dt', ['f32', 'bf16'])
 @pytest.mark.parametrize('low', [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min])
 def test_a_bias_of_the_lowest_value_masks(A, low, dt):
