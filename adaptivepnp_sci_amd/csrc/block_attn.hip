@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     const Seq sq = seq_of(a, b);
     const int R = a.qb * a.G, r0 = chunk * 32 * RW;
     const bool any = there_is && g * a.qb + r0 / a.G < sq.qlen;             // a live row in this chunk
-    const int row = r0 + rw * 32 + li, tok = g * a.qb + row / a.G, gl = row % a.G, head = hk * a.G + gl;
-    const bool live = there_is && row < R && tok < sq.qlen;
+    int row = r0 + rw * 32 + li, tok = g * a.qb + row / a.G, gl = row % a.G, head = hk * a.G + gl;
+    bool live = there_is && row < R && tok < sq.qlen;
     const int qkey = sq.shift + tok;                      // key position of the row
     const int lim = !live ? -1 : a.causal ? min(qkey, sq.klen - 1) : sq.klen - 1;       // its last visible key
 
@@ -114,7 +114,11 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         const int there = min(KT, sq.klen - key0);
         ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, smem + buf * C::BYTES, rw);
         if constexpr (!ONE_V) vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, smem + (2 + buf) * C::BYTES, rw);
-        if (a.k_pos && tset < KT) kpr = tset < there ? a.k_pos[(size_t)b * a.Lk + key0 + tset] : 0;
+        if (a.k_pos && tset < KT) {
+            int x = tset;
+            if constexpr (LEAN) asm volatile("" : "+v"(x));                  // (no address in registers between tiles)
+            kpr = x < there ? a.k_pos[(size_t)b * a.Lk + key0 + x] : 0;
+        }
     };
     const int far = 2 * a.maxd;                           // the two ends, where most tiles lie: their bias in registers
     const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
@@ -221,6 +225,15 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     f32x16a o[NB];
     sums.blocks(o);
     const Attn& z = late_args();                          // (what only the end needs is read again there: the loop's scalars fit the registers)
+    if constexpr (LEAN) {                                 // (the row's place as well: no register holds it through the loop)
+        int x = li;
+        asm volatile("" : "+v"(x));
+        row = r0 + rw * 32 + x;
+        tok = g * z.qb + row / z.G;
+        gl = row % z.G;
+        head = hk * z.G + gl;
+        live = there_is && row < R && tok < sq.qlen;
+    }
     // Tiles with masked keys and values that are not numbers: only rows that see a key take its value, by plain loads
     if (spoilt) {
         const T* const qr = (const T*)z.q + b * z.sq.b + tok * z.sq.t + head * z.sq.h;

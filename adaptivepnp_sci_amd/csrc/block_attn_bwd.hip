@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
     using C = DqCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32;
+    constexpr bool LEAN = sizeof(T) == 2;                 // K read behind the vector work, the ends' bias from LDS: nothing in scratch at three waves
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
     if (blockIdx.x < plans) {                             // the first workgroups cut the chunks of the launch behind this one
         plan_chunks(a, blockIdx.x, a.qb * a.G, CH, (int*)smem_all);
@@ -253,12 +254,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
         const f32x16a dp = dma_rows<T, DP>(kt + DmaTile<T, DP>::BYTES, gf, lane);
         __builtin_amdgcn_s_setprio(0);
         ColTile<T, DP> kc;
-        kc.read(kt, lane);
+        if constexpr (!LEAN) kc.read(kt, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
         // fp32: the large numbers, score and log-sum-exp, meet in one fused operation, and what is small is added behind it; bf16 weights
         // are rounded to 8 bits anyway: one operation
         if (dist >= 0) {
-            const float b = !a.nbuckets ? 0.f : dist == 0 ? bias_lo : dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
+            const float b = !a.nbuckets ? 0.f : !LEAN && dist == 0 ? bias_lo : !LEAN && dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
             if constexpr (sizeof(T) == 4) {
                 const float rest = b + shift.lo;
 #pragma unroll
@@ -298,6 +299,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
             }
         }
         __builtin_amdgcn_s_setprio(1);
+        if constexpr (LEAN) kc.read(kt, lane);
         kc.template mma<2>(s, sums);                      // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
         __builtin_amdgcn_s_setprio(0);
     }
