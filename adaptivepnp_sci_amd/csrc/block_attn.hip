@@ -7,19 +7,19 @@
 // costs no accuracy in floating point, and the accumulators are not rescaled.
 //
 // What it is bound by, measured:
-//   bf16, 128 wide, 16384 queries of 32 heads (16 a group), 16 blocks of 64 each: 404 us, 660 TFLOP/s against 1150 of a large matrix
-//     product.  A tile is 512 cycles of matrix work and about 125 vector instructions, 16 of them exponentials (700 cycles); 215 registers
-//     and 64 KB of tiles a workgroup leave two waves a SIMD, which overlap the two only in part (LDS is busy 17 % of the time and has no bank
-//     conflicts).  Taken out one at a time, of then 490 us: the requests for tiles 426, they and the barriers 387, the second product 440,
-//     the exponentials 499.  64 rows a wave: 636 us, the accumulators no longer fit beside the operands.
-//   fp32, 48 wide, 131072 tokens, 16 blocks of 64: 274 us, 94 TFLOP/s against 133; a quarter of the second product is padding to 64.
+//   bf16, 128 wide, 16384 queries of 32 heads over 8 key heads, groups of 16 queries, 16 blocks of 64 each: 381 us, 700 TFLOP/s against 1150
+//     of a large matrix product.  A tile is 512 cycles of matrix work and about 125 vector instructions, 16 of them exponentials (700 cycles); three
+//     waves a SIMD (168 registers, 50 KB of LDS a workgroup) overlap the two in part, two waves less (406 us; LDS is busy 17 % of the time
+//     and has no bank conflicts).  Taken out one at a time, of then 490 us with two: the requests for tiles 426, they and the
+//     barriers 387, the second product 440, the exponentials 499.  64 rows a wave: 636 us, the accumulators no longer fit beside the operands.
+//   fp32, 48 wide, 131072 tokens, 16 blocks of 64: 242 us, 106 TFLOP/s against 133; four workgroups a CU are a round of three and one of one.
 //   bf16, 128 wide, one token of 16 sequences, 64 blocks of 64: 48 us + 4.8 of the join, 5.1 TB/s of the keys and values read.
 //   Workgroups in contiguous eighths a die: 73.5 us at 2 x 4096 bf16 tokens, 16 heads of 64, in turn over the dies 83.9.
 #include "block_attn.hpp"
 
 namespace scipnp {
 
-// LEAN, bf16 of 96 and 128 columns: three waves a SIMD instead of two (417 instead of 460 us for the first case above, kernel alone; 139
+// LEAN, bf16 of 96 and 128 columns: three waves a SIMD instead of two (381 instead of 406 us for the first case above; 139
 // instead of 155 at 8192 queries of 32 heads of 96 in groups of 16).  V is read behind the softmax, 64 columns at a time, which saves the
 // registers; and of V there is one buffer where only two waves share a pair of tiles, which saves the LDS: it is asked for when its
 // tile's scores begin.  Not where there is no third workgroup for a CU (52 us instead of 49 at 4096 queries of 16 heads of 128), nor

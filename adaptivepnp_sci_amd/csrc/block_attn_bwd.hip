@@ -6,8 +6,8 @@
 // into chunks of equal length, since a first block is chosen by every group and most blocks by few.
 //
 // Four launches: the selection turned round; dQ, dbias, delta and the chunks; dK and dV; the chunks' sums.  2 x 4096 bf16 tokens, 16
-// heads of 64 over 4 key heads, 16 blocks of 64: 5 + 97 + 104 + 9 us behind a forward pass of 74; 65536 fp32 tokens of 48, one head:
-// 5 + 215 + 350 + 17 behind 158.  (One launch more for each of delta, the chunks and dbias: 350 us instead of 311 for the first.)
+// heads of 64 over 4 key heads, 16 blocks of 64: 5 + 77 + 102 + 9 us behind a forward pass of 70; 65536 fp32 tokens of 48, one head:
+// 5 + 191 + 311 + 17 behind 133.  (One launch more for each of delta, the chunks and dbias: 350 us instead of 311 for the first.)
 #include "block_attn.hpp"
 
 namespace scipnp {
@@ -107,8 +107,8 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
 
 // ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
 // most tiles lie) in registers.  Three products a tile and vector work of twice their length: 77 us for 131072 bf16 rows of 64 with
-// about 1000 keys each (three waves a SIMD; with two, and no register in scratch outside the loop, 98; 128 wide two instead of one: 72 us less), 196 us for 65536 x 1024 of 48
-// wide fp32 (99 TFLOP/s)
+// about 1000 keys each (three waves a SIMD; two, with the transposed keys read before the vector work: 98; 128 wide two waves instead of one: 72 us less),
+// 191 us for 65536 x 1024 of 48 wide fp32 (101 TFLOP/s against 133)
 template <typename T, int DP>
 struct DqCfg {
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
 // dK += Q^T dS with the transposed rows as A and the score registers as B.
 // Bound by the vector work between the products: four products of 32 x 32 take 512 cycles a tile at bf16, 64 wide, the rest about
 // 900, of which the rows' books are a fifth (they were half while every lane divided for its own requests: 447 instead of 350 us in
-// fp32).  Chunks of a 2048th of all rows: larger ones leave CUs idle at the end (117 us instead of 104 at a 1024th), smaller ones pay
+// fp32).  Chunks of a 2048th of all rows: larger ones leave CUs idle at the end (113 us instead of 103 at a 1024th), smaller ones pay
 // for their beginnings (110 at a 4096th).
 // What a row brings besides: its last visible key, delta, log-sum-exp, and its bias where all 64 keys share its bucket.
 template <typename T, int DP>
