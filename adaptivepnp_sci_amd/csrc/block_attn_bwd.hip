@@ -170,7 +170,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
     load_frags<T, DP>(live ? (const T*)a.q + b * a.sq.b + (long long)tok * a.sq.t + head * a.sq.h : nullptr, a.D, hi, qf);
     load_frags<T, DP>(live ? (const T*)a.dout + b * a.sdo.b + (long long)tok * a.sdo.t + head * a.sdo.h : nullptr, a.D, hi, gf);
     const size_t stat = ((size_t)b * a.Hq + head) * a.Lq + tok;
-    Shift shift = {0.f, 0.f};                             // minus the row's log-sum-exp
+    // minus the row's log-sum-exp.  A row that does not exist (or saw nothing) has a weight of exp2(-inf) = 0 whatever its bias: the sums of
+    // dbias run over all rows of a wave, and its exponential of a large bias would be infinity there, times a zero
+    Shift shift = {-INFINITY, 0.f};
     if (live) {
         const float lse = a.lse[stat];
         if (lse == -INFINITY) lim = -1;                   // (a row that saw nothing: of its keys, or because the bias masks them)
