@@ -89,6 +89,11 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     ko.init(rw, lane, ks, a.D);
     vo.init(rw, lane, vs, a.D);
     __syncthreads();
+    // a bias of this key head masks (uniform; few tables do): its keys are masked like those behind the last visible one, and what they hold
+    // is kept out of the products tile by tile
+    bool masks = false;
+    for (int i = lane; i < a.nbuckets * a.G; i += 64) masks |= bias.tbl[i] == -INFINITY;
+    masks = __ballot(masks) != 0;
 
     const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist);
     const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, count = max(0, min(ntiles, t_begin + per) - t_begin);
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         if constexpr (LEAN) vt.at(v_at, lane);
         else vt.read(v_at, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
-        const bool masked = cur + KT - 1 > min_lim;
+        const bool masked = masks || cur + KT - 1 > min_lim;
         bool skip = false;
         float c = a.scale2, add = 0.f;
         if (dist >= 0 && a.nbuckets) add = !LEAN && dist == 0 ? bias_lo : !LEAN && dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
@@ -165,6 +170,14 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, add);
+            }
+            if (masks) {                                  // (a key that is not a number, plus minus infinity, would still be none)
+                int y = qp;
+                asm volatile("" : "+v"(y));               // (the biases are read again: no register holds them through the tiles of every call)
+                float x[16];
+                if (dist < 0) tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, y, gl, hi, x);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = (dist < 0 ? x[r] : add) == -INFINITY ? -INFINITY : s[r];
             }
             if (masked) {
                 if (!LEAN && !vt.finite()) {                       // (what its values add comes behind the loop, key by key)
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         const T* const qr = (const T*)z.q + b * z.sq.b + tok * z.sq.t + head * z.sq.h;
         for (int t = t_begin; t < t_begin + count; ++t) {
             const int cur = __builtin_amdgcn_readfirstlane(list[t / tpb]) * z.block + t % tpb * KT, there = min(KT, sq.klen - cur);
-            if (cur + KT - 1 <= min_lim) continue;
+            if (!masks && cur + KT - 1 <= min_lim) continue;
             bool bad = false;
             for (int j = 0; j < there; ++j)
                 for (int d = lane; d < z.D; d += 64) bad |= !(fabsf((float)vb[(cur + j) * z.sv.t + d]) < INFINITY);
@@ -248,13 +261,14 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
                 if (!live || cur + j > lim) continue;
                 const T* const kr = kb + (cur + j) * z.sk.t;
                 const T* const vr = vb + (cur + j) * z.sv.t;
-                float x = 0.f;
-                for (int d = 0; d < z.D; ++d) x = fmaf((float)kr[d], (float)qr[d], x);
-                x *= z.scale2;
+                float x = 0.f, add = 0.f;
                 if (z.nbuckets) {
                     const int kp = z.k_pos ? z.k_pos[(size_t)b * z.Lk + cur + j] : cur + j;
-                    x += bias.tbl[bias.lut[clamp_dist(kp - qp, z.maxd)] * z.G + gl];
+                    add = bias.tbl[bias.lut[clamp_dist(kp - qp, z.maxd)] * z.G + gl];
+                    if (add == -INFINITY) continue;
                 }
+                for (int d = 0; d < z.D; ++d) x = fmaf((float)kr[d], (float)qr[d], x);
+                x = fmaf(x, z.scale2, add);
                 const float p = __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
                 each_four<T, DP>(hi, [&](int d, auto at) {
                     if (d >= z.D) return;

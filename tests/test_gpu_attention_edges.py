@@ -69,3 +69,58 @@ def test_large_biases_beside_rows_that_do_not_exist(A, B, Lq, Lk, Hq, Hk, D, qb,
     within(out, *want['out'], 'out')
     for name, t in zip(('dq', 'dk', 'dv', 'dbias'), A.block_attention_backward(g.cuda(), *args, saved, **on_gpu(how))):
         within(t, *want[name], name)
+
+
+# ------------------------------------------------------------------ keys that a bias masks
+def spoil(gen, k, v, at):
+    """infinities and NaN in the keys and values at those places"""
+    for i, x in enumerate(at):
+        k[..., x, :, i % k.shape[-1]] = (math.nan, math.inf, -math.inf)[i % 3]
+        v[..., x, :, (3 * i + 1) % k.shape[-1]] = (math.inf, math.nan, -math.inf)[i % 3]
+
+
+MASKED = [  # times, B, Lq, Lk, Hq, Hk, D, qb
+    (1, 1, 150, 150, 2, 1, 64, 16), (1, 2, 70, 70, 1, 1, 48, 64), (1, 1, 90, 90, 6, 2, 128, 8), (1, 1, 64, 64, 1, 1, 8, 200), (1, 1, 100, 100, 3, 3, 112, 32),
+    (90, 1, 130, 130, 8, 2, 128, 16), (90, 1, 140, 140, 4, 1, 96, 64),      # (more than two workgroups a CU)
+]
+
+
+@pytest.mark.parametrize('low', [-math.inf, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('times,B,Lq,Lk,Hq,Hk,D,qb', MASKED)
+def test_what_a_key_masked_by_its_bias_holds_does_not_reach_a_query(A, times, B, Lq, Lk, Hq, Hk, D, qb, dt, low):
+    """buckets of the keys behind a query masked, for one head or for all: a causal mask in another form"""
+    gen, T = torch.Generator().manual_seed(Lq * D), DT[dt]
+    q, k, v = randn(gen, B, Lq, Hq, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T)
+    spoil(gen, k, v, [Lk // 2, Lk // 2 + 1, Lk - 2, Lk - 1])
+    for some in (False, True):
+        bias = 0.3 * randn(gen, 8, Hq)
+        bias[4:, :1 if some else None] = low
+        how = dict(block=64, query_block=qb, scale=0.3 / math.sqrt(D), causal=False, qlen=None, klen=None, bucket_of=A.bucket_table(8, 40), bias=bias,
+                   q_pos=None, k_pos=None)
+        sel = every_block(B, Hk, Lq, Lk, qb)
+        val, err = reference(q, k, v, sel, how)['out']
+        assert torch.isfinite(val).any() and not torch.isfinite(val).all()
+        got = A.block_attention(*(t.repeat(times, 1, 1, 1).cuda() for t in (q, k, v, sel)), **on_gpu(how))
+        within(got[:B], val, err, 'out')
+        within(got[-B:], val, err, 'out of the last')
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('at', [[300, 301, 700, 1279], [300, 301, 1279]])        # (head 0 sees key 700)
+@pytest.mark.parametrize('Lq,qb,D', [(128, 64, 56), (128, 16, 128), (2, 1, 128), (1, 1, 64)])
+def test_frames_masked_by_their_distance(A, Lq, qb, D, at, dt):
+    """whole tiles of one bucket, masked; the keys split over workgroups where there are few queries"""
+    gen, T, Lk = torch.Generator().manual_seed(Lq + D), DT[dt], 1280
+    q, k, v = randn(gen, 1, Lq, 2, D, dtype=T), randn(gen, 1, Lk, 1, D, dtype=T), randn(gen, 1, Lk, 1, D, dtype=T)
+    spoil(gen, k, v, at)
+    table = torch.arange(9, dtype=torch.int32)                                # a bucket for every distance up to four frames
+    bias = 0.3 * randn(gen, 9, 2)
+    bias[torch.tensor([0, 1, 7, 8]), 0] = -math.inf                          # head 0 sees two frames around its own
+    bias[torch.tensor([0, 3, 6, 8]), 1] = -math.inf
+    how = dict(block=64, query_block=qb, scale=0.3 / math.sqrt(D), causal=False, qlen=None, klen=None, bucket_of=table, bias=bias,
+               q_pos=torch.full((1, Lq), 5, dtype=torch.int32), k_pos=(torch.arange(Lk, dtype=torch.int32) // 128)[None].contiguous())
+    sel = every_block(1, 1, Lq, Lk, qb)
+    val, err = reference(q, k, v, sel, how)['out']
+    assert 700 in at or torch.isfinite(val[:, :, 0]).all()
+    within(A.block_attention(q.cuda(), k.cuda(), v.cuda(), sel.cuda(), **on_gpu(how)), val, err, 'out')
