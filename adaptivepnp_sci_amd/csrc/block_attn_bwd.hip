@@ -294,10 +294,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
                 int d[16];
                 tile_buckets(a, bias, cur, a.k_pos ? kp : nullptr, qp, hi, d);
 #pragma unroll
-                for (int half = 0; half < 2; ++half)      // (the two lanes of a row share its words: one after the other)
+                for (int half = 0; half < 2; ++half) {    // (the two lanes of a row share its words: one after the other, the fence keeps them apart)
                     if (hi == half)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) mine[d[r] * HROW] += s[r];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
             }
         }
         __builtin_amdgcn_s_setprio(1);
