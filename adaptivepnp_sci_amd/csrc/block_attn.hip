@@ -391,7 +391,7 @@ int attn_check(const scipnp_block_attn_args* a) {
     if (a->num_buckets) {
         SCIPNP_REQUIRE(a->bias && a->bucket_of, "buckets need bias and bucket_of");
         SCIPNP_REQUIRE(a->max_distance > 0 && a->max_distance <= 4096, "max_distance %d: 1 to 4096", a->max_distance);
-        SCIPNP_REQUIRE(a->num_buckets * (a->Hq / a->Hk) <= 2048, "buckets times query heads of a key head: at most 2048");
+        SCIPNP_REQUIRE((long long)a->num_buckets * (a->Hq / a->Hk) <= 2048, "buckets times query heads of a key head: at most 2048");
     }
     SCIPNP_ALIGNED(a->q); SCIPNP_ALIGNED(a->k); SCIPNP_ALIGNED(a->v);
     SCIPNP_STRIDES(a->q_stride, a->dtype); SCIPNP_STRIDES(a->k_stride, a->dtype); SCIPNP_STRIDES(a->v_stride, a->dtype);

@@ -304,11 +304,12 @@ __global__ void __launch_bounds__(64 * SEL_WAVES) select_blocks_kernel(Select a)
     const int col = lane & 15, kq = lane >> 4, gc = g0 + col;
     const bool group = col < ngr && gc * a.qb < qlen;
     const int last = klen - qlen + min((gc + 1) * a.qb, qlen) - 1;
-    const int own = last >= 0 ? last / a.block : (last - a.block + 1) / a.block;
-    const int seen = min((klen + a.block - 1) / a.block, !a.causal ? a.nb : last < 0 ? 0 : last / a.block + 1);        // blocks it may choose
+    const int own = last >= 0 ? last / a.block : -1 - (-1 - last) / a.block;        // (no sum here passes 32 bits, whatever the block)
+    const int there = klen > 0 ? (klen - 1) / a.block + 1 : 0;
+    const int seen = min(there, !a.causal ? a.nb : last < 0 ? 0 : last / a.block + 1);        // blocks it may choose
     // no group here sees a block from `nb` on (its own rows end with the last group's last query): neither scored nor looked at
     const int lastq = min((g0 + ngr) * a.qb, qlen), end = klen - qlen + lastq;
-    const int nb = lastq <= g0 * a.qb ? 0 : min((klen + a.block - 1) / a.block, !a.causal ? a.nb : end <= 0 ? 0 : (end - 1) / a.block + 1);
+    const int nb = lastq <= g0 * a.qb ? 0 : min(there, !a.causal ? a.nb : end <= 0 ? 0 : (end - 1) / a.block + 1);
     const int nt = (nb + 15) / 16;
     const double* const qrow = qs + (col < a.gpw ? col : 0) * qst + 4 * kq;
     const float* const means = a.summary + ((size_t)b * a.nb * a.Hk + hk) * a.D;
@@ -398,13 +399,15 @@ int scipnp_block_summary(const void* k, const int64_t* k_stride, int dtype, cons
     Summary a = {};
     a.k = k; a.sk = strides_of(k_stride); a.klen = klen; a.out = summary;
     a.B = B; a.Lk = Lk; a.Hk = Hk; a.D = D; a.block = block; a.newest = newest;
-    a.nb = (Lk + block - 1) / block;
-    a.chunks = Hk * (D / (16 / (int)attn_esize(dtype)));
+    SCIPNP_REQUIRE((Lk - 1) / block + 1 < (1 << 24), "%d blocks: fewer than 2^24 (a larger block)", (Lk - 1) / block + 1);
+    a.nb = (Lk - 1) / block + 1;                          // (no sum that a block or a length near 2^31 would carry past 32 bits)
+    const long long chunks = (long long)Hk * (D / (16 / (int)attn_esize(dtype)));
+    SCIPNP_REQUIRE(chunks < (1 << 24), "too many key heads");
+    a.chunks = (int)chunks;
     a.cols = a.chunks < 256 ? a.chunks : 256;
     a.splits = 256 / a.cols;
-    const int touched = newest ? (newest + block - 1) / block + 1 : a.nb;
+    const int touched = newest ? (newest - 1) / block + 2 : a.nb;
     const int ny = (a.chunks + a.cols - 1) / a.cols;
-    SCIPNP_REQUIRE(ny < 65536, "too many key heads");
     const dim3 grid((unsigned)(touched < a.nb ? touched : a.nb), (unsigned)ny, (unsigned)B);
     if (dtype == SCIPNP_BF16) block_summary_kernel<__bf16><<<grid, 256, 0, (hipStream_t)s>>>(a);
     else block_summary_kernel<float><<<grid, 256, 0, (hipStream_t)s>>>(a);
@@ -425,12 +428,12 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s) {
     SCIPNP_ALIGNED(a->summary);
     SCIPNP_STRIDES(a->q_stride, a->dtype);
     Select p = {};
-    p.nb = (a->Lk + a->block - 1) / a->block;
+    p.nb = (a->Lk - 1) / a->block + 1;
     SCIPNP_REQUIRE(p.nb <= SEL_MAX_BLOCKS, "%d key blocks: at most %d (a larger block)", p.nb, SEL_MAX_BLOCKS);
     p.q = a->q; p.sq = strides_of(a->q_stride); p.summary = a->summary; p.qlen = a->qlen; p.klen = a->klen; p.sel = a->sel;
     p.B = a->B; p.Lq = a->Lq; p.Lk = a->Lk; p.Hq = a->Hq; p.Hk = a->Hk; p.D = a->D; p.block = a->block; p.qb = a->query_block;
     p.n = a->n_sel; p.sink = a->sink; p.local = a->local; p.causal = a->causal;
-    p.ng = (a->Lq + a->query_block - 1) / a->query_block;
+    p.ng = (a->Lq - 1) / a->query_block + 1;
     // groups of a workgroup: up to 16 (the columns of a matrix instruction) with at most 64 KB of scores, two workgroups a CU
     p.gpw = 65536 / (p.nb * 4);
     p.gpw = p.gpw > 16 ? 16 : p.gpw;

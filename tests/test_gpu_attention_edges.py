@@ -124,3 +124,30 @@ def test_frames_masked_by_their_distance(A, Lq, qb, D, at, dt):
     val, err = reference(q, k, v, sel, how)['out']
     assert 700 in at or torch.isfinite(val[:, :, 0]).all()
     within(A.block_attention(q.cuda(), k.cuda(), v.cuda(), sel.cuda(), **on_gpu(how)), val, err, 'out')
+
+
+# ------------------------------------------------------------------ sizes at the ends of 32 bits
+@pytest.mark.parametrize('block', [2 ** 31 - 1, 2 ** 31 - 64, 2 ** 30])
+def test_one_block_of_any_length(A, block):
+    """a block as long as a 32-bit number goes: all keys are its own"""
+    gen = torch.Generator().manual_seed(4)
+    q, k = randn(gen, 2, 9, 2, 16), randn(gen, 2, 100, 1, 16)
+    klen, qlen = torch.tensor([100, 3], dtype=torch.int32), torch.tensor([9, 5], dtype=torch.int32)
+    summ = A.block_summary(k.cuda(), block, klen.cuda())
+    val = O.summary(k, block, klen)
+    within(summ, val, O.U32 * val.abs() + 1e-15, 'summary')
+    for causal in (False, True):
+        for sink, local in ((0, 0), (1, 1), (0, 2)):
+            got = A.select_blocks(q.cuda(), summ, 2, block, 4, keys=100, causal=causal, qlen=qlen.cuda(), klen=klen.cuda(), sink=sink, local=local)
+            assert torch.equal(got.cpu(), O.select(q, summ.cpu(), 2, block, 4, 100, causal, qlen, klen, sink, local)), (causal, sink, local)
+    got = A.select_blocks(q.cuda(), summ, 2, block, 4)              # (keys: as many as the block)
+    assert torch.equal(got.cpu(), torch.tensor([0, -1], dtype=torch.int32).expand(2, 1, 3, 2))
+
+
+@pytest.mark.parametrize('newest', [2 ** 31 - 1, 2 ** 31 - 64, 500])
+def test_every_token_is_among_the_newest(A, newest):
+    gen = torch.Generator().manual_seed(6)
+    k, klen = randn(gen, 3, 500, 2, 64).cuda(), torch.tensor([500, 0, 65], dtype=torch.int32).cuda()
+    got, want = A.block_summary(k, 64, klen, newest=newest, out=torch.full((3, 8, 2, 64), 7.0).cuda()), A.block_summary(k, 64, klen)
+    for b, n in enumerate((8, 0, 2)):
+        assert torch.equal(got[b, :n], want[b, :n]) and (got[b, n:] == 7).all()
