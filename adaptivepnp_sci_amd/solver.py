@@ -367,10 +367,12 @@ class AdmmRun:
                 via_mosaic = True
             else:
                 ops.pm_pre_denoise(self.x, b_in, w, self.x_rgb, None, None, inv_rho, inv_tau, nsig)
+            gate = gate and (self.update_i < self.update_times or self.update_times < 0)
             if gate and self.denoiser == 'nonlocal_color':
                 from .nonlocal_prior import nonlocal_online_finetune
                 nonlocal_online_finetune(self.model, self.eng, net_in, self.y, self.Phi, nsig, self.lr_, self.update_per_iter, logf=self.logf)
-            elif gate and self.two_stage and (self.update_i < self.update_times or self.update_times < 0):
+                self.update_i += 1
+            elif gate and self.two_stage:
                 from .finetune import fastdvdnet_online_finetune
                 fastdvdnet_online_finetune(self.model, self.eng, net_in, self.y, self.Phi, nsig, self.lr_,
                                            self.update_per_iter, logf=self.logf,
