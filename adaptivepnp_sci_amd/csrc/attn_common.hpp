@@ -7,6 +7,7 @@ namespace scipnp {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2a __attribute__((ext_vector_type(2)));
 typedef float f32x4a __attribute__((ext_vector_type(4)));
 typedef float f32x16a __attribute__((ext_vector_type(16)));
 typedef short s16x4a __attribute__((ext_vector_type(4)));

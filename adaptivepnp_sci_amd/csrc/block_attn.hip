@@ -37,7 +37,7 @@ struct FwdCfg {
 // A workgroup holds `sets` sets of RW waves, each with work of its own: four waves a workgroup land one on each SIMD of a CU, where
 // workgroups of one or two leave some SIMDs with three waves and some with one.
 template <typename T, int DP, int RW, bool SAVE, bool LEAN>          // SAVE: out32 wanted (a training pass)
-__global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
+__global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW > 1) ? 3 : 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = FwdCfg<T, DP, RW, LEAN>;
     using Frag = typename Mat<T>::Frag;
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     int* const list = (int*)(smem + C::MAIN + C::KP);
     int* const nlist = list + a.n;
     const Bias bias = load_bias(a, lut, (float*)(smem + C::MAIN + C::KP + (a.n + 4) / 4 * 16), hk, tset, 64 * RW);
-    if (threadIdx.x == 0) *longest = 0;
+    if (threadIdx.x == 0) longest[0] = longest[1] = 0;
     if (rw == 0) {
         int c = 0;
         if (any) {
@@ -89,8 +89,7 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     ko.init(rw, lane, ks, a.D);
     vo.init(rw, lane, vs, a.D);
     __syncthreads();
-    // a bias of this key head masks (uniform; few tables do): its keys are masked like those behind the last visible one, and what they hold
-    // is kept out of the products tile by tile
+    // a bias of this key head masks (uniform; few tables do): its keys' scores are replaced, like those behind the last visible key
     bool masks = false;
     for (int i = lane; i < a.nbuckets * a.G; i += 64) masks |= bias.tbl[i] == -INFINITY;
     masks = __ballot(masks) != 0;
@@ -107,8 +106,7 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     }
     const T* const kb = (const T*)a.k + b * a.sk.b + hk * a.sk.h;
     const T* const vb = (const T*)a.v + b * a.sv.b + hk * a.sv.h;
-    int kpr = 0;
-    int blk = t_begin / tpb, off = (t_begin - blk * tpb) * KT;              // the next tile to ask for
+    int blk, off;                                         // the next tile to ask for
     auto next_key = [&]() -> int {
         const int key = __builtin_amdgcn_readfirstlane(list[blk]) * a.block + off;
         off += KT;
@@ -119,19 +117,22 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         const int there = min(KT, sq.klen - key0);
         ko.issue(kb + (long long)key0 * a.sk.t, there, ks, a.D, smem + buf * C::BYTES, rw);
         if constexpr (!ONE_V) vo.issue(vb + (long long)key0 * a.sv.t, there, vs, a.D, smem + (2 + buf) * C::BYTES, rw);
-        if (a.k_pos && tset < KT) {
-            int x = tset;
-            if constexpr (LEAN) asm volatile("" : "+v"(x));                  // (no address in registers between tiles)
-            kpr = x < there ? a.k_pos[(size_t)b * a.Lk + key0 + x] : 0;
-        }
+        if (a.k_pos && rw == 0) issue_positions(a.k_pos + (size_t)b * a.Lk + key0, there, kp_lds + buf * KT, lane);
     };
     const int far = 2 * a.maxd;                           // the two ends, where most tiles lie: their bias in registers
     const float bias_lo = a.nbuckets ? bias.tbl[bias.lut[0] * a.G + gl] : 0.f, bias_hi = a.nbuckets ? bias.tbl[bias.lut[far] * a.G + gl] : 0.f;
     Acc<T, DP> sums;
+    float m, l;
+    f32x16a o[NB];
+    // One pass, and a careful second one where the first left a sum that is no number: an infinity or a NaN among the values meets weights of
+    // zero (masked keys) and parts of a weight that are zero or negative, and 0 x inf is none.  The second pass has zeros in their
+    // place; they come behind it, to the rows that see their keys.  (The test costs 16 operations a column block; a look at the values of
+    // every masked tile costs a tenth of the tile.)
+    bool careful = false;
+    for (;; careful = true) {
     sums.zero();
-    float m = -INFINITY, l = 0.f;
-    bool spoilt = false;
-
+    m = -INFINITY, l = 0.f;
+    blk = t_begin / tpb, off = (t_begin - blk * tpb) * KT;
     int key0 = 0;
     if (count > 0) {
         key0 = next_key();
@@ -140,7 +141,6 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
     for (int t = 0; t < count; ++t) {
         const int buf = t & 1, cur = key0;
         int* const kp = kp_lds + buf * KT;
-        if (a.k_pos && tset < KT) kp[tset] = kpr;
         dma_wait<RW>();                                   // this tile has landed, and everyone is done with the other buffer
         if constexpr (ONE_V) vo.issue(vb + (long long)cur * a.sv.t, min(KT, sq.klen - cur), vs, a.D, smem + 2 * C::BYTES, rw);
         if (t + 1 < count) {
@@ -148,7 +148,13 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
             issue(key0, buf ^ 1);
         }
         const char* const kt = smem + buf * C::BYTES;
-        const char* const v_at = smem + (ONE_V ? 2 : 2 + buf) * C::BYTES;
+        char* const v_at = smem + (ONE_V ? 2 : 2 + buf) * C::BYTES;
+        if constexpr (!ONE_V) {
+            if (careful) {
+                scrub<T, DP, RW>(v_at, rw, lane);
+                dma_wait<RW>();
+            }
+        }
         // (a wave with products to issue goes before one in its softmax: 73.6 -> 69.5 us in training at 2 x 4096 tokens, 16 heads of 64)
         __builtin_amdgcn_s_setprio(1);
         f32x16a s = dma_rows<T, DP, LEAN>(kt, qf, lane);
@@ -158,32 +164,31 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         else vt.read(v_at, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
         const bool masked = masks || cur + KT - 1 > min_lim;
-        bool skip = false;
         float c = a.scale2, add = 0.f;
         if (dist >= 0 && a.nbuckets) add = !LEAN && dist == 0 ? bias_lo : !LEAN && dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
         if (dist < 0 || masked || c < 0.f) {              // the scores one by one
             if (dist < 0) {
-                float x[16];
-                tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x);
+                constexpr int N = LEAN ? 8 : 16;          // (half of them at a time takes fewer registers)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, x[r]);
+                for (int r0 = 0; r0 < 16; r0 += N) {
+                    float x[N];
+                    tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x, r0);
+                    // (a bias that masks, plus a score that is no number, would still be none)
+                    if (masks)
+#pragma unroll
+                        for (int r = 0; r < N; ++r) s[r0 + r] = x[r] == -INFINITY ? 0.f : s[r0 + r];
+#pragma unroll
+                    for (int r = 0; r < N; ++r) s[r0 + r] = fmaf(s[r0 + r], c, x[r]);
+                    if constexpr (LEAN) __builtin_amdgcn_sched_barrier(0);
+                }
             } else {
+                if (masks)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = add == -INFINITY ? 0.f : s[r];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, add);
             }
-            if (masks) {                                  // (a key that is not a number, plus minus infinity, would still be none)
-                int y = qp;
-                asm volatile("" : "+v"(y));               // (the biases are read again: no register holds them through the tiles of every call)
-                float x[16];
-                if (dist < 0) tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, y, gl, hi, x);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = (dist < 0 ? x[r] : add) == -INFINITY ? -INFINITY : s[r];
-            }
             if (masked) {
-                if (!LEAN && !vt.finite()) {                       // (what its values add comes behind the loop, key by key)
-                    spoilt = skip = true;
-                    vt.clear();
-                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = cur + tile_key(r, hi) <= lim ? s[r] : -INFINITY;
             }
@@ -211,32 +216,44 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         // P rounded to bf16 is off by 2^-8 of each probability, of the order of the output's own rounding; with out32 wanted it is
         // taken whole: delta = sum dO O enters every score's gradient, and the sums of dbias cancel down to its error
-        if constexpr (sizeof(T) == 4) {
-            if (skip) continue;
-        }
-        if constexpr (ONE_V) dma_wait_but<DmaOffsets<T, DP, RW>::N>(t + 1 < count);
-        if constexpr (LEAN) {
-            if (masked && !vt.template finite<false>()) {
-                spoilt = true;
-                continue;
+        if constexpr (ONE_V) {
+            dma_wait_but<DmaOffsets<T, DP, RW>::N>(t + 1 < count);
+            if (careful) {
+                scrub<T, DP, RW>(v_at, rw, lane);
+                dma_wait<RW>();
             }
         }
         __builtin_amdgcn_s_setprio(1);
         if constexpr (LEAN) vt.read(v_at, lane);
-        vt.template mma<SAVE ? 3 : 1>(s, sums);
+        const Weights<T, SAVE ? 3 : 1> w(s);
+        vt.mma(w, sums);
         if constexpr (LEAN && NB == 4) {
             vt.read(v_at, lane, 2);
-            vt.template mma<SAVE ? 3 : 1>(s, sums, 2);
+            vt.mma(w, sums, 2);
         }
         __builtin_amdgcn_s_setprio(0);
     }
     for (int t = count; t < trips; ++t) {                 // (the other sets' barriers)
         dma_wait<RW>();
         if constexpr (ONE_V) dma_wait<RW>();
+        if (careful) dma_wait<RW>();
     }
     l += __shfl_xor(l, 32, 64);
-    f32x16a o[NB];
     sums.blocks(o);
+    if (careful) break;
+    float none = 0.f;
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) none = fmaf(o[db][r], 0.f, none);
+    bool again = __ballot(live && none != 0.f && l - l == 0.f) != 0;          // (a row with a score that is no number is none in any case)
+    if constexpr (RW > 1) {                               // waves that share tiles go through them together
+        if (again && lane == 0) longest[1] = 1;
+        __syncthreads();
+        again = __builtin_amdgcn_readfirstlane(longest[1]) != 0;
+    }
+    if (!again) break;
+    }
     const Attn& z = late_args();                          // (what only the end needs is read again there: the loop's scalars fit the registers)
     if constexpr (LEAN) {                                 // (the row's place as well: no register holds it through the loop)
         int x = li;
@@ -247,12 +264,11 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
         head = hk * z.G + gl;
         live = there_is && row < R && tok < sq.qlen;
     }
-    // Tiles with masked keys and values that are not numbers: only rows that see a key take its value, by plain loads
-    if (spoilt) {
+    // Values that are no numbers, to the rows that see their keys, by plain loads
+    if (careful) {
         const T* const qr = (const T*)z.q + b * z.sq.b + tok * z.sq.t + head * z.sq.h;
         for (int t = t_begin; t < t_begin + count; ++t) {
             const int cur = __builtin_amdgcn_readfirstlane(list[t / tpb]) * z.block + t % tpb * KT, there = min(KT, sq.klen - cur);
-            if (!masks && cur + KT - 1 <= min_lim) continue;
             bool bad = false;
             for (int j = 0; j < there; ++j)
                 for (int d = lane; d < z.D; d += 64) bad |= !(fabsf((float)vb[(cur + j) * z.sv.t + d]) < INFINITY);
@@ -268,12 +284,14 @@ __global__ void __launch_bounds__(256, LEAN ? 3 : 2) block_attn_kernel(Attn a, i
                     if (add == -INFINITY) continue;
                 }
                 for (int d = 0; d < z.D; ++d) x = fmaf((float)kr[d], (float)qr[d], x);
-                x = fmaf(x, z.scale2, add);
-                const float p = __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
+                const float p = __builtin_amdgcn_exp2f(fmaf(x, z.scale2, add) - (m == -INFINITY ? 0.f : m));
                 each_four<T, DP>(hi, [&](int d, auto at) {
                     if (d >= z.D) return;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[at(e) >> 4][at(e) & 15] = fmaf(p, (float)vr[d + e], o[at(e) >> 4][at(e) & 15]);
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = (float)vr[d + e];
+                        o[at(e) >> 4][at(e) & 15] = fmaf(p, fabsf(v) < INFINITY ? 0.f : v, o[at(e) >> 4][at(e) & 15]);
+                    }
                 });
             }
         }

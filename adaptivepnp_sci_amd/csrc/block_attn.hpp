@@ -59,17 +59,24 @@ struct DmaTile {
     static constexpr int BYTES = KT * LC * 16;
     static constexpr int PIECES = BYTES / 1024;
 };
-constexpr unsigned DMA_NONE = 0xFFFFFF00u;                // an offset outside every descriptor
+constexpr unsigned DMA_NONE = 0x80000000u;                // an offset outside every descriptor, and so with a tile's rows added (token strides are below 2^26 bytes)
 
 // this lane's offsets of a wave's pieces (piece = first + i * step): row * stride + chunk * 16
 template <typename T, int DP, int STEP>
 struct DmaOffsets {
-    static constexpr int N = (DmaTile<T, DP>::PIECES + STEP - 1) / STEP;
-    unsigned off[N];
+    static constexpr int N = (DmaTile<T, DP>::PIECES + STEP - 1) / STEP, LC = DmaTile<T, DP>::LC;
+    // the swizzle repeats every 16 rows: pieces that far apart have one offset, but for those rows (held each for itself, the offsets of
+    // 128 bf16 columns would be four registers more than three waves a SIMD have)
+    static constexpr int period() {
+        int p = 1;
+        while (p < N && p * STEP * 64 % (16 * LC)) ++p;
+        return p;
+    }
+    static constexpr int P = period(), ROWS = P * STEP * 64 / LC;
+    unsigned off[P];
     __device__ __forceinline__ void init(int first, int lane, unsigned stride_bytes, int D) {
-        constexpr int LC = DmaTile<T, DP>::LC;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < P; ++i) {
             const int x = (first + i * STEP) * 64 + lane, row = x / LC, c = (x % LC) ^ swz<T, LC>(row);
             off[i] = c * Mat<T>::E < D && row < KT ? (unsigned)row * stride_bytes + 16u * c : DMA_NONE;
         }
@@ -81,12 +88,26 @@ struct DmaOffsets {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int piece = first + i * STEP;
+            unsigned at = off[i % P];
+            if (i >= P) {
+                asm volatile("" : "+v"(at));              // (or the compiler adds in front of the loop and holds the sums)
+                at += i / P * ROWS * stride_bytes;
+            }
             if (DmaTile<T, DP>::PIECES % STEP == 0 || piece < DmaTile<T, DP>::PIECES)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + 1024 * piece), 16, off[i], 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + 1024 * piece), 16, at, 0, 0, 0);
         }
 #endif
     }
 };
+
+// the positions of a tile's keys, the same way: `live` of 32, zeros behind them
+__device__ __forceinline__ void issue_positions(const int* base, int live, int* to, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (unsigned)live * 4u, 0x00020000);
+    asm volatile("" : "+v"(lane));                        // (no register holds the offset between tiles)
+    if (lane < KT) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 4, 4 * lane, 0, 0, 0);
+#endif
+}
 
 // score products: A B^T, A = row li of the tile.  read() brings the rows into registers (all reads under way at once), mma() multiplies
 template <typename T, int DP>
@@ -199,6 +220,35 @@ struct Acc {
                 }
     }
 };
+// P in front of a second product: bf16, PARTS numbers a weight (each what the ones before it left over); fp32, as it is
+template <typename T, int PARTS>
+struct Weights {
+    bf16x8 p[PARTS][2];
+    __device__ __forceinline__ explicit Weights(const f32x16a& x) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                f32x2a rest = {x[8 * k + i], x[8 * k + i + 1]};
+#pragma unroll
+                for (int n = 0; n < PARTS; ++n) {
+                    const bf16x2 y = __builtin_convertvector(rest, bf16x2);
+                    p[n][k][i] = y[0];
+                    p[n][k][i + 1] = y[1];
+                    if (n + 1 < PARTS) {                  // (their floats from the pair's bits: the compiler would convert each a second time)
+                        unsigned u = __builtin_bit_cast(unsigned, y);
+                        rest[0] -= __uint_as_float(u << 16);
+                        rest[1] -= __uint_as_float(u & 0xFFFF0000u);
+                    }
+                }
+            }
+    }
+};
+template <int PARTS>
+struct Weights<float, PARTS> {
+    const f32x16a& x;
+    __device__ __forceinline__ explicit Weights(const f32x16a& x_) : x(x_) {}
+};
 template <typename T, int DP, int PART = (DP + 31) / 32>   // PART: column blocks held at a time (bf16)
 struct ColTile {
     static constexpr int LC = DmaTile<T, DP>::LC, NB = PART;
@@ -289,75 +339,18 @@ struct ColTile {
                          : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]), "n"(0), "n"(DOWN), "n"(STEP), "n"(STEP + DOWN));
     }
 #endif
-    // No infinity and no NaN in the tile: a masked weight of 0 would carry it into rows that do not see it (0 x inf)
-    template <bool READ = true>
-    __device__ __forceinline__ bool finite() const {
-        float sum = 0.f;                                  // of x * 0
-#if defined(__HIP_DEVICE_COMPILE__)
-        if constexpr (sizeof(T) == 2 && !READ) {
-            const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
-#pragma unroll 2
-            for (int i = 0; i < DmaTile<T, DP>::PIECES; ++i) {
-                const bf16x8 x = *(const bf16x8*)(tile + i * 1024 + lane * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[2 * e], x[2 * e + 1]}, zero, sum, false);
-            }
-        } else if constexpr (sizeof(T) == 2) {
-            const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
-#pragma unroll
-            for (int db = 0; db < NB; ++db)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{u[db][k].v[2 * i], u[db][k].v[2 * i + 1]}, zero, sum, false);
-        } else {
-#pragma unroll 4
-            for (int i = 0; i < DmaTile<T, DP>::PIECES; ++i) {
-                const f32x4a x = *(const f32x4a*)(tile + i * 1024 + lane * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum = fmaf(x[e], 0.f, sum);
-            }
-        }
-#endif
-        return __ballot(sum != 0.f) == 0;
-    }
-    __device__ __forceinline__ void clear() {             // (bf16, where the columns are in registers)
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int db = 0; db < NB; ++db)
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) u[db][k].v[i] = (__bf16)0.f;
-        }
-    }
-    template <int PARTS = 1>
-    __device__ __forceinline__ void mma(const f32x16a& p, Acc<T, DP>& sums, int first = 0) const {
+    template <int PARTS>
+    __device__ __forceinline__ void mma(const Weights<T, PARTS>& w, Acc<T, DP>& sums, int first = 0) const {
         auto& acc = sums.x;
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                bf16x8 pb, p1, p2;
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = p[8 * k + i];
-                    pb[i] = (__bf16)x;
-                    if constexpr (PARTS > 1) {
-                        const float r1 = x - (float)pb[i];
-                        p1[i] = (__bf16)r1;
-                        if constexpr (PARTS > 2) p2[i] = (__bf16)(r1 - (float)p1[i]);
-                    }
-                }
+                for (int n = 0; n < PARTS; ++n)
 #pragma unroll
-                for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, pb, acc[first + db], 0, 0, 0);
-                if constexpr (PARTS > 1)
-#pragma unroll
-                    for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p1, acc[first + db], 0, 0, 0);
-                if constexpr (PARTS > 2)
-#pragma unroll
-                    for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, p2, acc[first + db], 0, 0, 0);
-            }
+                    for (int db = 0; db < NB; ++db) acc[first + db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[db][k].v, w.p[n][k], acc[first + db], 0, 0, 0);
         } else if constexpr (Acc<T, DP>::N16) {
+            const f32x16a& p = w.x;
             constexpr int NC = DP / 16;
             const int l = lane & 15, j = lane >> 4, first = (j & 1) + 4 * (j >> 1);
             const char* const base = tile + first * LC * 16 + 4 * (l & 3);
@@ -381,6 +374,7 @@ struct ColTile {
                 }
             }
         } else {
+            const f32x16a& p = w.x;
             constexpr int W = NB == 3 ? 1 : NB;            // floats of a read
             typedef float vec __attribute__((ext_vector_type(W == 1 ? 1 : W)));
             const int li = lane & 31, hi = lane >> 5;
@@ -413,6 +407,21 @@ struct ColTile {
         }
     }
 };
+// zeros in the place of the tile's infinities and NaN, a wave's pieces
+template <typename T, int DP, int STEP>
+__device__ __forceinline__ void scrub(char* tile, int first, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef T vec __attribute__((ext_vector_type(Mat<T>::E)));
+    asm volatile("" : "+v"(lane));                        // (no address of this stays in registers through the tiles of every call)
+    for (int i = first; i < DmaTile<T, DP>::PIECES; i += STEP) {
+        vec* const at = (vec*)(tile + i * 1024 + lane * 16);
+        vec x = *at;
+#pragma unroll
+        for (int e = 0; e < Mat<T>::E; ++e) x[e] = fabsf((float)x[e]) < INFINITY ? x[e] : (T)0.f;
+        *at = x;
+    }
+#endif
+}
 // the accumulators of a lane's row, four neighbouring columns at a time: f(column, values, block and register of each)
 template <typename T, int DP, typename F>
 __device__ __forceinline__ void each_four(int hi, F f) {
@@ -576,23 +585,25 @@ __device__ __forceinline__ int tile_distance(const Attn& a, RowRange q, int key0
     const int lo = clamp_dist(klo - q.hi, a.maxd), hi = clamp_dist(khi - q.lo, a.maxd);
     return lo == hi ? lo : -1;
 }
-// the bias of 16 scores of a lane's row, position by position
-__device__ __forceinline__ void tile_buckets(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int hi, int (&d)[16]) {
+// the bias of N of the 16 scores of a lane's row from the first-th on, position by position
+template <int N>
+__device__ __forceinline__ void tile_buckets(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int hi, int (&d)[N], int first = 0) {
     if (kp) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) d[r] = kp[tile_key(r, hi)];
+        for (int r = 0; r < N; ++r) d[r] = kp[tile_key(first + r, hi)];
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) d[r] = key0 + tile_key(r, hi);
+        for (int r = 0; r < N; ++r) d[r] = key0 + tile_key(first + r, hi);
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) d[r] = s.lut[clamp_dist(d[r] - qp, a.maxd)];
+    for (int r = 0; r < N; ++r) d[r] = s.lut[clamp_dist(d[r] - qp, a.maxd)];
 }
-__device__ __forceinline__ void tile_bias(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int gl, int hi, float (&x)[16]) {
-    int d[16];
-    tile_buckets(a, s, key0, kp, qp, hi, d);
+template <int N>
+__device__ __forceinline__ void tile_bias(const Attn& a, const Bias& s, int key0, const int* kp, int qp, int gl, int hi, float (&x)[N], int first = 0) {
+    int d[N];
+    tile_buckets(a, s, key0, kp, qp, hi, d, first);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = s.tbl[d[r] * a.G + gl];
+    for (int r = 0; r < N; ++r) x[r] = s.tbl[d[r] * a.G + gl];
 }
 inline size_t bias_lds(int nbuckets, int maxd, int G) { return (size_t)bias_lut_bytes(nbuckets, maxd) + ((size_t)nbuckets * G * 4 + 15) / 16 * 16; }
 

@@ -126,6 +126,27 @@ def test_frames_masked_by_their_distance(A, Lq, qb, D, at, dt):
     within(A.block_attention(q.cuda(), k.cuda(), v.cuda(), sel.cuda(), **on_gpu(how)), val, err, 'out')
 
 
+@pytest.mark.parametrize('save', [False, True])
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('times,B,Lq,Lk,Hq,Hk,D,qb,causal', [
+    (1, 1, 100, 300, 2, 1, 64, 16, False), (1, 2, 130, 130, 2, 2, 128, 32, True), (1, 1, 1, 900, 4, 1, 128, 1, False), (1, 1, 70, 130, 1, 1, 56, 64, False),
+    (90, 1, 130, 130, 8, 2, 128, 16, True), (90, 1, 140, 140, 4, 1, 96, 64, False), (60, 1, 130, 200, 4, 1, 128, 64, False),
+])
+def test_an_infinite_value_arrives_as_one(A, times, B, Lq, Lk, Hq, Hk, D, qb, causal, dt, save):
+    """infinities and NaN among values that are seen: in their columns, and in no other"""
+    gen, T = torch.Generator().manual_seed(Lq + Lk + D), DT[dt]
+    q, k, v = randn(gen, B, Lq, Hq, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T)
+    v[0, 0, 0, 1], v[0, Lk // 2, 0, 5], v[-1, 3, -1, D - 1] = math.inf, -math.inf, math.nan
+    how = dict(block=64, query_block=qb, scale=0.3 / math.sqrt(D), causal=causal, bucket_of=A.bucket_table(8, 40, not causal), bias=0.3 * randn(gen, 8, Hq))
+    sel = every_block(B, Hk, Lq, Lk, qb)
+    val, err = reference(q, k, v, sel, how)['out']
+    assert torch.isfinite(val).any() and torch.isinf(val).any() and torch.isnan(val).any()
+    got = A.block_attention(*(t.repeat(times, 1, 1, 1).cuda() for t in (q, k, v, sel)), save=save, **on_gpu(how))
+    got = got[0] if save else got
+    within(got[:B], val, err, 'out')
+    within(got[-B:], val, err, 'out of the last')
+
+
 # ------------------------------------------------------------------ sizes at the ends of 32 bits
 @pytest.mark.parametrize('block', [2 ** 31 - 1, 2 ** 31 - 64, 2 ** 30])
 def test_one_block_of_any_length(A, block):
