@@ -81,13 +81,16 @@ def weigh(P, V, mask):
     return torch.stack([P[i, m] @ V[m] for i, m in enumerate(mask)])
 
 
-def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None, bias=None, q_pos=None, k_pos=None, dout=None):
+def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None, bias=None, q_pos=None, k_pos=None, dout=None,
+              parts=1):
     """float64 results and element-wise bounds of the error of a computation whose products and sums are fp32 and whose probabilities
-    and score gradients are rounded to the inputs' type in front of the second products:
+    and score gradients are held in `parts` numbers of the inputs' type in front of the second products (each rounds what the ones
+    before it left over):
     {name: (value, bound)} of out, lse, and with dout dq, dk, dv, dbias."""
     B, Lq, Hq, D = q.shape
     Lk, Hk = k.shape[1:3]
     G, u = Hq // Hk, U[q.dtype]
+    up = u ** parts if q.dtype != torch.float32 else 0.0
     z = lambda *s: torch.zeros(*s, dtype=torch.float64)  # noqa: E731
     names = {'out': z(*q.shape), 'lse': torch.full((B, Hq, Lq), -math.inf, dtype=torch.float64)}
     if dout is not None:
@@ -129,7 +132,7 @@ def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None
             eP = 2 * worst + (n + 16) * U32                                    # relative, of a probability (its sum included)
             O, A = weigh(P, V, mask), weigh(P, V.abs(), mask)
             val['out'][b, :ql, h] = O
-            err['out'][b, :ql, h] = A * (u * (q.dtype != torch.float32) + eP + (n + 16) * U32) + u * O.abs()
+            err['out'][b, :ql, h] = A * (up + eP + (n + 16) * U32) + u * O.abs()
             val['lse'][b, h, :ql] = torch.where(some, top[:, 0] + L[:, 0].log(), torch.tensor(-math.inf, dtype=torch.float64))
             err['lse'][b, h, :ql] = (eP[:, 0] + 16 * U32 * (1 + top[:, 0].abs() + L[:, 0].log().abs()))
             if dout is None:
@@ -143,14 +146,14 @@ def attention(q, k, v, sel, block, qb, scale, causal, qlen, klen, bucket_of=None
             el = (err['lse'][b, h, :ql] + 4 * U32 * val['lse'][b, h, :ql].abs().masked_fill(~some, 0.0))[:, None]
             eQ = eP + el + 4 * U32 * S.abs().masked_fill(~mask, 0.0)           # P again, from lse
             eD = P * e_in + (eQ + 4 * U32) * dS.abs()
-            eT = eD + (u if q.dtype != torch.float32 else 0.0) * dS.abs()      # rounded in front of the product
+            eT = eD + up * dS.abs()      # rounded in front of the product
             rows = ql + 16
             val['dq'][b, :ql, h] = dS @ K * scale
             err['dq'][b, :ql, h] = abs(scale) * ((eT + (n + 16) * U32 * dS.abs()) @ K.abs()) + u * (dS @ K * scale).abs()
             val['dk'][b, :, c] += dS.T @ Q * scale
             err['dk'][b, :, c] += abs(scale) * ((eT + G * rows * U32 * dS.abs()).T @ Q.abs())
             val['dv'][b, :, c] += P.T @ g
-            err['dv'][b, :, c] += (P * (eQ + (u if q.dtype != torch.float32 else 0.0) + G * rows * U32)).T @ g.abs()
+            err['dv'][b, :, c] += (P * (eQ + up + G * rows * U32)).T @ g.abs()
             if bias is not None:
                 eB = eD + (n + 16) * U32 * dS.abs()
                 for i in range(bias.shape[0]):

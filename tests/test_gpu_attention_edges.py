@@ -172,3 +172,27 @@ def test_every_token_is_among_the_newest(A, newest):
     got, want = A.block_summary(k, 64, klen, newest=newest, out=torch.full((3, 8, 2, 64), 7.0).cuda()), A.block_summary(k, 64, klen)
     for b, n in enumerate((8, 0, 2)):
         assert torch.equal(got[b, :n], want[b, :n]) and (got[b, n:] == 7).all()
+
+
+# ------------------------------------------------------------------ the digits of the weights
+DIGITS = [  # times, B, Lq, Lk, Hq, Hk, D, qb, causal
+    (1, 1, 96, 257, 4, 1, 64, 16, False), (1, 2, 130, 130, 2, 2, 128, 16, True), (1, 1, 3, 700, 8, 2, 128, 1, True), (1, 1, 1, 1500, 4, 1, 40, 1, False),
+    (1, 1, 200, 200, 1, 1, 96, 64, False), (90, 1, 130, 130, 8, 2, 128, 16, True), (90, 1, 140, 140, 4, 1, 96, 64, False),
+]
+
+
+@pytest.mark.parametrize('times,B,Lq,Lk,Hq,Hk,D,qb,causal', DIGITS)
+def test_bf16_weights_keep_sixteen_digits(A, times, B, Lq, Lk, Hq, Hk, D, qb, causal):
+    """only the result is rounded to bf16: where the values cancel, a weight of eight digits is off by far more than that.  Two bf16 numbers
+    hold a weight to 2^-8 of 2^-8 of it (half a step of what the first left over)"""
+    gen, T = torch.Generator().manual_seed(Lq + D), torch.bfloat16
+    q, k, v = randn(gen, B, Lq, Hq, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T), randn(gen, B, Lk, Hk, D, dtype=T)
+    how = dict(block=64, query_block=qb, scale=0.5 / math.sqrt(D), causal=causal, bucket_of=A.bucket_table(8, 20, not causal), bias=randn(gen, 8, Hq))
+    sel = every_block(B, Hk, Lq, Lk, qb)
+    val, err = reference(q, k, v, sel, how, parts=2)['out']
+    args = [t.repeat(times, 1, 1, 1).cuda() for t in (q, k, v, sel)]
+    for save in (False, True):
+        got = A.block_attention(*args, save=save, **on_gpu(how))
+        got = got[0] if save else got
+        within(got[:B], val, err, f'out, save {save}')
+        within(got[-B:], val, err, f'out of the last, save {save}')
