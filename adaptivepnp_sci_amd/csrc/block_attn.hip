@@ -19,16 +19,17 @@
 
 namespace scipnp {
 
-// LEAN, bf16 of 96 and 128 columns: three waves a SIMD instead of two (381 instead of 406 us for the first case above; 139
-// instead of 155 at 8192 queries of 32 heads of 96 in groups of 16).  V is read behind the softmax, 64 columns at a time, which saves the
-// registers; and of V there is one buffer where only two waves share a pair of tiles, which saves the LDS: it is asked for when its
-// tile's scores begin.  Not where there is no third workgroup for a CU (52 us instead of 49 at 4096 queries of 16 heads of 128), nor
-// with P in three parts of 128 columns (30 registers would go to scratch in the loop), nor for one wave a set (LDS).
+// LEAN, bf16 of 96 and 128 columns and two waves a pair of tiles: three waves a SIMD instead of two (189 instead of 197 us at 8192 queries of
+// 32 heads of 96 in groups of 16, 464 instead of 469 for the first case above).  V is read behind the softmax, 64 columns at a time, which
+// saves the registers, and there is one buffer of V, which saves the LDS: it is asked for when its tile's scores begin.  Not where
+// there is no third workgroup for a CU (52 us instead of 49 at 4096 queries of 16 heads of 128), nor with P in three parts of 128 columns (30
+// registers would go to scratch in the loop), nor for one wave a set (LDS), nor for four (101 us instead of 95 at 8192 queries of 16 heads of 96 in
+// groups of 64).
 template <typename T, int DP, int RW, bool SAVE>
-constexpr bool can_be_lean() { return sizeof(T) == 2 && DP > 64 && RW > 1 && !(SAVE && DP == 128); }
+constexpr bool can_be_lean() { return sizeof(T) == 2 && DP > 64 && RW == 2 && !(SAVE && DP == 128); }
 template <typename T, int DP, int RW, bool LEAN>
 struct FwdCfg {
-    static constexpr bool ONE_V = LEAN && RW == 2;
+    static constexpr bool ONE_V = LEAN;
     static constexpr int BYTES = DmaTile<T, DP>::BYTES;
     static constexpr int MAIN = (ONE_V ? 3 : 4) * BYTES;                      // two K, one or two V
     static constexpr int KP = 2 * KT * 4;
@@ -455,7 +456,7 @@ static int fwd_launch(const Attn& p, hipStream_t st) {
 template <typename T, int DP, int RW, bool SAVE>
 static int fwd_pick(const Attn& p, hipStream_t st) {
     if constexpr (can_be_lean<T, DP, RW, SAVE>()) {        // (more than two workgroups of four waves for each of 256 CUs)
-        if ((long long)p.B * p.Hk * p.ng * p.chunks * p.splits > 512 * (4 / RW)) return fwd_launch<T, DP, RW, SAVE, true>(p, st);
+        if ((long long)p.B * p.Hk * p.ng * p.chunks * p.splits > 512 * 2) return fwd_launch<T, DP, RW, SAVE, true>(p, st);
     }
     return fwd_launch<T, DP, RW, SAVE, false>(p, st);
 }
