@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
         }
         __builtin_amdgcn_s_setprio(1);
         if constexpr (LEAN) kc.read(kt, lane);
-        kc.mma(Weights<T, 2>(s), sums);                      // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
+        kc.mma(Weights<T, 2>(s), sums);                   // (dS in 16 bits: its rows sum to zero, so a rounding to 8 weighs more than the result's own)
         __builtin_amdgcn_s_setprio(0);
     }
     for (int t = count; t < trips; ++t) dma_wait<RW>();   // (the other sets' barriers)
@@ -591,9 +591,9 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) 
         }
         __builtin_amdgcn_s_setprio(1);
         if constexpr (LATE) gc.read(at + BYTES, lane);
-        gc.mma(Weights<T, 1>(s), vacc);
+        gc.mma(Weights<T, 2>(s), vacc);                   // (bf16: P and dS in 16 bits, as in the pass for dQ; with 8 the gradients were 1.4 x as far off)
         if constexpr (LATE) qc.read(at, lane);
-        qc.mma(Weights<T, 1>(dp), kacc);
+        qc.mma(Weights<T, 2>(dp), kacc);
         __builtin_amdgcn_s_setprio(0);
     }
     f32x16a dk[NB], dv[NB];

@@ -196,3 +196,16 @@ def test_bf16_weights_keep_sixteen_digits(A, times, B, Lq, Lk, Hq, Hk, D, qb, ca
         got = got[0] if save else got
         within(got[:B], val, err, f'out, save {save}')
         within(got[-B:], val, err, f'out of the last, save {save}')
+
+
+@pytest.mark.parametrize('B,Lq,Lk,Hq,Hk,D,qb,causal', [c[1:] for c in DIGITS[:5]])
+def test_bf16_gradients_keep_sixteen_digits(A, B, Lq, Lk, Hq, Hk, D, qb, causal):
+    gen, T = torch.Generator().manual_seed(Lq + D), torch.bfloat16
+    q, k, v, g = (randn(gen, B, L, h, D, dtype=T) for L, h in ((Lq, Hq), (Lk, Hk), (Lk, Hk), (Lq, Hq)))
+    how = dict(block=64, query_block=qb, scale=0.5 / math.sqrt(D), causal=causal, bucket_of=A.bucket_table(8, 20, not causal), bias=randn(gen, 8, Hq))
+    sel = every_block(B, Hk, Lq, Lk, qb)
+    want = reference(q, k, v, sel, how, dout=g, parts=2)
+    args = [t.cuda() for t in (q, k, v, sel)]
+    _, saved = A.block_attention(*args, save=True, **on_gpu(how))
+    for name, t in zip(('dq', 'dk', 'dv', 'dbias'), A.block_attention_backward(g.cuda(), *args, saved, **on_gpu(how))):
+        within(t, *want[name], name)
