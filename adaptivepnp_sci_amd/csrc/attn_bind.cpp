@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <cmath>
 #include <string>
@@ -146,6 +147,18 @@ const Tensor& needed(PyObject* o, const char* name) {
     if (!t) refuse(PyExc_ValueError, "%s is missing", name);
     return *t;
 }
+// A given result must not have places that are one in memory, nor share memory with what the call reads or writes elsewhere: rows are read and
+// written in any order.  (Views that interleave are told apart by nobody cheaply: only overlaps that are certain are refused.)
+bool in_place(const Tensor& a, const Tensor& b) { return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides(); }
+void apart(const Tensor* out, const char* name, const Tensor* other, const char* other_name) {
+    if (!out || !other || !out->numel() || !other->numel()) return;
+    const auto s = at::get_overlap_status(*out, *other);
+    if (out->data_ptr() == other->data_ptr() || s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+        refuse(PyExc_ValueError, "%s shares memory with %s", name, other_name);
+}
+void single(const Tensor* out, const char* name) {
+    if (out && at::has_internal_overlap(*out) == at::MemOverlap::Yes) refuse(PyExc_ValueError, "%s has several places in one memory location (an expanded tensor)", name);
+}
 int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? SCIPNP_F32 : SCIPNP_BF16; }
 Tensor new_bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
@@ -201,6 +214,15 @@ PyObject* head_norm_rotate(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const Tensor *out_q = given(o[8], "out_q"), *out_k = given(o[9], "out_k"), *v = given(o[10], "v"), *out_v = given(o[11], "out_v"), *slots = given(o[12], "slots");
     if (slots && !out_k) refuse(PyExc_ValueError, "slots need out_k (a cache)");
     if (v && !out_v) refuse(PyExc_ValueError, "v needs out_v");
+    const struct { const Tensor *out, *in; const char *name, *in_name; } own[] = {{out_q, &q, "out_q", "q"}, {out_k, k, "out_k", "k"}, {v ? out_v : nullptr, v, "out_v", "v"}};
+    for (int i = 0; i < 3; ++i) {
+        single(own[i].out, own[i].name);
+        for (int j = 0; j < 3; ++j) {
+            if (i != j) apart(own[i].out, own[i].name, own[j].in, own[j].in_name);
+            else if (own[i].out && own[i].in && !(i && slots) && !in_place(*own[i].out, *own[i].in)) apart(own[i].out, own[i].name, own[i].in, own[i].in_name);
+            if (j < i) apart(own[i].out, own[i].name, own[j].out, own[j].name);
+        }
+    }
     Norm c(call, q, k, o[2], o[3], o[4], o[5], o[6], o[7]);
     scipnp_head_norm_args& a = c.a;
     Tensor new_q, new_k;
@@ -270,6 +292,7 @@ PyObject* block_summary(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (block < 1 || newest < 0) refuse(PyExc_ValueError, "block %d must be positive, newest %d not negative", block, newest);
     const Tensor *klen = given(o[2], "klen"), *out = given(o[4], "out");
     if (newest && !out) refuse(PyExc_ValueError, "newest needs out");
+    apart(out, "out", &k, "k");
     const Tokens t = tokens(k, "k");
     const int64_t shape[4] = {k.size(0), (k.size(1) + block - 1) / block, k.size(2), k.size(3)};
     const int32_t* const kl = (const int32_t*)array(klen, "klen", {k.size(0)}, at::kInt);
@@ -375,8 +398,12 @@ struct Attention {
 // (the fourteen of Attention, out, save)
 PyObject* block_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     ENTER(16)
-    Attention c(call, o);
     const Tensor* out = given(o[14], "out");
+    single(out, "out");
+    apart(out, "out", given(o[1], "k"), "k");
+    apart(out, "out", given(o[2], "v"), "v");
+    if (const Tensor* const q = given(o[0], "q"); q && out && !in_place(*out, *q)) apart(out, "out", q, "q");
+    Attention c(call, o);
     Tensor made, lse, rest, out32;
     if (out) call.on_device(*out, "out");
     else made = at::empty_like(c.q), out = &made, c.a.zero_rest = 1;

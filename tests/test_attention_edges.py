@@ -41,3 +41,38 @@ def test_heads_are_counted_in_64_bits(lib):
     a = _lib.BlockAttnArgs(dtype=1, B=1, Lq=1, Lk=64, Hq=1 << 26, Hk=1, D=64, block=64, query_block=1, n_sel=1, scale=1.0, q=P, k=P, v=P, out=P, sel=P,
                            num_buckets=64, max_distance=4, bias=P, bucket_of=P, q_stride=st, k_stride=st, v_stride=st, out_stride=st)
     refused(lib, lib.scipnp_block_attn(C.byref(a), None), 'at most 2048')
+
+
+# ------------------------------------------------------------------ results that share memory
+def test_results_in_the_memory_of_something_else_are_refused():
+    import torch
+    from adaptivepnp_sci_amd import attention as A
+    q, k, v, w = torch.zeros(2, 64, 2, 64), torch.zeros(2, 64, 2, 64), torch.zeros(2, 64, 2, 64), torch.ones(64)
+    sel = torch.zeros(2, 2, 16, 1, dtype=torch.int32)
+    flat = torch.zeros(2 * 64 * 2 * 64 + 64)
+    part = flat[64:].view(2, 64, 2, 64)                           # overlaps flat[:-64] by all but a row
+    whole = flat[:-64].view(2, 64, 2, 64)
+    one = torch.zeros(2, 1, 2, 64).expand(2, 64, 2, 64)
+    for call, word in (
+            (lambda: A.block_attention(q, k, v, sel, query_block=4, out=k), 'out shares memory with k'),
+            (lambda: A.block_attention(q, k, v, sel, query_block=4, out=v), 'out shares memory with v'),
+            (lambda: A.block_attention(part, k, v, sel, query_block=4, out=whole), 'out shares memory with q'),
+            (lambda: A.block_attention(q, k, v, sel, query_block=4, out=one), 'out has several places'),
+            (lambda: A.block_attention(q, part, v, sel, query_block=4, out=whole), 'out shares memory with k'),
+            (lambda: A.head_norm_rotate(q, k, w, w, out_q=k), 'out_q shares memory with k'),
+            (lambda: A.head_norm_rotate(q, k, w, w, out_k=q), 'out_k shares memory with q'),
+            (lambda: A.head_norm_rotate(q, k, w, w, out_q=v, out_k=v), 'out_k shares memory with out_q'),
+            (lambda: A.head_norm_rotate(part, None, w, out_q=whole), 'out_q shares memory with q'),
+            (lambda: A.head_norm_rotate(q, None, w, out_q=one), 'out_q has several places'),
+            (lambda: A.head_norm_rotate(q, k, w, w, out_k=torch.zeros_like(k), v=v, out_v=k), 'out_v shares memory with k'),
+            (lambda: A.head_norm_rotate(q, k, w, w, out_k=v, v=v, out_v=torch.zeros_like(v)), 'out_k shares memory with v'),
+            (lambda: A.head_norm_rotate(q, k[:, :1], w, w, out_k=v, v=v[:, :1], out_v=k, slots=torch.zeros(2, 1, dtype=torch.int32)), 'shares memory'),
+            (lambda: (lambda t: A.block_summary(t, 1, out=t))(torch.zeros(1, 64, 1, 8)), 'out shares memory with k')):
+        with pytest.raises((ValueError, _lib.ScipnpError), match=word):
+            call()
+    packed = torch.zeros(2, 64, 6, 64)                            # views of one projection, in place: not refused for their memory
+    for call in (lambda: A.head_norm_rotate(packed[:, :, :2], packed[:, :, 2:4], w, w, out_q=packed[:, :, :2], out_k=packed[:, :, 2:4]),
+                 lambda: A.block_attention(packed[:, :, :2], packed[:, :, 2:4], packed[:, :, 4:], sel, query_block=4, out=packed[:, :, :2]),
+                 lambda: A.head_norm_rotate(q, k, w, w, out_q=q, out_k=k, v=v, out_v=v)):
+        with pytest.raises(_lib.ScipnpError, match='no CPU fallback'):
+            call()

@@ -209,3 +209,23 @@ def test_bf16_gradients_keep_sixteen_digits(A, B, Lq, Lk, Hq, Hk, D, qb, causal)
     _, saved = A.block_attention(*args, save=True, **on_gpu(how))
     for name, t in zip(('dq', 'dk', 'dv', 'dbias'), A.block_attention_backward(g.cuda(), *args, saved, **on_gpu(how))):
         within(t, *want[name], name)
+
+
+# ------------------------------------------------------------------ results in place
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('Lq,Lk,qb', [(150, 150, 16), (2, 2000, 1)])
+def test_results_in_the_queries_own_memory(A, Lq, Lk, qb, dt):
+    """views of one projection, written in place: keys split over workgroups, and not"""
+    gen, T = torch.Generator().manual_seed(Lq), DT[dt]
+    packed = randn(gen, 2, Lq, 6, 64, dtype=T).cuda()
+    k, v = randn(gen, 2, Lk, 2, 64, dtype=T).cuda(), randn(gen, 2, Lk, 2, 64, dtype=T).cuda()
+    q = packed[:, :, 1:5]
+    sel, how = every_block(2, 2, Lq, Lk, qb).cuda(), dict(block=64, query_block=qb, causal=True)
+    want, before = A.block_attention(q, k, v, sel, **how), packed.clone()
+    assert A.block_attention(q, k, v, sel, out=q, **how) is q
+    assert torch.equal(q, want) and torch.equal(packed[:, :, [0, 5]], before[:, :, [0, 5]])
+    w, turns = torch.ones(64).cuda(), A.rotary_turns(32, device='cuda')
+    a, b = packed[:, :, :4], packed[:, :, 4:]
+    wa, wb = A.head_norm_rotate(a, b, w, w, turns)
+    A.head_norm_rotate(a, b, w, w, turns, out_q=a, out_k=b)
+    assert torch.equal(a, wa) and torch.equal(b, wb)
