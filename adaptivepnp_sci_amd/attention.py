@@ -16,6 +16,10 @@ cache); q has Hq heads, k and v Hk, Hq a multiple of Hk.  float32 inputs are mul
 softmax statistics are fp32 or fp64 in either type.  Sequence b has qlen[b] queries and klen[b] keys (int32, None: all); query i
 stands at key position klen - qlen + i, so a cache with one new token needs klen only.  Every call is asynchronous on the current
 stream of the tensors' device, allocates its workspace from torch, gives the same bits for the same inputs, and can be captured.
+
+Like every kernel of this package the calls are outside autograd: results require no gradient whatever the inputs do, forward-mode tangents
+are dropped, and the *_backward functions are called by hand or from a torch.autograd.Function of the program.  A given result that is
+written raises its version counter, so autograd refuses a backward pass that had saved what was there.
 """
 import ctypes as C
 import importlib

@@ -159,6 +159,10 @@ void apart(const Tensor* out, const char* name, const Tensor* other, const char*
 void single(const Tensor* out, const char* name) {
     if (out && at::has_internal_overlap(*out) == at::MemOverlap::Yes) refuse(PyExc_ValueError, "%s has several places in one memory location (an expanded tensor)", name);
 }
+// a given result was written: autograd notices where it had saved what was there
+void written(const Tensor* out) {
+    if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
 int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? SCIPNP_F32 : SCIPNP_BF16; }
 Tensor new_bytes(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
@@ -249,6 +253,7 @@ PyObject* head_norm_rotate(PyObject*, PyObject* const* o, Py_ssize_t n) {
     }
     const scipnp_stream_t st = call.stream();
     done(WITHOUT_GIL(head_norm(&a, st)), "scipnp_head_norm_rotate");
+    written(out_q), written(out_k), written(v ? out_v : nullptr);
     return Py_BuildValue("NN", o[8] == Py_None ? wrap(new_q) : back(o[8]), !k ? back(Py_None) : o[9] == Py_None ? wrap(new_k) : back(o[9]));
     LEAVE
 }
@@ -304,6 +309,7 @@ PyObject* block_summary(PyObject*, PyObject* const* o, Py_ssize_t n) {
     float* const p = (float*)array(out, "out", shape, at::kFloat);
     const scipnp_stream_t st = call.stream();
     done(WITHOUT_GIL(summary_fn(t.p, t.s, type_of(k), kl, p, (int)k.size(0), (int)k.size(1), (int)k.size(2), (int)k.size(3), block, newest, st)), "scipnp_block_summary");
+    written(out);
     return o[4] == Py_None ? wrap(made) : back(o[4]);
     LEAVE
 }
@@ -416,6 +422,7 @@ PyObject* block_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     const Tensor ws = c.workspace(0);
     const scipnp_stream_t st = call.stream();
     done(WITHOUT_GIL(attn_fn(&c.a, st)), "scipnp_block_attn");
+    written(out);
     PyObject* const r = o[14] == Py_None ? wrap(made) : back(o[14]);
     return save ? Py_BuildValue("N(NNN)", r, wrap(lse), wrap(out32), wrap(rest)) : r;
     LEAVE

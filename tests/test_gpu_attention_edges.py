@@ -229,3 +229,25 @@ def test_results_in_the_queries_own_memory(A, Lq, Lk, qb, dt):
     wa, wb = A.head_norm_rotate(a, b, w, w, turns)
     A.head_norm_rotate(a, b, w, w, turns, out_q=a, out_k=b)
     assert torch.equal(a, wa) and torch.equal(b, wb)
+
+
+# ------------------------------------------------------------------ beside autograd
+def test_results_beside_autograd(A):
+    """results require no gradient; a given one that autograd had saved is noticed"""
+    w = torch.ones(64, device='cuda', requires_grad=True)
+    q, k = (torch.randn(1, 64, 2, 64, device='cuda', requires_grad=True) for _ in range(2))
+    sel = every_block(1, 2, 64, 64, 16).cuda()
+    results = [*A.head_norm_rotate(q, k, w, w), A.block_summary(k), A.block_attention(q, k, k, sel, query_block=16),
+               *A.block_attention(q, k, k, sel, query_block=16, save=True)[1]]
+    assert not any(t.requires_grad for t in results)
+    for write in (lambda t: A.head_norm_rotate(q, k, w, w, out_q=t), lambda t: A.head_norm_rotate(q, k, w, w, out_k=t),
+                  lambda t: A.head_norm_rotate(q, k, w, w, out_k=torch.empty_like(t), v=k, out_v=t),
+                  lambda t: A.block_attention(q, k, k, sel, query_block=16, out=t), lambda t: A.block_summary(k, 1, out=t)):
+        t = torch.zeros(1, 64, 2, 64, device='cuda')
+        loss = (t * q).sum()                              # (saves t for the gradient of q)
+        write(t)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()
+    with torch.inference_mode():
+        t = torch.zeros(1, 64, 2, 64, device='cuda')
+    assert A.block_attention(q, k, k, sel, query_block=16, out=t) is t and torch.equal(t, results[3])
