@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <torch/version.h>
 #include <cmath>
 #include <string>
 #include "../../include/scipnp.h"
@@ -471,4 +472,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attn_bind", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__attn_bind(void) { return PyModule_Create(&module); }
+// (built_for: a tensor's layout in memory is that of the torch whose headers this saw)
+PyMODINIT_FUNC PyInit__attn_bind(void) {
+    PyObject* const m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", TORCH_VERSION) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

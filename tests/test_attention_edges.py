@@ -76,3 +76,22 @@ def test_results_in_the_memory_of_something_else_are_refused():
                  lambda: A.head_norm_rotate(q, k, w, w, out_q=q, out_k=k, v=v, out_v=v)):
         with pytest.raises(_lib.ScipnpError, match='no CPU fallback'):
             call()
+
+
+# ------------------------------------------------------------------ the build
+def test_the_libraries_build_without_python(tmp_path):
+    """a C host has no torch: plain make asks for the libraries alone there, and for the Python module as well where it can be built"""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(_lib.__file__), 'csrc')
+    for python, built in (('false', False), ('python3', True)):
+        r = subprocess.run(['make', '-n', '-C', csrc, f'PYTHON={python}', f'BIND_OUT={tmp_path}/none.so'], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, r.stderr
+        assert ('-ltorch_python' in r.stdout) == built, r.stdout
+
+
+def test_a_module_of_another_torch_is_refused(monkeypatch):
+    from adaptivepnp_sci_amd import attention as A
+    monkeypatch.setattr(A.torch, '__version__', '1.0.0+other')
+    with pytest.raises(_lib.ScipnpError, match='built for torch'):
+        A._bind()
