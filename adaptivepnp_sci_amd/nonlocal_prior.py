@@ -85,6 +85,8 @@ class NonLocalEngine:
     def forward(self, frames, sigma, save=False):
         """frames planar (B,3,H,W) -> denoised planar (B,3,H,W), owned by the engine and overwritten by the next call.  save: also what
         the backward pass needs (a single clip)"""
+        if tuple(frames.shape) != tuple(self.out.shape):
+            raise ValueError(f'frames must be {tuple(self.out.shape)}, got {tuple(frames.shape)}')
         ops.patch_tokens(frames, self.tokens, self.units, self.shifts, LIFT)
         A.head_norm_rotate(self.tokens, self.tokens, self.wq, self.wk, eps=_EPS, out_q=self.q, out_k=self.k)
         A.block_summary(self.k, self.block, out=self.summary)
@@ -112,14 +114,22 @@ def nonlocal_online_finetune(model, eng, frames, y_pm, Phi_pm, sigma, lr_, updat
     input `frames` (B,3,H,W), the loss of the network denoisers' online finetunes; y_pm [4][M][N], Phi_pm [B][4][M][N] plane-major.
     The module's parameters and the engine's are the updated ones afterwards; a new Adam each event."""
     from . import finetune as F
-    _lib.require_gpu()
     if eng.units != 1:
         raise ValueError('the finetune needs weights of its own for every clip: one unit')
+    M, N = eng.H // 2, eng.W // 2
+    if eng.H % 2 or eng.W % 2:
+        raise ValueError(f'{eng.H}x{eng.W} frames have no whole Bayer cells: the finetune needs even sizes')
+    for name, t, shape in (('frames', frames, (eng.B, 3, eng.H, eng.W)), ('y_pm', y_pm, (4, M, N)), ('Phi_pm', Phi_pm, (eng.B, 4, M, N))):
+        if tuple(t.shape) != shape or t.dtype != F32 or not t.is_contiguous():
+            raise ValueError(f'{name} must be contiguous float32 {shape}, got {t.dtype} {tuple(t.shape)} contiguous={t.is_contiguous()}')
+        if t.device != eng.out.device:
+            raise ValueError(f'{name} is on {t.device}, the engine on {eng.out.device}')
+    _lib.require_gpu()
     if update_per_iter <= 0:
         return model
     lib = _lib.load()
     nblocks = C.c_int(0)
-    size = (eng.H // 2, eng.W // 2, eng.B, C.byref(nblocks))
+    size = (M, N, eng.B, C.byref(nblocks))
     _lib.check(lib.scipnp_fastdvd_loss_grad(None, None, None, None, None, *size, None), 'size')
     part = torch.empty(nblocks.value, dtype=torch.float64, device=eng.device)
     dout, (m, v) = torch.empty_like(eng.out), (torch.zeros_like(eng.flat) for _ in range(2))

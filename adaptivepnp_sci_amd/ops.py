@@ -680,8 +680,21 @@ def fastdvd_noisy_input(v, noise_f64):
     return out
 
 
+def _patch_shapes(frames, tokens, units, shifts):
+    """the kernels trust the sizes of `frames` for both tensors"""
+    if frames.dim() != 4 or frames.shape[1] != 3:
+        raise ValueError(f'frames must be (B,3,H,W), got {tuple(frames.shape)}')
+    B, _, H, W = frames.shape
+    if units > 0 and B % units == 0 and shifts in (1, 2, 4):          # (the entry refuses others)
+        more = 2 if shifts > 1 else 0
+        shape = (units * shifts, B // units * -(-(H + more) // 32) * -(-(W + more) // 32) * 64, 1, 56)
+        if tuple(tokens.shape) != shape:
+            raise ValueError(f'tokens of {B} frames of {H}x{W} in {units} clips, {shifts} grids: shape {shape}, got {tuple(tokens.shape)}')
+
+
 def patch_tokens(frames, tokens, units, shifts, constant, scale=1.0, replicate=True):
     """planar frames (B,3,H,W) -> patch tokens (units * shifts, L, 1, 56) of the non-local prior (nonlocal_prior.py)"""
+    _patch_shapes(frames, tokens, units, shifts)
     B, _, H, W = frames.shape
     _call('scipnp_patch_tokens', _p(frames, 'frames'), _p(tokens, 'tokens'), B, H, W, units, shifts, float(constant), float(scale), int(replicate), _stream())
     return tokens
@@ -689,6 +702,7 @@ def patch_tokens(frames, tokens, units, shifts, constant, scale=1.0, replicate=T
 
 def patch_frames(tokens, frames, units, shifts):
     """patch tokens -> planar frames (B,3,H,W), the mean over the shifted grids"""
+    _patch_shapes(frames, tokens, units, shifts)
     B, _, H, W = frames.shape
     _call('scipnp_patch_frames', _p(tokens, 'tokens'), _p(frames, 'frames'), B, H, W, units, shifts, _stream())
     return frames
