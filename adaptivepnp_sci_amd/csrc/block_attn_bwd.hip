@@ -658,16 +658,17 @@ __device__ __forceinline__ void dbias_pair(const Attn& a, int pair) {
 template <typename T>
 __global__ void __launch_bounds__(256) attn_end_kernel(Attn a, int subs, unsigned joins) {
     if (blockIdx.x >= joins) {
+        if (blockIdx.y) return;
         const int pair = (blockIdx.x - joins) * 4 + (threadIdx.x >> 6);
         if (pair < a.nbuckets * a.Hq) dbias_pair(a, pair);
         return;
     }
-    const unsigned parts = (2 * KB * (a.D / 4) + 255) / 256, x = blockIdx.x / parts;
+    const unsigned x = blockIdx.x;
     const int sub = x % subs, j = x / subs % a.nb, bh = x / subs / a.nb, hk = bh % a.Hk, b = bh / a.Hk;
     const int* const cs = a.chunk_start + (size_t)bh * (a.nb + 1);
     const int c0 = cs[j], n = cs[j + 1] - c0;
     if (n == 1) return;
-    const int per = a.D / 4, i = blockIdx.x % parts * 256 + threadIdx.x, which = i / (KB * per), k = i / per % KB, d = 4 * (i % per);
+    const int per = a.D / 4, i = blockIdx.y * 256 + threadIdx.x, which = i / (KB * per), k = i / per % KB, d = 4 * (i % per);
     const int key = j * a.block + sub * KB + k;
     if (which > 1 || key >= a.Lk) return;
     f32x4a s = {0.f, 0.f, 0.f, 0.f};
@@ -759,8 +760,8 @@ static int bwd_run(const Attn& p, const BwdPlan& bp, hipStream_t st) {
     else rc = p.D <= 32 ? bwd_launch<T, 32>(p, bp, st) : p.D <= 64 ? bwd_launch<T, 64>(p, bp, st)
                  : p.D <= 96 ? bwd_launch<T, 96>(p, bp, st) : bwd_launch<T, 128>(p, bp, st);
     if (rc) return rc;
-    const unsigned joins = (unsigned)(p.nb * bp.subs) * (unsigned)(p.B * p.Hk) * (unsigned)((2 * KB * (p.D / 4) + 255) / 256);
-    attn_end_kernel<T><<<joins + (p.dbias ? (p.nbuckets * p.Hq + 3) / 4 : 0), 256, 0, st>>>(p, bp.subs, joins);
+    const unsigned joins = (unsigned)(p.nb * bp.subs) * (unsigned)(p.B * p.Hk), parts = (unsigned)((2 * KB * (p.D / 4) + 255) / 256);
+    attn_end_kernel<T><<<dim3(joins + (p.dbias ? (p.nbuckets * p.Hq + 3) / 4 : 0), parts), 256, 0, st>>>(p, bp.subs, joins);
     return launch_status("scipnp_block_attn_backward");
 }
 

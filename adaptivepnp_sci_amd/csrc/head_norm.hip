@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(256) head_norm_kernel(HeadNorm a) {
     const NormLds s = norm_lds(a, lds);
     const int l = threadIdx.x % LPR, slot0 = threadIdx.x / LPR;
     constexpr int RPI = 256 / LPR;                        // rows per pass of the workgroup
-    const long long tokens = (long long)a.B * a.L, t0 = (long long)blockIdx.x * a.TT;
+    const long long tokens = (long long)a.B * a.L, t0 = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * a.TT;
+    if (t0 >= tokens) return;                             // (uniform; the grid's last row)
     const int nt = (int)min((long long)a.TT, tokens - t0);
     const int nl = a.D >> 3, nr = a.rot >> 3, half = a.rot >> 1;
     const bool on = l < nl, turned = l < nr;
@@ -329,7 +330,7 @@ static HeadNorm head_norm_params(const scipnp_head_norm_args* a) {
 }
 
 template <int LPR>
-static void head_norm_launch(const HeadNorm& p, int dtype, bool backward, unsigned grid, hipStream_t st) {
+static void head_norm_launch(const HeadNorm& p, int dtype, bool backward, dim3 grid, hipStream_t st) {
     size_t lds = (size_t)p.TT * (sizeof(Token) + (p.rot / 2) * sizeof(double2));
     if (backward) {
         const size_t red = (size_t)(256 / LPR) * p.D * sizeof(double);
@@ -341,7 +342,7 @@ static void head_norm_launch(const HeadNorm& p, int dtype, bool backward, unsign
         else head_norm_kernel<float, LPR><<<grid, 256, lds, st>>>(p);
     }
 }
-static void head_norm_dispatch(int lpr, const HeadNorm& p, int dtype, bool backward, unsigned grid, hipStream_t st) {
+static void head_norm_dispatch(int lpr, const HeadNorm& p, int dtype, bool backward, dim3 grid, hipStream_t st) {
     switch (lpr) {
         case 1: head_norm_launch<1>(p, dtype, backward, grid, st); break;
         case 2: head_norm_launch<2>(p, dtype, backward, grid, st); break;
@@ -364,7 +365,9 @@ int scipnp_head_norm_rotate(const scipnp_head_norm_args* a, scipnp_stream_t s) {
     const int lpr = head_norm_lpr(a->D);
     p.TT = head_norm_tokens(a, lpr);
     const long long tiles = ((long long)a->B * a->L + p.TT - 1) / p.TT;
-    head_norm_dispatch(lpr, p, a->dtype, false, (unsigned)tiles, (hipStream_t)s);
+    // (a dimension of the grid holds 2^32 threads: 2^24 workgroups, of which 2^28 tokens of one small head are too many)
+    const long long row = tiles < (1 << 22) ? tiles : 1 << 22;
+    head_norm_dispatch(lpr, p, a->dtype, false, dim3((unsigned)row, (unsigned)((tiles + row - 1) / row)), (hipStream_t)s);
     return launch_status("scipnp_head_norm_rotate");
 }
 
@@ -383,7 +386,7 @@ int scipnp_head_norm_rotate_backward(const scipnp_head_norm_args* a, scipnp_stre
     p.TT = head_norm_tokens(a, lpr);
     p.part = (double*)a->workspace;
     const int n = head_norm_bwd_groups(a);
-    head_norm_dispatch(lpr, p, a->dtype, true, (unsigned)n, (hipStream_t)s);
+    head_norm_dispatch(lpr, p, a->dtype, true, dim3((unsigned)n), (hipStream_t)s);
     head_norm_dw_kernel<<<(2 * a->D + 3) / 4, 256, 0, (hipStream_t)s>>>(p.part, a->dwq, a->dwk, n, a->D);
     return launch_status("scipnp_head_norm_rotate_backward");
 }

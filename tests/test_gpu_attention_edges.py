@@ -251,3 +251,53 @@ def test_results_beside_autograd(A):
     with torch.inference_mode():
         t = torch.zeros(1, 64, 2, 64, device='cuda')
     assert A.block_attention(q, k, k, sel, query_block=16, out=t) is t and torch.equal(t, results[3])
+
+
+# ------------------------------------------------------------------ grids past 2^24 workgroups
+def room(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f'{gib} GiB of free memory needed')
+
+
+def test_a_norm_of_more_tokens_than_a_row_of_the_grid(A):
+    """2^28 tokens and a few, one head of 8"""
+    room(12)
+    L = (1 << 28) + 5
+    x = torch.full((1, L, 1, 8), 7.0, dtype=torch.bfloat16, device='cuda')
+    w, turns = torch.arange(1.0, 9.0, device='cuda'), A.rotary_turns(8, device='cuda')
+    at = [0, 1, (1 << 26) - 1, 1 << 26, (1 << 28) - 1, 1 << 28, L - 1]
+    gen = torch.Generator().manual_seed(1)
+    rows = randn(gen, 1, len(at), 1, 8, dtype=torch.bfloat16).cuda()
+    x[:, at] = rows
+    pos = torch.tensor([at], dtype=torch.int32, device='cuda')
+    want = A.head_norm_rotate(rows, None, w, None, turns, pos)[0]
+    A.head_norm_rotate(x, None, w, None, turns, out_q=x)
+    assert torch.equal(x[:, at], want) and not (x[0, -1000:-5] == 7).all(-1).any()
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_gradients_of_more_blocks_than_a_row_of_the_grid(A):
+    """2^20 blocks of 64 keys and a few, 128 wide: 16 workgroups each join a block's chunks"""
+    room(150)
+    B, Lk, D, T = 32, (1 << 21) + 64, 128, torch.bfloat16
+    gen = torch.Generator().manual_seed(2)
+    k0, v0 = randn(gen, 1, 64, 1, D, dtype=T).cuda(), randn(gen, 1, 64, 1, D, dtype=T).cuda()
+    k, v = torch.zeros(1, Lk, 1, D, dtype=T, device='cuda'), torch.zeros(1, Lk, 1, D, dtype=T, device='cuda')
+    k[:, -64:], v[:, -64:] = k0, v0
+    q, g = randn(gen, B, 1, 1, D, dtype=T).cuda(), randn(gen, B, 1, 1, D, dtype=T).cuda()
+    how = dict(block=64, query_block=1)
+
+    def grads(k, v, last):
+        sel = torch.full((B, 1, 1, 1), last, dtype=torch.int32, device='cuda')
+        args = (q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), sel)
+        saved = A.block_attention(*args, save=True, **how)[1]
+        return A.block_attention_backward(g, *args, saved, **how)[:3]
+    want = grads(k0, v0, 0)
+    got = grads(k, v, Lk // 64 - 1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][:, -64:], want[1]) and torch.equal(got[2][:, -64:], want[2])
+    for t in got[1:]:
+        assert not any(t[b, i:i + (1 << 19)].any() for b in range(B) for i in range(0, Lk - 64, 1 << 19) if i + (1 << 19) <= Lk - 64)
+    del got, t
+    torch.cuda.empty_cache()
