@@ -301,3 +301,25 @@ def test_gradients_of_more_blocks_than_a_row_of_the_grid(A):
         assert not any(t[b, i:i + (1 << 19)].any() for b in range(B) for i in range(0, Lk - 64, 1 << 19) if i + (1 << 19) <= Lk - 64)
     del got, t
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ views
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('Lq,Lk,Hq,Hk,D,qb', [(190, 190, 4, 2, 40, 16), (150, 150, 8, 2, 128, 16), (3, 1500, 4, 1, 64, 1), (70, 70, 1, 1, 48, 64)])
+def test_a_strided_result_holds_the_bits_of_a_tight_one(A, Lq, Lk, Hq, Hk, D, qb, dt):
+    """columns and heads of a wider tensor, and (B, H, L, D) storage: every row in its place, nothing beside it"""
+    gen, T = torch.Generator().manual_seed(Lq + D), DT[dt]
+    q, k, v = randn(gen, 2, Lq, Hq, D, dtype=T).cuda(), randn(gen, 2, Lk, Hk, D, dtype=T).cuda(), randn(gen, 2, Lk, Hk, D, dtype=T).cuda()
+    sel = every_block(2, Hk, Lq, Lk, qb).cuda()
+    how = dict(block=64, query_block=qb, causal=True, bucket_of=A.bucket_table(8, 20, False, device='cuda'), bias=randn(gen, 8, Hq).cuda())
+    for save in (False, True):
+        want = A.block_attention(q, k, v, sel, save=save, **how)
+        want = want[0] if save else want
+        assert want.float().abs().amax() > 0
+        wide = torch.full((2, Lq, Hq + 2, 2 * D), 3.0, dtype=T).cuda()
+        A.block_attention(q, k, v, sel, out=wide[:, :, 1:-1, :D], save=save, **how)
+        assert torch.equal(wide[:, :, 1:-1, :D], want)
+        assert (wide[..., D:] == 3).all() and (wide[:, :, [0, -1]] == 3).all()
+        heads = torch.full((2, Hq, Lq + 1, D), 3.0, dtype=T).cuda()
+        A.block_attention(q, k, v, sel, out=heads.transpose(1, 2)[:, :Lq], save=save, **how)
+        assert torch.equal(heads.transpose(1, 2)[:, :Lq], want) and (heads[:, :, Lq] == 3).all()
