@@ -90,7 +90,7 @@ def head_norm_rotate(q, k=None, wq=None, wk=None, turns=None, positions=None, fi
                      out_v=None, slots=None):
     """(q', k'): every head normalised by its root mean square, times the weight wq / wk (D,), its first 2 * turns.numel() dimensions
     turned by the token's position (positions (B, L) int32, None: first + index); pair i is dimensions i and i + turns.numel().
-    Computed in fp64 and rounded once.  With out_k (and v, out_v) the keys (and values, unchanged) go there; with slots (B, L) int32
+    Computed in fp64 and rounded at the end (bfloat16 by way of float32).  With out_k (and v, out_v) the keys (and values, unchanged) go there; with slots (B, L) int32
     to row slots[b, l] of it -- a cache (B, Lmax, Hk, D).  A slot outside the cache drops the row; two tokens of a sequence with the
     same slot leave either.  out_q / out_k / out_v may be q / k / v themselves; results that share memory in another way are refused."""
     return (_bound or _bind()).head_norm_rotate(q, k, wq, wk, turns, positions, first, eps, out_q, out_k, v, out_v, slots)

@@ -15,6 +15,7 @@
 //   fp32, 48 wide, 131072 tokens, 16 blocks of 64: 242 us, 106 TFLOP/s against 133; four workgroups a CU are a round of three and one of one.
 //   bf16, 128 wide, one token of 16 sequences, 64 blocks of 64: 48 us + 4.8 of the join, 5.1 TB/s of the keys and values read.
 //   Workgroups in contiguous eighths a die: 73.5 us at 2 x 4096 bf16 tokens, 16 heads of 64, in turn over the dies 83.9.
+#include <type_traits>
 #include "block_attn.hpp"
 
 namespace scipnp {
@@ -90,10 +91,6 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
     ko.init(rw, lane, ks, a.D);
     vo.init(rw, lane, vs, a.D);
     __syncthreads();
-    // a bias of this key head masks (uniform; few tables do): its keys' scores are replaced, like those behind the last visible key
-    bool masks = false;
-    for (int i = lane; i < a.nbuckets * a.G; i += 64) masks |= bias.tbl[i] == -INFINITY;
-    masks = __ballot(masks) != 0;
 
     const int tpb = a.block / KT, ntiles = __builtin_amdgcn_readfirstlane(*nlist);
     const int per = (ntiles + a.splits - 1) / a.splits, t_begin = part * per, count = max(0, min(ntiles, t_begin + per) - t_begin);
@@ -125,12 +122,13 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
     Acc<T, DP> sums;
     float m, l;
     f32x16a o[NB];
-    // One pass, and a careful second one where the first left a sum that is no number: an infinity or a NaN among the values meets weights of
-    // zero (masked keys) and parts of a weight that are zero or negative, and 0 x inf is none.  The second pass has zeros in their
-    // place; they come behind it, to the rows that see their keys.  (The test costs 16 operations a column block; a look at the values of
-    // every masked tile costs a tenth of the tile.)
-    bool careful = false;
-    for (;; careful = true) {
+    // One pass, and a careful second one where the first left a sum that is no number.  An infinity or a NaN among the values meets weights of
+    // zero (masked keys) and parts of a weight that are zero or negative, and 0 x inf is none: the second pass has zeros in their
+    // place; they come behind it, to the rows that see their keys.  A score that is no number stays none when a bias of -infinity masks it:
+    // the second pass replaces it.  (What the first pass costs for this is its test, 16 operations a column block.)
+    bool masks = false;                                   // a bias of this key head masks (uniform)
+    auto pass = [&](auto second) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(second)::value;
     sums.zero();
     m = -INFINITY, l = 0.f;
     blk = t_begin / tpb, off = (t_begin - blk * tpb) * KT;
@@ -150,11 +148,9 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
         }
         const char* const kt = smem + buf * C::BYTES;
         char* const v_at = smem + (ONE_V ? 2 : 2 + buf) * C::BYTES;
-        if constexpr (!ONE_V) {
-            if (careful) {
-                scrub<T, DP, RW>(v_at, rw, lane);
-                dma_wait<RW>();
-            }
+        if constexpr (CAREFUL && !ONE_V) {
+            scrub<T, DP, RW>(v_at, rw, lane);
+            dma_wait<RW>();
         }
         // (a wave with products to issue goes before one in its softmax: 73.6 -> 69.5 us in training at 2 x 4096 tokens, 16 heads of 64)
         __builtin_amdgcn_s_setprio(1);
@@ -164,18 +160,17 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
         if constexpr (LEAN) vt.at(v_at, lane);
         else vt.read(v_at, lane);
         const int dist = a.nbuckets ? tile_distance(a, range, cur, a.k_pos ? kp : nullptr, lane) : 0;
-        const bool masked = masks || cur + KT - 1 > min_lim;
+        const bool masked = cur + KT - 1 > min_lim;
         float c = a.scale2, add = 0.f;
         if (dist >= 0 && a.nbuckets) add = !LEAN && dist == 0 ? bias_lo : !LEAN && dist == far ? bias_hi : bias.tbl[bias.lut[dist] * a.G + gl];
-        if (dist < 0 || masked || c < 0.f) {              // the scores one by one
+        if (dist < 0 || masked || c < 0.f || (CAREFUL && masks)) {              // the scores one by one
             if (dist < 0) {
                 constexpr int N = LEAN ? 8 : 16;          // (half of them at a time takes fewer registers)
 #pragma unroll
                 for (int r0 = 0; r0 < 16; r0 += N) {
                     float x[N];
                     tile_bias(a, bias, cur, a.k_pos ? kp : nullptr, qp, gl, hi, x, r0);
-                    // (a bias that masks, plus a score that is no number, would still be none)
-                    if (masks)
+                    if constexpr (CAREFUL)
 #pragma unroll
                         for (int r = 0; r < N; ++r) s[r0 + r] = x[r] == -INFINITY ? 0.f : s[r0 + r];
 #pragma unroll
@@ -183,7 +178,7 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
                     if constexpr (LEAN) __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
-                if (masks)
+                if constexpr (CAREFUL)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = add == -INFINITY ? 0.f : s[r];
 #pragma unroll
@@ -220,7 +215,7 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
         // enters every score's gradient, and the sums of dbias cancel down to its error
         if constexpr (ONE_V) {
             dma_wait_but<DmaOffsets<T, DP, RW>::N>(t + 1 < count);
-            if (careful) {
+            if constexpr (CAREFUL) {
                 scrub<T, DP, RW>(v_at, rw, lane);
                 dma_wait<RW>();
             }
@@ -238,24 +233,33 @@ __global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW
     for (int t = count; t < trips; ++t) {                 // (the other sets' barriers)
         dma_wait<RW>();
         if constexpr (ONE_V) dma_wait<RW>();
-        if (careful) dma_wait<RW>();
+        if constexpr (CAREFUL) dma_wait<RW>();
     }
     l += __shfl_xor(l, 32, 64);
     sums.blocks(o);
-    if (careful) break;
-    float none = 0.f;
+    };
+    pass(std::false_type{});
+    bool careful;
+    {
+        float none[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int db = 0; db < NB; ++db)
+        for (int db = 0; db < NB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) none = fmaf(o[db][r], 0.f, none);
-    bool again = __ballot(live && none != 0.f && l - l == 0.f) != 0;          // (a row with a score that is no number is none in any case)
-    if constexpr (RW > 1) {                               // waves that share tiles go through them together
-        if (again && lane == 0) longest[1] = 1;
-        __syncthreads();
-        again = __builtin_amdgcn_readfirstlane(longest[1]) != 0;
+            for (int r = 0; r < 16; ++r) none[r & 3] = fmaf(o[db][r], 0.f, none[r & 3]);
+        const bool number = l - l == 0.f;                 // (if not, the row is none unless masked keys made it so)
+        careful = __ballot(live && (!number || (none[0] + none[1]) + (none[2] + none[3]) != 0.f)) != 0;
+        if (careful) {
+            for (int i = lane; i < a.nbuckets * a.G; i += 64) masks |= bias.tbl[i] == -INFINITY;
+            masks = __ballot(masks) != 0;
+            careful = masks || __ballot(live && number && (none[0] + none[1]) + (none[2] + none[3]) != 0.f) != 0;
+        }
+        if constexpr (RW > 1) {                           // waves that share tiles go through them together
+            if (careful && lane == 0) longest[1] = 1;
+            __syncthreads();
+            careful = __builtin_amdgcn_readfirstlane(longest[1]) != 0;
+        }
     }
-    if (!again) break;
-    }
+    if (careful) pass(std::true_type{});
     const Attn& z = late_args();                          // (what only the end needs is read again there: the loop's scalars fit the registers)
     if constexpr (LEAN) {                                 // (the row's place as well: no register holds it through the loop)
         int x = li;

@@ -2,7 +2,7 @@
 //   n = x * r * w,  r = 1 / sqrt(mean(x^2) + eps);   y_i = n_i c - n_{i+h} s,  y_{i+h} = n_{i+h} c + n_i s   (h = rot / 2)
 //   g = the same rotation by the opposite angle of dy;  dw = sum g x r;  dx = r (g w - x r mean(g w x r))
 //
-// Everything between the load and the store is fp64 and rounded once: a query's last bit can cross a border of the block selection
+// Everything between the load and the store is fp64 and rounded at the end (bf16: by way of fp32, half a step and 2^-25 off): a query's last bit can cross a border of the block selection
 // that follows, and the keys of a cache must not depend on which call wrote them.  The kernel reads and writes each element once and
 // costs about 8 fp64 operations per element against 4 bytes of traffic in bf16: 16384 tokens of 40 bf16 heads of 128 take 76 us, 4.4
 // TB/s (a copy reaches 5.2); their arithmetic alone would take 38.  In fp32, 131072 tokens of 8 heads of 48: 89 us forward (4.5 TB/s),
@@ -311,7 +311,8 @@ static int head_norm_lpr(int D) { int l = 1; while (l * 8 < D) l <<= 1; return l
 static int head_norm_bwd_groups(const scipnp_head_norm_args* a) {
     const int tt = head_norm_tokens(a, head_norm_lpr(a->D));
     const long long tiles = ((long long)a->B * a->L + tt - 1) / tt;
-    // three workgroups a CU, as many as its registers hold (four: a second round a third full, 164 + 7 instead of 139 + 6 us), each with its
+    // three workgroups a CU, as many as the registers hold (149 to 165 in every form of the kernel; four: a second round a third full, 164 + 7
+    // instead of 139 + 6 us at 131072 fp32 tokens of 8 heads of 48), each with its
     // share of dw
     return (int)(tiles < 768 ? tiles : 768);
 }

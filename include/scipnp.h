@@ -714,7 +714,7 @@ int scipnp_bilinear_up2_bwd_c8(const float* d_up_c8, float* d_in, int E, int h, 
 
 /* norm of every head with its learned weight, and the rotation by the token's position, one pass:
  *   n = x / sqrt(mean(x^2) + eps) * w;  (n_i, n_{i+rot/2}) turned by positions * turns[i] (turns of the circle per position, fp64)
- * computed in fp64 and rounded once.  k / v may be NULL; v rows are copied.  slots (B, L) int32: the row of out_k / out_v that
+ * computed in fp64 and rounded at the end (bf16 by way of fp32).  k / v may be NULL; v rows are copied.  slots (B, L) int32: the row of out_k / out_v that
  * token l goes to (a cache; NULL: row l); a slot outside [0, Lout) drops the row.  positions (B, L) int32, NULL: first + l.
  * backward: dx of x (in `out_*`), dw fp32 from the gradients g_q / g_k of the rotated heads (v, slots not used). */
 typedef struct {
@@ -759,7 +759,8 @@ int scipnp_select_blocks(const scipnp_select_args* a, scipnp_stream_t s);
  * causal: keys behind the query's position are masked.  bias fp32 (num_buckets, Hq) (NULL: none), bucket_of int32
  * (2 * max_distance + 1), q_pos (B, Lq) / k_pos (B, Lk) int32 (NULL: the key positions of query and key).  A row without a key:
  * zeros, lse = -inf.  zero_rest: rows of out behind qlen are set to zero (0: left as they are).  lse
- * fp32 (B, Hq, Lq), what its rounding left in lse_rest, and out32 fp32 (B, Lq, Hq, D) (the unrounded result) are written when given;
+ * fp32 (B, Hq, Lq), what its rounding left in lse_rest, and out32 fp32 (B, Lq, Hq, D) (the unrounded result) are written when given (rows
+ * behind qlen are not);
  * the backward pass reads them.  backward: dq, dk, dv in dtype, dbias fp32; every row is written (zeros behind qlen / klen). */
 typedef struct {
     size_t struct_size;                 /* = sizeof(scipnp_block_attn_args) */

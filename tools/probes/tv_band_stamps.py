@@ -19,7 +19,7 @@ for (C_, M, N) in ((32, 128, 128), (8, 256, 256)):
     for _ in range(20):
         ops.tv_chambolle(x, b, -1.0, out, plan, 0.1, kernel=4)
     torch.cuda.synchronize()
-    # ONE stamped launch into a fresh buffer (scalar stores of several launches to the same words do not land in order)
+    # ONE stamped launch into a fresh buffer: the stamps are of that launch alone
     plan.stop_iter = torch.zeros(64 + 2 * 2 * 64 + 64, dtype=torch.int32, device=dev)      # [0,64): stop iterations; then 2 x 64 stamps
     torch.cuda.synchronize()
     ops.tv_chambolle(x, b, -1.0, out, plan, 0.1, kernel=4)
