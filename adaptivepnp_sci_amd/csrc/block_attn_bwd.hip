@@ -357,8 +357,8 @@ struct DkvCfg {
     static_assert(JOIN <= MAIN, "the join reuses the tiles");
     static constexpr int LIST = 1032;                     // query groups of a chunk
 };
-// bf16: the transposed rows are read early, under the vector work, up to 64 wide (103 us, late 106).  96 wide they would leave one wave a
-// SIMD; read late, there are two (the whole backward pass of 131072 rows: 376 us instead of 497)
+// bf16: the transposed rows are read behind the vector work.  Early, under it, they would leave one wave a SIMD at 96 columns (the whole
+// backward pass of 131072 rows: 497 us instead of 376, then) and gain nothing at 64 (283 us both ways)
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) block_attn_dkv_kernel(Attn a, int subs, unsigned magic_r, unsigned magic_g) {
@@ -366,7 +366,6 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) 
     using C = DkvCfg<T, DP>;
     using Frag = typename Mat<T>::Frag;
     constexpr int NB = (DP + 31) / 32, LC = DmaTile<T, DP>::LC, PIECES = DmaTile<T, DP>::PIECES, MINE = (PIECES + 1) / 2, BYTES = DmaTile<T, DP>::BYTES;
-    constexpr bool LATE = DP > 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // (chunks in turn over the XCDs: the last of a sequence and key head's slots are empty)
     const int sub = blockIdx.x % subs, c = blockIdx.x / subs % a.max_chunks, bh = blockIdx.x / subs / a.max_chunks, hk = bh % a.Hk, b = bh / a.Hk;
@@ -542,10 +541,6 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) 
         f32x16a dp = dma_rows<T, DP>(at + BYTES, vf, lane);
         __builtin_amdgcn_s_setprio(0);
         ColTile<T, DP> gc, qc;
-        if constexpr (!LATE) {
-            gc.read(at + BYTES, lane);
-            qc.read(at, lane);
-        }
         const float* const mine = info + 4 * hi;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -590,9 +585,9 @@ __global__ void __launch_bounds__(256, DP > (sizeof(T) == 2 ? 96 : 64) ? 1 : 2) 
             }
         }
         __builtin_amdgcn_s_setprio(1);
-        if constexpr (LATE) gc.read(at + BYTES, lane);
+        gc.read(at + BYTES, lane);
         gc.mma(Weights<T, 2>(s), vacc);                   // (bf16: P and dS in 16 bits, as in the pass for dQ; with 8 the gradients were 1.4 x as far off)
-        if constexpr (LATE) qc.read(at, lane);
+        qc.read(at, lane);
         qc.mma(Weights<T, 2>(dp), kacc);
         __builtin_amdgcn_s_setprio(0);
     }
