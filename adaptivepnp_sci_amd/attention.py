@@ -90,8 +90,8 @@ def head_norm_rotate(q, k=None, wq=None, wk=None, turns=None, positions=None, fi
                      out_v=None, slots=None):
     """(q', k'): every head normalised by its root mean square, times the weight wq / wk (D,), its first 2 * turns.numel() dimensions
     turned by the token's position (positions (B, L) int32, None: first + index); pair i is dimensions i and i + turns.numel().
-    Computed in fp64 and rounded at the end (bfloat16 by way of float32).  With out_k (and v, out_v) the keys (and values, unchanged) go there; with slots (B, L) int32
-    to row slots[b, l] of it -- a cache (B, Lmax, Hk, D).  A slot outside the cache drops the row; two tokens of a sequence with the
+    Computed in fp64 and rounded at the end (bfloat16 by way of float32).  With out_k (and v, out_v) the keys (and values, unchanged) go
+    there; with slots (B, L) int32 to row slots[b, l] of it -- a cache (B, Lmax, Hk, D).  A slot outside the cache drops the row; two tokens of a sequence with the
     same slot leave either.  out_q / out_k / out_v may be q / k / v themselves; results that share memory in another way are refused."""
     return (_bound or _bind()).head_norm_rotate(q, k, wq, wk, turns, positions, first, eps, out_q, out_k, v, out_v, slots)
 
@@ -125,8 +125,9 @@ def block_attention(q, k, v, sel, block=64, query_block=64, scale=None, causal=F
     name the positions (None: the key positions), e.g. the frame of each token of a video; differences must fit 32 bits.  A bias below
     -1e30 (-inf, a type's lowest value) masks its keys.  A query without a visible key gives zeros; what a key holds that a query does
     not see -- NaN, infinity -- does not reach it.  Rows behind qlen are zeros, or left as they were in a given `out` (q itself, or memory of its own).
-    save=True returns (out, saved) for block_attention_backward, saved = (log-sum-exp (B, Hq, Lq), fp32 result, what the first was rounded by); bfloat16 probabilities are then multiplied whole, not rounded, so that
-    the saved fp32 result carries the gradient (out is the same up to its rounding)."""
+    bfloat16 probabilities go into the product with v in two numbers, off by 2^-16.  save=True returns (out, saved) for
+    block_attention_backward, saved = (log-sum-exp (B, Hq, Lq), fp32 result, what the first was rounded by; rows behind qlen are not written);
+    the probabilities are then multiplied whole, in three, because the saved result carries the gradient: out can differ by a rounding."""
     return (_bound or _bind()).block_attention(q, k, v, sel, block, query_block, scale, causal, qlen, klen, bucket_of, bias, q_pos, k_pos, out, save)
 
 

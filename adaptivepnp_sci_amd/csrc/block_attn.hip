@@ -6,26 +6,28 @@
 // where the tile has one bucket and no mask.  The maximum m is moved only when a tile exceeds it by 2^8: until then p <= 2^8, which
 // costs no accuracy in floating point, and the accumulators are not rescaled.
 //
-// What it is bound by, measured:
-//   bf16, 128 wide, 16384 queries of 32 heads over 8 key heads, groups of 16 queries, 16 blocks of 64 each: 381 us, 700 TFLOP/s against 1150
-//     of a large matrix product.  A tile is 512 cycles of matrix work and about 125 vector instructions, 16 of them exponentials (700 cycles); three
-//     waves a SIMD (168 registers, 50 KB of LDS a workgroup) overlap the two in part, two waves less (406 us; LDS is busy 17 % of the time
-//     and has no bank conflicts).  Taken out one at a time, of then 490 us with two: the requests for tiles 426, they and the
-//     barriers 387, the second product 440, the exponentials 499.  64 rows a wave: 636 us, the accumulators no longer fit beside the operands.
-//   fp32, 48 wide, 131072 tokens, 16 blocks of 64: 242 us, 106 TFLOP/s against 133; four workgroups a CU are a round of three and one of one.
-//   bf16, 128 wide, one token of 16 sequences, 64 blocks of 64: 48 us + 4.8 of the join, 5.1 TB/s of the keys and values read.
-//   Workgroups in contiguous eighths a die: 73.5 us at 2 x 4096 bf16 tokens, 16 heads of 64, in turn over the dies 83.9.
+// What it is bound by, measured (in a program that has run for a while: the first dozen launches behind a pause take a fifth longer):
+//   bf16, 128 wide, 16384 queries of 32 heads over 8 key heads, groups of 16 queries, 16 blocks of 64 each: 451 us; 590 TFLOP/s of one score and
+//     one value product a pair, 890 of the three it does (P in two parts), against 1150 of a large matrix product.  A tile is 768 cycles of
+//     matrix work and about 190 vector instructions, 16 of them exponentials (one part: 512 and 140, 382 us); three waves a SIMD (168 registers,
+//     50 KB of LDS a workgroup) overlap the two in part.  LDS is busy 18 % of the time and has no bank conflicts.  64 rows a wave
+//     were slower: the accumulators no longer fit beside the operands.
+//   fp32, 48 wide, 131072 tokens, 16 blocks of 64: 237 us, 109 TFLOP/s against 133; four workgroups a CU are a round of three and one of one.
+//     56 wide (the non-local prior, 2 x 147968 tokens): 738 us, 92 TFLOP/s, and 105 with the padding to 64 that it multiplies.
+//   bf16, 128 wide, one token of 16 sequences, 64 blocks of 64: 48 us + 4.9 of the join, 5.6 TB/s of the keys and values read.
+//   fp32 of that: 166 us, 3.2 TB/s; the tiles of 128 columns leave LDS for two waves a CU.
+//   Workgroups in contiguous eighths a die were an eighth faster at 2 x 4096 bf16 tokens, 16 heads of 64, than in turn over the dies.
 #include <type_traits>
 #include "block_attn.hpp"
 
 namespace scipnp {
 
-// LEAN, bf16 of 96 and 128 columns and two waves a pair of tiles: three waves a SIMD instead of two (189 instead of 197 us at 8192 queries of
-// 32 heads of 96 in groups of 16, 464 instead of 469 for the first case above).  V is read behind the softmax, 64 columns at a time, which
+// LEAN, bf16 of 96 and 128 columns and two waves a pair of tiles: three waves a SIMD instead of two (191 instead of 199 us at 8192 queries of
+// 32 heads of 96 in groups of 16, 452 instead of 465 for the first case above).  V is read behind the softmax, 64 columns at a time, which
 // saves the registers, and there is one buffer of V, which saves the LDS: it is asked for when its tile's scores begin.  Not where
 // there is no third workgroup for a CU (52 us instead of 49 at 4096 queries of 16 heads of 128), nor with P in three parts of 128 columns (30
-// registers would go to scratch in the loop), nor for one wave a set (LDS), nor for four (101 us instead of 95 at 8192 queries of 16 heads of 96 in
-// groups of 64).
+// registers would go to scratch in the loop), nor for one wave a set (LDS), nor for four (101 us instead of 96 at 8192 queries of 16 heads of 96 in
+// groups of 64, 119 instead of 109 at 128 wide).
 template <typename T, int DP, int RW, bool SAVE>
 constexpr bool can_be_lean() { return sizeof(T) == 2 && DP > 64 && RW == 2 && !(SAVE && DP == 128); }
 template <typename T, int DP, int RW, bool LEAN>
@@ -39,7 +41,8 @@ struct FwdCfg {
 // A workgroup holds `sets` sets of RW waves, each with work of its own: four waves a workgroup land one on each SIMD of a CU, where
 // workgroups of one or two leave some SIMDs with three waves and some with one.
 template <typename T, int DP, int RW, bool SAVE, bool LEAN>          // SAVE: out32 wanted (a training pass)
-__global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW > 1) ? 3 : 2) block_attn_kernel(Attn a, int sets, int set_bytes) {
+__global__ void __launch_bounds__(256, LEAN || (sizeof(T) == 4 && DP == 64 && RW > 1) ? 3 : 2)   // (fp32 of 64: 168 registers, a few spilt outside the loop)
+block_attn_kernel(Attn a, int sets, int set_bytes) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using C = FwdCfg<T, DP, RW, LEAN>;
     using Frag = typename Mat<T>::Frag;

@@ -6,8 +6,9 @@
 // into chunks of equal length, since a first block is chosen by every group and most blocks by few.
 //
 // Four launches: the selection turned round; dQ, dbias, delta and the chunks; dK and dV; the chunks' sums.  2 x 4096 bf16 tokens, 16
-// heads of 64 over 4 key heads, 16 blocks of 64: 5 + 77 + 102 + 9 us behind a forward pass of 70; 65536 fp32 tokens of 48, one head:
-// 5 + 191 + 311 + 17 behind 133.  (One launch more for each of delta, the chunks and dbias: 350 us instead of 311 for the first.)
+// heads of 64 over 4 key heads, 16 blocks of 64: 5 + 67 + 105 + 10 us behind a forward pass of 59 with 54 % of the pairs
+// live, 280 for the four with all of them; 65536 fp32 tokens of 48, one head: 5 + 177 + 288 + 17 behind 122.  (One launch more for each of delta,
+// the chunks and dbias: an eighth more for the first.)
 #include "block_attn.hpp"
 
 namespace scipnp {
@@ -106,9 +107,9 @@ __device__ __forceinline__ void plan_chunks(const Attn& a, int bh, int R, int CH
 }
 
 // ---- dQ, dbias: the forward's sets of waves and tiles.  The bias sums: one LDS word a bucket and row, the two ends (where
-// most tiles lie) in registers.  Three products a tile and vector work of twice their length: 77 us for 131072 bf16 rows of 64 with
-// about 1000 keys each (three waves a SIMD; two, with the transposed keys read before the vector work: 98; 128 wide two waves instead of one: 72 us less),
-// 191 us for 65536 x 1024 of 48 wide fp32 (101 TFLOP/s against 133)
+// most tiles lie) in registers.  Three products a tile and vector work of twice their length: 67 us for 131072 bf16 rows of 64, 54 % of
+// them live, with about 1000 keys each (three waves a SIMD; two, with the transposed keys read before the vector work, were a quarter slower; 128 wide two
+// waves instead of one: 72 us less), 177 us for 65536 x 1024 of 48 wide fp32 (109 TFLOP/s against 133)
 template <typename T, int DP>
 struct DqCfg {
     static constexpr int TILE = 2 * DmaTile<T, DP>::BYTES;                    // K and V
@@ -343,10 +344,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (DP > 64 ? 2 : 3) : DP >
 // a wave keeps its 32 keys and values in registers (the B operands) and streams rows, which the memory system writes to LDS
 // (global_load ... lds: the rows of a tile may belong to several query groups): S, dP with the rows as A, then dV += dO^T P and
 // dK += Q^T dS with the transposed rows as A and the score registers as B.
-// Bound by the vector work between the products: four products of 32 x 32 take 512 cycles a tile at bf16, 64 wide, the rest about
-// 900, of which the rows' books are a fifth (they were half while every lane divided for its own requests: 447 instead of 350 us in
-// fp32).  Chunks of a 2048th of all rows: larger ones leave CUs idle at the end (113 us instead of 103 at a 1024th), smaller ones pay
-// for their beginnings (110 at a 4096th).
+// Bound by the vector work between the products: the products of 32 x 32, the second ones in two parts, take 768 cycles a tile at bf16, 64
+// wide, the rest about 1000, of which the rows' books are a fifth (they were half while every lane divided for its own requests: 447
+// instead of 350 us in fp32, then).  Chunks of a 2048th of all rows: larger ones leave CUs idle at the end (the whole backward pass at 2 x 4096 tokens
+// of 64 286 us instead of 280 at a 1024th, 1292 instead of 1200 in fp32 at 56 wide; 555 instead of 580 at 128), smaller ones pay for their
+// beginnings (318 at a 4096th).
 // What a row brings besides: its last visible key, delta, log-sum-exp, and its bias where all 64 keys share its bucket.
 template <typename T, int DP>
 struct DkvCfg {

@@ -15,8 +15,8 @@ struct Summary {
 };
 
 // One workgroup per (sequence, block, column tile): a thread owns 16 bytes of a key head's row and every splits-th key of the block,
-// eight loads in flight; the splits are added in LDS in order.  Reads each key once: 16 x 32768 bf16 keys of 8 x 128 in 165 us,
-// 5.9 TB/s less what lies behind the sequences -- the rate of a read of that size.
+// eight loads in flight; the splits are added in LDS in order.  Reads each key once: 16 x 32768 bf16 keys of 8 x 128 in 200 us,
+// 5.4 TB/s (a large read reaches 6.0); 165 us, 5.0 TB/s, where lengths of half to all of them leave 78 % live.  fp32 5.7 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) block_summary_kernel(Summary a) {
     constexpr int E = 16 / sizeof(T);
@@ -237,9 +237,9 @@ __device__ void select_best(const unsigned* keys, int nb, int n, int32_t* out, i
 //   2. the scores of 16 blocks x 16 groups at a time on the fp64 matrix unit (v_mfma_f64_16x16x4_f64: lane -> row lane & 15,
 //      contraction lane >> 4; result register r: row 4 r + (lane >> 4), column lane & 15): a mean key is read once for all groups;
 //   3. a wave chooses the blocks of one group.
-// 16384 bf16 queries of 32 x 128 in groups of 16, 16 of 256 blocks: 54 us, of which the queries take 34 (their 134 MB 26 at the copy
+// 16384 bf16 queries of 32 x 128 in groups of 16, 16 of 256 blocks: 52 us, of which the queries take 34 (their 134 MB 26 at the copy
 // rate), the scores 11 (half the fp64 matrix rate) and the choice 9, one after the other in every workgroup.  2048 fp32 groups of 64 x 48, 16 of
-// 2048 blocks: 40 us, 7 + 23 + 10; half the matrix columns are empty there, eight groups' scores fill the LDS.
+// 2048 blocks: 39 us, 7 + 23 + 10; half the matrix columns are empty there, eight groups' scores fill the LDS.
 typedef double f64x4a __attribute__((ext_vector_type(4)));
 constexpr int SEL_WAVES = 8;
 

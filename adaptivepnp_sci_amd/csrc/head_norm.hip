@@ -2,12 +2,12 @@
 //   n = x * r * w,  r = 1 / sqrt(mean(x^2) + eps);   y_i = n_i c - n_{i+h} s,  y_{i+h} = n_{i+h} c + n_i s   (h = rot / 2)
 //   g = the same rotation by the opposite angle of dy;  dw = sum g x r;  dx = r (g w - x r mean(g w x r))
 //
-// Everything between the load and the store is fp64 and rounded at the end (bf16: by way of fp32, half a step and 2^-25 off): a query's last bit can cross a border of the block selection
-// that follows, and the keys of a cache must not depend on which call wrote them.  The kernel reads and writes each element once and
+// Everything between the load and the store is fp64 and rounded at the end (bf16: by way of fp32, half a step and 2^-25 off): a query's
+// last bit can cross a border of the block selection that follows, and the keys of a cache must not depend on which call wrote them.  The kernel reads and writes each element once and
 // costs about 8 fp64 operations per element against 4 bytes of traffic in bf16: 16384 tokens of 40 bf16 heads of 128 take 76 us, 4.4
-// TB/s (a copy reaches 5.2); their arithmetic alone would take 38.  In fp32, 131072 tokens of 8 heads of 48: 89 us forward (4.5 TB/s),
-// 139 backward (4.3 TB/s) and 6 for the sum of dw over the workgroups.  One token of 16 sequences: 5.7 us, latency.  (Rows asked for while the one
-// before is computed: 121 instead of 99 us, fewer waves fit.)
+// TB/s (a copy reaches 5.2); their arithmetic alone would take 38.  In fp32, 131072 tokens of 8 heads of 48: 83 us forward (4.8 TB/s),
+// 132 backward (4.6 TB/s) and 6 for the sum of dw over the workgroups; backward of the first in bf16 139 (3.6 TB/s), in fp32 196 (5.1).  One
+// token of 16 sequences: 5.8 us, latency.  (Rows asked for while the one before is computed were a fifth slower, fewer waves fit.)
 //
 // A row (one head of one token) is held by LPR = 2^k >= D / 8 lanes; a lane has two chunks of four elements, both halves of its
 // pairs, so the rotation needs no exchange: lane l < rot/8 holds 4l.. and rot/2 + 4l.., the lanes behind it the unrotated rest.
