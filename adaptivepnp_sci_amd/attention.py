@@ -24,6 +24,7 @@ written raises its version counter, so autograd refuses a backward pass that had
 import ctypes as C
 import importlib
 import math
+import re
 
 import torch
 
@@ -43,7 +44,7 @@ def _bind():
         mod = importlib.import_module('._attn_bind', __package__)
     except ImportError as e:
         raise ScipnpError(f'{e}: build it with `make -C adaptivepnp_sci_amd/csrc`') from e
-    if mod.built_for != torch.__version__.split('+')[0]:
+    if mod.built_for != '.'.join(re.findall(r'\d+', torch.__version__)[:3]):          # (the headers know the three numbers)
         raise ScipnpError(f'_attn_bind.so was built for torch {mod.built_for}, this is {torch.__version__}: build it again with `make -C adaptivepnp_sci_amd/csrc`')
     mod.bind(*(C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES), _lib.check, ScipnpError, torch.cuda.current_device,
              getattr(torch._C, '_cuda_getCurrentRawStream', None) or _raw_stream)

@@ -772,6 +772,7 @@ int scipnp_block_attn_backward(const scipnp_block_attn_args* a, scipnp_stream_t 
     if (const int rc = attn_check(a)) return rc;
     SCIPNP_REQUIRE(a->dout && a->dq && a->dk && a->dv && a->lse && a->lse_rest && a->out32, "backward needs dout, dq, dk, dv, lse, lse_rest and out32");
     SCIPNP_REQUIRE(!a->num_buckets || a->dbias, "backward with a bias needs dbias");
+    SCIPNP_REQUIRE((long long)a->num_buckets * a->Hq < (1ll << 24), "too many buckets and query heads");
     SCIPNP_ALIGNED(a->dout); SCIPNP_ALIGNED(a->dq); SCIPNP_ALIGNED(a->dk); SCIPNP_ALIGNED(a->dv); SCIPNP_ALIGNED(a->out32);
     SCIPNP_STRIDES(a->dout_stride, a->dtype);
     const BwdPlan bp = bwd_plan(a);

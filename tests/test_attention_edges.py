@@ -41,6 +41,10 @@ def test_heads_are_counted_in_64_bits(lib):
     a = _lib.BlockAttnArgs(dtype=1, B=1, Lq=1, Lk=64, Hq=1 << 26, Hk=1, D=64, block=64, query_block=1, n_sel=1, scale=1.0, q=P, k=P, v=P, out=P, sel=P,
                            num_buckets=64, max_distance=4, bias=P, bucket_of=P, q_stride=st, k_stride=st, v_stride=st, out_stride=st)
     refused(lib, lib.scipnp_block_attn(C.byref(a), None), 'at most 2048')
+    full = dict(dout=P, dq=P, dk=P, dv=P, lse=P, lse_rest=P, out32=P, dbias=P, dout_stride=st)
+    a = _lib.BlockAttnArgs(dtype=1, B=1, Lq=1, Lk=64, Hq=32 * 40000, Hk=40000, D=64, block=64, query_block=1, n_sel=1, scale=1.0, q=P, k=P, v=P, out=P, sel=P,
+                           num_buckets=64, max_distance=4, bias=P, bucket_of=P, q_stride=st, k_stride=st, v_stride=st, out_stride=st, **full)
+    refused(lib, lib.scipnp_block_attn_backward(C.byref(a), None), 'buckets and query heads')
 
 
 # ------------------------------------------------------------------ results that share memory
@@ -92,6 +96,10 @@ def test_the_libraries_build_without_python(tmp_path):
 
 def test_a_module_of_another_torch_is_refused(monkeypatch):
     from adaptivepnp_sci_amd import attention as A
+    have = A.torch.__version__.split('+')[0]
+    monkeypatch.setattr(A, '_bound', None)
     monkeypatch.setattr(A.torch, '__version__', '1.0.0+other')
     with pytest.raises(_lib.ScipnpError, match='built for torch'):
         A._bind()
+    monkeypatch.setattr(A.torch, '__version__', have + 'a0+git123')           # (a build of the same three numbers)
+    assert A._bind().built_for == have
